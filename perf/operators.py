@@ -130,7 +130,7 @@ def _run_own(state):
 
     case, x = state["case"], state["x"]
     if case["op"] == "pack":
-        return unpack_8bit(*pack_8bit(x), dtype=x.dtype)
+        return unpack_8bit(pack_8bit(x))
     if case["op"].startswith("norm"):
         y = group_norm_2d(x, case["groups"], state["weight"], state["bias"], eps=EPS, activation=case["act"],
                           checkpoint_8bit=case["bits"] == 8)  # fmt: skip
