@@ -16,12 +16,12 @@ class LayerNorm2d(nn.LayerNorm):
 
 
 class Block(nn.Module):
-    def __init__(self, dim, make_conv):
+    def __init__(self, dim, make_conv, make_act=nn.GELU):
         super().__init__()
         self.conv = make_conv(dim)
         self.norm = nn.LayerNorm(dim)
         self.fc1 = nn.Linear(dim, 4 * dim)
-        self.act = nn.GELU()
+        self.act = make_act()
         self.fc2 = nn.Linear(4 * dim, dim)
         self.gamma = nn.Parameter(torch.ones(dim))
 
@@ -37,13 +37,13 @@ def plain_conv(dim):
 
 class ConvNeXtGw8(nn.Module):
     def __init__(self, make_conv=plain_conv, widths=(96, 192, 384, 768), depths=(3, 3, 9, 3), classes=1000,
-                 norm2d=LayerNorm2d):
+                 norm2d=LayerNorm2d, make_act=nn.GELU):
         super().__init__()
         layers = [nn.Conv2d(3, widths[0], 4, stride=4), norm2d(widths[0])]
         for i, (w, d) in enumerate(zip(widths, depths)):
             if i > 0:
                 layers += [norm2d(widths[i - 1]), nn.Conv2d(widths[i - 1], w, 2, stride=2)]
-            layers += [Block(w, make_conv) for _ in range(d)]
+            layers += [Block(w, make_conv, make_act) for _ in range(d)]
         self.features = nn.Sequential(*layers)
         self.norm = nn.LayerNorm(widths[-1])
         self.head = nn.Linear(widths[-1], classes)

@@ -1,0 +1,361 @@
+// Backward of the group norm with an activation of group_norm_2d.hip (NHWC tensors, gfx950).
+//
+//   xhat = (in - mean) * rstd          mean and rstd of the forward pass; in as it was, or its 8-bit form (SPIO_GN_KEPT)
+//   dz = dout * act'(xhat * weight + bias),  g = dz * weight,  m = pixels * C/G
+//   din = rstd * (g - sum_group(g) / m - xhat * sum_group(g * xhat) / m)
+//   dweight[c] = sum dz * xhat,  dbias[c] = sum dz          float32, over images and pixels
+//
+// The group's sums are those of its channels times their weights, so one pair of sums for each image and channel
+// serves all three gradients.  HBM-bound: where an image's slice of channels fits the registers of one workgroup
+// (SPIO_GN_SPLIT 0) input and gradient are read once, and a second launch adds the images' rows of channel sums.  Otherwise
+// the first launch leaves a row of channel sums for every stretch and the pair of each group; the second one reads
+// input and gradient again, and its first workgroups add the rows meanwhile.  Nothing is atomic: every sum is
+// made in the same order always.
+#include "spio_group_norm.h"
+
+#ifndef SPIO_GN_AFFINE
+#define SPIO_GN_AFFINE 1  // the sums over images are wanted
+#endif
+
+namespace {
+
+using namespace gn;
+
+struct Input {  // the norm's input as the backward pass has it
+#if SPIO_GN_KEPT
+    pw_uint2 code;
+    unsigned exponent;
+#else
+    pw::Unit v;
+#endif
+};
+
+struct Chunk {
+    Input x[UN];
+    pw::Unit dy[UN];
+    unsigned off[UN];
+    int pixels;
+    long long first;
+};
+
+template <int POLICY>
+PW_DEVICE void load_chunk(Chunk& c, const void* in, const unsigned char* exponents, const void* dout, const Place& p,
+                          long long pixels) {
+    const long long begin = SPIO_GN_SPLIT ? (long long)p.stretch * SPAN : 0;
+    const long long left = pixels - begin;
+    c.pixels = (int)(left < SPAN ? left : SPAN);
+    c.first = p.image * pixels + begin;
+    constexpr int IN_BYTES = SPIO_GN_KEPT ? 1 : pw::VALUE_BYTES;
+    const pw_rsrc rs_in = pw::buffer(reinterpret_cast<const unsigned char*>(in) + c.first * (C * IN_BYTES),
+                                     (unsigned)c.pixels * (C * IN_BYTES));
+    const pw_rsrc rs_exp = pw::buffer(exponents + c.first * BLOCKS, SPIO_GN_KEPT ? (unsigned)c.pixels * BLOCKS : 0);
+    const pw_rsrc rs_dout = pw::buffer(reinterpret_cast<const unsigned char*>(dout) + c.first * (C * pw::VALUE_BYTES),
+                                       (unsigned)c.pixels * (C * pw::VALUE_BYTES));
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+        const int pixel = p.row + u * ROWS;
+        c.off[u] = p.live ? (unsigned)(pixel * C + p.channel) * pw::VALUE_BYTES : pw::OOB;
+#if SPIO_GN_KEPT
+        c.x[u].code = __builtin_amdgcn_raw_buffer_load_b64(rs_in, p.live ? pixel * C + p.channel : (int)pw::OOB, 0, POLICY);
+        c.x[u].exponent = __builtin_amdgcn_raw_buffer_load_b8(
+            rs_exp, p.live ? pixel * BLOCKS + p.channel / 32 : (int)pw::OOB, 0, 0);
+#else
+        c.x[u].v = pw::load_unit<POLICY>(rs_in, c.off[u]);
+#endif
+        c.dy[u] = pw::load_unit<POLICY>(rs_dout, c.off[u]);
+    }
+}
+
+PW_DEVICE void input_values(float (&x)[8], const Input& in) {
+#if SPIO_GN_KEPT
+    pw::decode(x, in.code, pw::block_step(in.exponent));
+#else
+    pw::unpack(x, in.v);
+#endif
+}
+
+struct Lane {  // a lane's eight channels
+    float w[8], b[8];
+    float mean[KEYS], rstd[KEYS];
+};
+
+PW_DEVICE void load_lane(Lane& l, const float* stats, const float* weight, const float* bias, const Place& p) {
+    if (SPIO_GN_HAS_WEIGHT)
+        load_vector(l.w, weight, p);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l.w[e] = 1.f;
+    if (SPIO_GN_HAS_BIAS && SPIO_ACT)
+        load_vector(l.b, bias, p);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l.b[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) {
+        const int g = p.slice * GS + group_of(p, k);
+        const float* s = stats + ((long long)p.image * GROUPS + (p.live ? g : 0)) * 2;
+        l.mean[k] = s[0];
+        l.rstd[k] = s[1];
+    }
+}
+
+// xhat and dz of a unit (what lies behind the last pixel has dy = 0, and with it dz)
+PW_DEVICE void work(float (&xhat)[8], float (&dz)[8], const Chunk& c, int u, const Lane& l) {
+    float x[8], dy[8];
+    input_values(x, c.x[u]);
+    pw::unpack(dy, c.dy[u]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        xhat[e] = (x[e] - l.mean[e / KEY_CHANNELS]) * l.rstd[e / KEY_CHANNELS];
+        dz[e] = pw::activate_grad(dy[e], __builtin_fmaf(xhat[e], l.w[e], l.b[e]));
+    }
+}
+
+// The chunk's sums of dz and of dz * xhat: [which][channel of the slice] in `red`, and in `row`, those of dz * xhat first.
+constexpr int WIDTH = SUP * 8;
+constexpr int COLUMNS = 2 * WIDTH;
+constexpr int PARTS = THREADS / COLUMNS > 1 ? THREADS / COLUMNS : 1;  // threads that share a column
+constexpr int RED = SUM_ROWS * COLUMNS > PARTS * COLUMNS ? SUM_ROWS * COLUMNS : PARTS * COLUMNS;
+
+PW_DEVICE void channel_sums(const Chunk& c, const Place& p, const Lane& l, float* red, float* row) {
+    float s1[8] = {}, s2[8] = {};
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+        if (p.live && p.row + u * ROWS < c.pixels) {
+            float xhat[8], dz[8];
+            work(xhat, dz, c, u, l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s1[e] += dz[e];
+                s2[e] = __builtin_fmaf(dz[e], xhat[e], s2[e]);
+            }
+        }
+    }
+    if (kFold) {
+#pragma unroll
+        for (int m = SUP; m < 64; m <<= 1)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s1[e] += lane_xor(s1[e], m);
+                s2[e] += lane_xor(s2[e], m);
+            }
+    }
+    if (kFold ? (p.tid & 63) < SUP : p.row < ROWS) {
+        float* to = red + (kFold ? p.tid >> 6 : p.row) * COLUMNS + p.sub * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            to[e] = s1[e];
+            to[WIDTH + e] = s2[e];
+        }
+    }
+    sync();
+    // a column's rows by PARTS threads, then those
+    float sum[(COLUMNS + THREADS - 1) / THREADS];
+#pragma unroll
+    for (int i = 0; i < (COLUMNS + THREADS - 1) / THREADS; ++i) {
+        sum[i] = 0.f;
+        const int col = PARTS > 1 ? p.tid % COLUMNS : p.tid + i * THREADS;
+        const int part = PARTS > 1 ? p.tid / COLUMNS : 0;
+        if (col < COLUMNS && part < PARTS)
+            for (int r = part; r < SUM_ROWS; r += PARTS) sum[i] += red[r * COLUMNS + col];
+    }
+    if (PARTS > 1) {
+        sync();
+        if (p.tid / COLUMNS < PARTS) red[p.tid] = sum[0];
+        sync();
+        if (p.tid < COLUMNS) {
+#pragma unroll
+            for (int q = 1; q < PARTS; ++q) sum[0] += red[q * COLUMNS + p.tid];
+        }
+    }
+    sync();
+#pragma unroll
+    for (int i = 0; i < (COLUMNS + THREADS - 1) / THREADS; ++i) {
+        const int col = p.tid + i * THREADS;
+        if (col < COLUMNS) {
+            red[col] = sum[i];
+            const int channel = p.slice * SLICE + col % WIDTH;
+            if (SPIO_GN_AFFINE && col % WIDTH < SLICE && channel < C) row[(1 - col / WIDTH) * C + channel] = sum[i];
+        }
+    }
+    sync();
+}
+
+// The pairs of sums of the slice's groups, from the channel sums that channel_sums left in `red`.
+PW_DEVICE void group_pairs(const Place& p, const float* red, float* pairs, const float* weight) {
+    constexpr int LANES = group_lanes();
+    const int part = p.tid % LANES;
+    for (int g = p.tid / LANES; g < GS; g += THREADS / LANES) {
+        float a = 0.f, b = 0.f;
+        for (int e = part; e < CG; e += LANES) {
+            const int col = g * CG + e;
+            const int channel = p.slice * SLICE + col;
+            const float w = SPIO_GN_HAS_WEIGHT && channel < C ? weight[channel] : 1.f;
+            a = __builtin_fmaf(red[col], w, a);
+            b = __builtin_fmaf(red[WIDTH + col], w, b);
+        }
+#pragma unroll
+        for (int m = 1; m < LANES; m <<= 1) {
+            a += lane_xor(a, m);
+            b += lane_xor(b, m);
+        }
+        if (part == 0) {
+            pairs[g] = a;
+            pairs[GS + g] = b;
+        }
+    }
+    sync();
+}
+
+PW_DEVICE void apply(const Chunk& c, const Place& p, const Lane& l, void* din, const float* pairs, long long pixels) {
+    const pw_rsrc rs = pw::buffer(reinterpret_cast<unsigned char*>(din) + c.first * (C * pw::VALUE_BYTES),
+                                  (unsigned)c.pixels * (C * pw::VALUE_BYTES));
+    const float count = 1.f / ((float)pixels * CG);
+    float m1[KEYS], m2[KEYS];
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) {
+        const int g = group_of(p, k) < GS ? group_of(p, k) : 0;
+        m1[k] = pairs[g] * count;
+        m2[k] = pairs[GS + g] * count;
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+        float xhat[8], dz[8], dx[8];
+        work(xhat, dz, c, u, l);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = e / KEY_CHANNELS;
+            const float g = SPIO_GN_HAS_WEIGHT ? __builtin_fmaf(dz[e], l.w[e], -m1[k]) : dz[e] - m1[k];
+            dx[e] = l.rstd[k] * __builtin_fmaf(xhat[e], -m2[k], g);
+        }
+        pw::store_unit<pw::STREAM>(rs, c.off[u], pw::pack(dx));
+    }
+}
+
+// sums[i] = sum over `rows` rows of rows[row][i], i < 2 * C: workgroup `block` has 32 columns, THREADS / 32 slices of
+// rows, which meet in LDS.
+PW_DEVICE void add_rows(float* sums, const float* table, long long rows, int block, float* red) {
+    constexpr int PARTS_OF_ROWS = THREADS / 32;
+    const int tid = (int)__builtin_amdgcn_workitem_id_x();
+    const int col = block * 32 + tid % 32, part = tid / 32;
+    float s = 0.f;
+    if (col < 2 * C) {
+        for (long long r = part; r < rows; r += PARTS_OF_ROWS * 16) {
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const long long row = r + i * PARTS_OF_ROWS;
+                v[i] = row < rows ? table[row * (2 * C) + col] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s += v[i];
+        }
+    }
+    red[tid] = s;
+    sync();
+    if (part == 0 && col < 2 * C) {
+        for (int i = 1; i < PARTS_OF_ROWS; ++i) s += red[i * 32 + tid];
+        sums[col] = s;
+    }
+}
+constexpr int ADDING = SPIO_GN_AFFINE ? (2 * C + 31) / 32 : 0;  // workgroups that add the rows
+
+}  // namespace
+
+#define SPIO_GN_CONCAT2(a, b) a##b
+#define SPIO_GN_CONCAT(a, b) SPIO_GN_CONCAT2(a, b)
+#define SPIO_GN_KERNEL extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS)))
+
+#if !SPIO_GN_SPLIT
+
+// rows[image][2][C]: 0 = grad_weight's, 1 = grad_bias's
+SPIO_GN_KERNEL SPIO_KERNEL_NAME(float* __restrict__ rows, void* __restrict__ din, const void* __restrict__ in,
+                                const unsigned char* __restrict__ exponents, const void* __restrict__ dout,
+                                const float* __restrict__ stats, const float* __restrict__ weight,
+                                const float* __restrict__ bias, long long pixels, long long) {
+    __shared__ float red[RED], pairs[2 * GS];
+    const Place p = place(__builtin_amdgcn_workgroup_id_x(), 1);
+    Chunk c;
+    load_chunk<pw::STREAM>(c, in, exponents, dout, p, pixels);
+    Lane l;
+    load_lane(l, stats, weight, bias, p);
+    channel_sums(c, p, l, red, rows + (long long)p.image * (2 * C));
+    group_pairs(p, red, pairs, weight);
+    apply(c, p, l, din, pairs, pixels);
+}
+
+#if SPIO_GN_AFFINE
+SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _reduce)(float* __restrict__ sums, const float* __restrict__ rows,
+                                                         long long images) {
+    __shared__ float red[THREADS];
+    add_rows(sums, rows, images, (int)__builtin_amdgcn_workgroup_id_x(), red);
+}
+#endif
+
+#else
+
+// rows[image][stretch][2][C], then pairs[image][2][group][stretch]
+SPIO_GN_KERNEL SPIO_KERNEL_NAME(float* __restrict__ rows, void*, const void* __restrict__ in,
+                                const unsigned char* __restrict__ exponents, const void* __restrict__ dout,
+                                const float* __restrict__ stats, const float* __restrict__ weight,
+                                const float* __restrict__ bias, long long pixels, long long images) {
+    __shared__ float red[RED], pairs[2 * GS];
+    const unsigned stretches = (unsigned)((pixels + SPAN - 1) / SPAN);
+    const Place p = place(__builtin_amdgcn_workgroup_id_x(), stretches);
+    Chunk c;
+    load_chunk<0>(c, in, exponents, dout, p, pixels);
+    Lane l;
+    load_lane(l, stats, weight, bias, p);
+    channel_sums(c, p, l, red, rows + ((long long)p.image * stretches + p.stretch) * (2 * C));
+    group_pairs(p, red, pairs, weight);
+    float* out = rows + (SPIO_GN_AFFINE ? images * stretches * (2 * C) : 0);
+    for (int i = p.tid; i < 2 * GS; i += THREADS) {
+        const int g = p.slice * GS + i % GS;
+        if (g < GROUPS) out[(((long long)p.image * 2 + i / GS) * GROUPS + g) * stretches + p.stretch] = pairs[i];
+    }
+}
+
+SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
+    float* __restrict__ sums, const float* __restrict__ rows, void* __restrict__ din, const void* __restrict__ in,
+    const unsigned char* __restrict__ exponents, const void* __restrict__ dout, const float* __restrict__ stats,
+    const float* __restrict__ weight, const float* __restrict__ bias, long long pixels, long long images) {
+    __shared__ float pairs[2 * GS > THREADS ? 2 * GS : THREADS];
+    const unsigned stretches = (unsigned)((pixels + SPAN - 1) / SPAN);
+    const unsigned block = __builtin_amdgcn_workgroup_id_x();
+    if (block < ADDING) {
+        add_rows(sums, rows, images * stretches, (int)block, pairs);
+        return;
+    }
+    // the last stretches first: the first launch read them last
+    const Place p = place((unsigned)images * stretches * SLICES - 1 - (block - ADDING), stretches);
+    Chunk c;
+    load_chunk<pw::STREAM>(c, in, exponents, dout, p, pixels);
+    Lane l;
+    load_lane(l, stats, weight, bias, p);
+    const float* parts = rows + (SPIO_GN_AFFINE ? images * stretches * (2 * C) : 0);
+    constexpr int LANES = group_lanes();
+    const int part = p.tid % LANES;
+    for (int g = p.tid / LANES; g < GS; g += THREADS / LANES) {
+        float a = 0.f, b = 0.f;
+        if (p.slice * GS + g < GROUPS) {
+            const float* s = parts + ((long long)p.image * 2 * GROUPS + p.slice * GS + g) * stretches;
+            for (unsigned i = part; i < stretches; i += LANES) {
+                a += s[i];
+                b += s[(long long)GROUPS * stretches + i];
+            }
+        }
+#pragma unroll
+        for (int m = 1; m < LANES; m <<= 1) {
+            a += lane_xor(a, m);
+            b += lane_xor(b, m);
+        }
+        if (part == 0) {
+            pairs[g] = a;
+            pairs[GS + g] = b;
+        }
+    }
+    sync();
+    apply(c, p, l, din, pairs, pixels);
+}
+
+#endif

@@ -1,0 +1,232 @@
+// What the kernels of element-wise work and of channels-last norms share (gfx950): units of eight values in one
+// of three types, activations, and the 8-bit form that a tensor is kept in between its two passes.
+//
+//   SPIO_DTYPE  0 float16, 1 bfloat16, 2 float32: the tensors' type; all arithmetic is in float32
+//   SPIO_ACT    0 none, 1 relu, 2 silu, 3 gelu (the one of the normal distribution, not tanh's)
+//
+// 8-bit form.  A block is up to 32 neighbouring values; it is held as one signed byte a value (its code) and one
+// byte for the block (its exponent, biased by 127):
+//   E     = the smallest exponent with max|x| < 127.5 * 2^(E-6), at least 7-127; byte E+127
+//   code  = x / 2^(E-6) to the nearest integer, ties to even: -127..127
+//   value = code * 2^(E-6)
+// A step is a power of two, so that quotient, product and the rounding are exact in float32 and a block is off by
+// half a step at most: 1/127.5 of its largest value, or 2^-127 where that is more.  (Values of more than 127.5 steps of the
+// largest exponent are held as 127.)  Byte 255 marks a block that held an infinity or a NaN;
+// all of it comes back as NaN.
+#ifndef SPIO_POINTWISE_H
+#define SPIO_POINTWISE_H
+
+#ifndef SPIO_DTYPE
+#error "SPIO_DTYPE is required"
+#endif
+#ifndef SPIO_ACT
+#define SPIO_ACT 0
+#endif
+
+typedef unsigned int pw_uint2 __attribute__((ext_vector_type(2)));
+typedef unsigned int pw_uint4 __attribute__((ext_vector_type(4)));
+typedef __amdgpu_buffer_rsrc_t pw_rsrc;
+
+namespace pw {
+
+#define PW_DEVICE __device__ inline __attribute__((always_inline))
+
+constexpr int VALUE_BYTES = SPIO_DTYPE == 2 ? 4 : 2;
+constexpr int QUADS = SPIO_DTYPE == 2 ? 2 : 1;  // 16-byte words of a unit
+constexpr int UNIT_BYTES = 16 * QUADS;
+constexpr unsigned OOB = 0x80000000u;           // an offset behind the end of every descriptor
+constexpr int STREAM = 2;                       // cache policy of what is read or written once
+
+PW_DEVICE float as_float(unsigned u) { return __builtin_bit_cast(float, u); }
+PW_DEVICE unsigned as_bits(float f) { return __builtin_bit_cast(unsigned, f); }
+
+// Bytes [base, base + bytes) as a buffer: loads behind its end give zeros, stores there are dropped.
+PW_DEVICE pw_rsrc buffer(const void* base, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+
+struct Unit {
+    pw_uint4 q[QUADS];
+};
+
+template <int POLICY>
+PW_DEVICE Unit load_unit(pw_rsrc rs, unsigned off) {
+    Unit u;
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) u.q[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(off + 16 * i), 0, POLICY);
+    return u;
+}
+// (The offset is in a vector register and the scalar one stays constant: 16-byte stores with a scalar offset can
+// store their data registers as they are after a following write.)
+template <int POLICY>
+PW_DEVICE void store_unit(pw_rsrc rs, unsigned off, const Unit& u) {
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) __builtin_amdgcn_raw_buffer_store_b128(u.q[i], rs, (int)(off + 16 * i), 0, POLICY);
+}
+
+PW_DEVICE void unpack(float (&v)[8], const Unit& u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (SPIO_DTYPE == 2) {
+            v[e] = as_float(u.q[e / 4 % QUADS][e % 4]);
+        } else {
+            const unsigned w = u.q[0][e / 2];
+            if (SPIO_DTYPE == 1)
+                v[e] = as_float(e % 2 ? w & 0xffff0000u : w << 16);
+            else
+                v[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)(e % 2 ? w >> 16 : w));
+        }
+    }
+}
+// Rounds to nearest, ties to even.
+PW_DEVICE Unit pack(const float (&v)[8]) {
+    Unit u;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        if (SPIO_DTYPE == 2) {
+            u.q[e / 4 % QUADS][e % 4] = as_bits(v[e]);
+            u.q[e / 4 % QUADS][e % 4 + 1] = as_bits(v[e + 1]);
+        } else {
+            unsigned short a, b;
+            if (SPIO_DTYPE == 1) {
+                a = __builtin_bit_cast(unsigned short, (__bf16)v[e]);
+                b = __builtin_bit_cast(unsigned short, (__bf16)v[e + 1]);
+            } else {
+                a = __builtin_bit_cast(unsigned short, (_Float16)v[e]);
+                b = __builtin_bit_cast(unsigned short, (_Float16)v[e + 1]);
+            }
+            u.q[0][e / 2] = (unsigned)a | (unsigned)b << 16;
+        }
+    }
+    return u;
+}
+
+// ---- activations ----
+
+// 1 / (1 + exp(-z)); the hardware's exponential and reciprocal are within a unit in the last place.
+PW_DEVICE float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+}
+
+// The normal distribution at z: `density` and `cdf`.  The upper tail is density * R(|z|), and R falls smoothly from
+// sqrt(pi/2) like 1/|z|: a polynomial in t = 1 / (1 + p|z|), fitted to its values (scipy's erfcx) at Chebyshev points of t
+// for |z| <= 14 by reweighted least squares, relative error 1.5e-7.  (Two degrees less, 4.6e-6, would do for results in 16
+// bits, but sums of many of them showed it: grad_bias of 16n 24c 144x144 was off by 1.6e-6 of its norm for 4e-7.)
+PW_DEVICE void normal(float z, float& density, float& cdf) {
+    const float a = __builtin_fabsf(z);
+    const float e = __builtin_amdgcn_exp2f(a * a * -0.721347520f);  // exp(-z^2 / 2)
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3f, 1.f));
+    float r = 0.03567488f;
+    r = __builtin_fmaf(r, t, -0.1572035f);
+    r = __builtin_fmaf(r, t, 0.2063542f);
+    r = __builtin_fmaf(r, t, -0.05368425f);
+    r = __builtin_fmaf(r, t, 0.12856192f);
+    r = __builtin_fmaf(r, t, 0.09991341f);
+    r = __builtin_fmaf(r, t, 0.12075397f);
+    r = __builtin_fmaf(r, t, 0.1196293f);
+    const float tail = e * (r * t);
+    cdf = z < 0.f ? tail : 1.f - tail;
+    density = e * 0.398942280f;
+}
+
+PW_DEVICE float activate(float z) {
+    if (SPIO_ACT == 1) return z < 0.f ? 0.f : z;  // (NaN stays)
+    if (SPIO_ACT == 2) return z * sigmoid(z);
+    if (SPIO_ACT == 3) {
+        float density, cdf;
+        normal(z, density, cdf);
+        return z * cdf;
+    }
+    return z;
+}
+
+// dy times the activation's derivative at z
+PW_DEVICE float activate_grad(float dy, float z) {
+    if (SPIO_ACT == 1) return z > 0.f ? dy : 0.f;
+    if (SPIO_ACT == 2) {
+        const float s = sigmoid(z);
+        return dy * __builtin_fmaf(z * s, 1.f - s, s);
+    }
+    if (SPIO_ACT == 3) {
+        float density, cdf;
+        normal(z, density, cdf);
+        return dy * __builtin_fmaf(z, density, cdf);
+    }
+    return dy;
+}
+
+// ---- 8-bit form ----
+
+// Bits of the largest magnitude of a unit, in the order of the tensors' type (a NaN's are the largest).
+PW_DEVICE unsigned largest(const Unit& u) {
+    if (SPIO_DTYPE == 2) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned w = u.q[i][j] & 0x7fffffffu;
+                m = m > w ? m : w;
+            }
+        return m;
+    }
+    typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+    ushort2_t m = __builtin_bit_cast(ushort2_t, u.q[0][0] & 0x7fff7fffu);
+#pragma unroll
+    for (int j = 1; j < 4; ++j)
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, u.q[0][j] & 0x7fff7fffu));
+    return m[0] > m[1] ? m[0] : m[1];
+}
+template <int CTRL>
+PW_DEVICE unsigned dpp_max(unsigned v) {
+    const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+    return v > other ? v : other;
+}
+// The exponent byte of the block that four neighbouring lanes hold a unit of each.
+PW_DEVICE unsigned block_exponent(const Unit& u) {
+    unsigned m = largest(u);
+    m = dpp_max<0xB1>(m);  // quad_perm [1,0,3,2]
+    m = dpp_max<0x4E>(m);  // quad_perm [2,3,0,1]
+    if (SPIO_DTYPE == 1) m <<= 16;
+    if (SPIO_DTYPE == 0) m = as_bits((float)__builtin_bit_cast(_Float16, (unsigned short)m));
+    // adding a 128th of a unit carries into the exponent where the mantissa is 127.5/64 or more
+    const unsigned e = (m + 0x10000u) >> 23;
+    const unsigned in_range = e < 7 ? 7 : e > 254 ? 254 : e;
+    return m >= 0x7f800000u ? 255 : in_range;
+}
+// The codes of a unit, by a product and a sum whose low byte is the integer (1.5 * 2^23 has a unit of one there).
+PW_DEVICE pw_uint2 encode(const float (&v)[8], unsigned exponent) {
+    const float inverse = as_float((260u - exponent) << 23);
+    constexpr float limit = 0x1.fcp127f;  // 127 steps of the largest exponent: the few values behind it are held as that
+    unsigned r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float x = SPIO_DTYPE == 0 ? v[e] : __builtin_amdgcn_fmed3f(v[e], -limit, limit);
+        r[e] = as_bits(__builtin_fmaf(x, inverse, 12582912.f));
+    }
+    pw_uint2 codes;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        // bytes 0 and 4 of two registers, then bytes 0, 1, 4, 5
+        const unsigned lo = __builtin_amdgcn_perm(r[4 * h + 1], r[4 * h], 0x0c0c0400u);
+        const unsigned hi = __builtin_amdgcn_perm(r[4 * h + 3], r[4 * h + 2], 0x0c0c0400u);
+        codes[h] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    }
+    return codes;
+}
+// The step of an exponent byte; NaN for that of a block without a value.
+PW_DEVICE float block_step(unsigned exponent) {
+    const unsigned e = exponent < 7 ? 7 : exponent;
+    return exponent == 255 ? as_float(0x7fc00000u) : as_float((e - 6) << 23);
+}
+PW_DEVICE void decode(float (&v)[8], const pw_uint2& codes, float step) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const unsigned w = codes[e / 4] ^ 0x80808080u;  // code + 128 as an unsigned byte
+        v[e] = ((float)(w >> 8 * (e % 4) & 0xff) - 128.f) * step;  // (128 steps can be too large a number)
+    }
+}
+
+}  // namespace pw
+
+#endif

@@ -7,6 +7,9 @@ from .conv2d_gw8_function import (
     reset_fused_backward_choices,
 )
 from .layernorm_2d_function import layernorm_2d, layernorm_2d_backward, layernorm_2d_gradients
+from .group_norm_2d_function import group_norm_2d
+from .activation_8bit_function import Packed8bit, activation_8bit, pack_8bit, unpack_8bit
+from .conv2d_gw8_8bit_function import conv2d_gw8_8bit
 from .. import native as _native_path
 
 _native_path.adopt(conv2d_gw8, "conv2d_gw8")

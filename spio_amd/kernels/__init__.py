@@ -27,3 +27,17 @@ from .layernorm_2d_kernel import (
     LayerNorm2dConfig,
     LayerNorm2dBwdConfig,
 )
+from .group_norm_2d_kernel import (
+    group_norm_2d_kernel_factory,
+    group_norm_2d_bwd_kernel_factory,
+    GroupNorm2dParams,
+    GroupNorm2dConfig,
+)
+from .activation_8bit_kernel import (
+    activation_8bit_kernel_factory,
+    activation_8bit_bwd_kernel_factory,
+    pack_8bit_kernel_factory,
+    unpack_8bit_kernel_factory,
+    Activation8bitParams,
+    Activation8bitConfig,
+)

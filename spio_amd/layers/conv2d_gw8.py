@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 from torch import nn
 
-from ..functional import conv2d_gw8
+from ..functional import conv2d_gw8, conv2d_gw8_8bit
 from ..kernels import Conv2dGw8Params
 
 
@@ -18,9 +18,13 @@ def _pair(x) -> Tuple[int, int]:
 
 
 class Conv2dGw8(nn.Conv2d):
-    """Grouped conv2d with group width 8 (C_in == C_out, groups == C // 8)."""
+    """Grouped conv2d with group width 8 (C_in == C_out, groups == C // 8).
+
+    `checkpoint_8bit` (an attribute, False) keeps the input for the weight gradient in 8 bits.
+    """
 
     Params = Conv2dGw8Params
+    checkpoint_8bit = False
 
     @staticmethod
     def make(*args, **kwargs) -> Optional[nn.Module]:
@@ -82,7 +86,8 @@ class Conv2dGw8(nn.Conv2d):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:  # pylint: disable=arguments-renamed
         padding_y, padding_x = _pair(self.padding)
-        return conv2d_gw8(
+        conv = conv2d_gw8_8bit if self.checkpoint_8bit else conv2d_gw8
+        return conv(
             x, self.weight, self.bias, stride=1, padding_y=padding_y, padding_x=padding_x,
             groups=self.groups,
         )  # fmt: skip
