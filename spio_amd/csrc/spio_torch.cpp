@@ -25,8 +25,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
@@ -47,7 +49,10 @@ constexpr auto CL = at::MemoryFormat::ChannelsLast;
 
 // ---- launch plans ---------------------------------------------------------------------------
 
-enum Kind : int64_t { FPROP = 0, DGRAD = 1, WGRAD = 2, BGRAD = 3, NORM = 4, NORM_BWD = 5 };
+enum Kind : int64_t {
+    FPROP = 0, DGRAD = 1, WGRAD = 2, BGRAD = 3, NORM = 4, NORM_BWD = 5,
+    GROUP_NORM = 6, GROUP_NORM_BWD = 7, ACTIVATION = 8, ACTIVATION_BWD = 9, PACK = 10, UNPACK = 11
+};
 
 // What selects a plan: the kind, the device and the numbers of the problem.
 struct Key {
@@ -73,7 +78,7 @@ struct Stage {
 struct Plan {
     Stage main, second;         // `second` of two-stage kernels
     Stage second_half;          // the second stage that stores grad_weight as float16
-    int64_t workspace = 0;      // bytes of partial results between the stages
+    int64_t workspace = 0;      // bytes of partial results between the stages; element-wise: values of a workgroup
     bool present = false;       // false: the shape does not use this kind (no fused backward, no float32 output)
     bool overwrites = false;    // the kernel stores its sums whole instead of adding to them
     std::shared_ptr<PyObject> kernel;  // the Python kernel whose code object `main` and `second` point into
@@ -130,8 +135,8 @@ PlanPtr find_plan(const Key& key) {
 }
 
 void launch(const Stage& stage, hipStream_t stream, std::initializer_list<const void*> args) {
-    const void* values[8];
-    void* params[8];
+    const void* values[16];
+    void* params[16];
     int n = 0;
     for (const void* a : args) {
         values[n] = a;
@@ -511,6 +516,221 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     }
 };
 
+// ---- group norm, activations, the 8-bit form --------------------------------------------------------
+
+const void* number(int64_t v) { return reinterpret_cast<const void*>(v); }  // as a kernel argument
+
+// The numbers that the Python side has for types and activations; -1: none of them.
+int64_t dtype_number(const Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kHalf: return 0;
+        case at::kBFloat16: return 1;
+        case at::kFloat: return 2;
+        default: return -1;
+    }
+}
+constexpr const char* ACTIVATIONS[4] = {"none", "relu", "silu", "gelu"};
+int64_t activation_number(PyObject* o) {
+    if (!PyUnicode_CheckExact(o)) return -1;
+    for (int i = 0; i < 4; ++i)
+        if (PyUnicode_CompareWithASCIIString(o, ACTIVATIONS[i]) == 0) return i;
+    return -1;
+}
+
+// The tensor, or a copy where it does not start on 16 bytes (the kernels load that much at once).
+Tensor aligned(const Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Preserve);
+}
+Tensor empty_bytes(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+constexpr int64_t BLOCK = 32;  // values of a block of the 8-bit form
+int64_t blocks(int64_t n) { return (n + BLOCK - 1) / BLOCK; }
+
+constexpr int64_t GROUP_NORM_MAX_CHANNELS = 4096;
+
+struct GroupNorm {
+    int64_t n, c, h, w, groups, dtype, act;
+    bool kept;
+    double eps;
+    Key key(Kind kind, int64_t device, bool weight, bool bias) const {
+        int64_t bits;
+        std::memcpy(&bits, &eps, sizeof bits);
+        return {{kind, device, n, c, h, w, groups, bits, dtype, act, weight * 2 + bias, kept}};
+    }
+    int64_t pixels() const { return h * w; }
+    std::vector<int64_t> codes() const { return {n, h, w, c}; }
+    std::vector<int64_t> exponents() const { return {n, h, w, blocks(c)}; }
+};
+
+struct GroupNormOutput {
+    Tensor y, stats, codes, exponents;
+};
+
+GroupNormOutput group_norm_forward(const GroupNorm& gn, const Tensor& x, const Tensor& weight, const Tensor& bias,
+                                   bool record) {
+    const auto plan = find_plan(gn.key(GROUP_NORM, x.get_device(), weight.defined(), bias.defined()));
+    hipStream_t stream = c10::hip::getCurrentHIPStream(x.get_device());
+    GroupNormOutput o;
+    o.y = empty_cl(x.sizes(), x.scalar_type(), x);
+    if (record) o.stats = at::detail::empty_cuda({gn.n, gn.groups, 2}, at::kFloat, x.device(), std::nullopt);
+    if (gn.kept) {
+        o.codes = empty_bytes(gn.codes(), at::kChar, x);
+        o.exponents = empty_bytes(gn.exponents(), at::kByte, x);
+    }
+    const void *px = number(gn.pixels()), *images = number(gn.n);
+    if (!plan->second.function) {
+        launch(plan->main, stream, {ptr(o.y), ptr(o.codes), ptr(o.exponents), ptr(o.stats), ptr(x), ptr(weight), ptr(bias),
+                                    px, images});
+    } else {
+        const Tensor partials = empty_1d(plan->workspace, at::kByte, x);
+        launch(plan->main, stream, {nullptr, nullptr, nullptr, ptr(partials), ptr(x), nullptr, nullptr, px, images});
+        launch(plan->second, stream, {ptr(o.stats), ptr(partials), ptr(o.y), ptr(o.codes), ptr(o.exponents), ptr(x),
+                                      ptr(weight), ptr(bias), px, images});
+    }
+    return o;
+}
+
+PyObject* g_group_norm_gradients = nullptr;  // Python: the gradients through the backward operator
+PyObject* g_activation_gradient = nullptr;
+
+// A gradient with the layout that the kernels read.
+Tensor to_cl(const Tensor& t) { return aligned(t.is_contiguous(CL) ? t : t.contiguous(CL)); }
+
+struct GroupNormFunction : torch::autograd::Function<GroupNormFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight_arg,
+                          const std::optional<Tensor>& bias_arg, const GroupNorm& gn) {
+        const Tensor weight = weight_arg.value_or(Tensor()), bias = bias_arg.value_or(Tensor());
+        const auto o = group_norm_forward(gn, to_cl(x), to_float_1d(weight), to_float_1d(bias), /*record=*/true);
+        ctx->save_for_backward({gn.kept ? o.codes : x, o.exponents, o.stats, weight, bias});
+        auto type = [](const Tensor& t) { return static_cast<int64_t>(t.defined() ? t.scalar_type() : at::kFloat); };
+        ctx->saved_data["v"] = std::vector<int64_t>{gn.n, gn.c, gn.h, gn.w, gn.groups, gn.dtype, gn.act, gn.kept,
+                                                    type(x), type(weight), type(bias)};
+        ctx->saved_data["eps"] = gn.eps;
+        return o.y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->saved_data["v"].toIntVector();
+        const GroupNorm gn{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7] != 0, ctx->saved_data["eps"].toDouble()};
+        auto type = [&](int i) { return static_cast<at::ScalarType>(v[i]); };
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &exponents = saved[1], &stats = saved[2], &weight = saved[3], &bias = saved[4];
+        const Tensor& dy = grads[0];
+        const bool has_weight = weight.defined(), has_bias = bias.defined();
+        const bool native = !stands_aside(dy) && dy.scalar_type() == type(8) && dy.sizes() == at::IntArrayRef({gn.n, gn.c, gn.h, gn.w}) &&
+                            (gn.kept ? is_again(x, dy, gn.codes(), at::kChar) && is_again(exponents, dy, gn.exponents(), at::kByte)
+                                     : is_again(x, dy, {gn.n, gn.c, gn.h, gn.w}, type(8))) &&
+                            is_again(stats, dy, {gn.n, gn.groups, 2}, at::kFloat) &&
+                            (!has_weight || is_again(weight, dy, {gn.c}, type(9))) &&
+                            (!has_bias || is_again(bias, dy, {gn.c}, type(10)));
+        // absent tensors have no edge (as in NormFunction)
+        const bool need_x = ctx->needs_input_grad(0), need_w = has_weight && ctx->needs_input_grad(1),
+                   need_b = has_bias && ctx->needs_input_grad(has_weight ? 2 : 1);
+        if (!native) {
+            py::gil_scoped_acquire gil;
+            auto optional_py = [](const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); };
+            py::tuple r = py::reinterpret_borrow<py::object>(g_group_norm_gradients)(
+                dy, x, optional_py(exponents), stats, gn.groups, optional_py(weight), optional_py(bias), gn.eps,
+                ACTIVATIONS[gn.act], need_x, need_w, need_b);
+            auto get = [&](int i) { return r[i].is_none() ? Tensor() : r[i].cast<Tensor>(); };
+            return {get(0), get(1), get(2), Tensor()};
+        }
+        RECORD_FUNCTION("spio::group_norm_2d_backward", tensors({dy, x, exponents, stats, weight, bias}));
+        const Tensor dyc = to_cl(dy);
+        const Tensor xc = gn.kept ? aligned(x.contiguous()) : to_cl(x);
+        const Tensor ec = exponents.defined() ? exponents.contiguous() : Tensor(), sc = stats.contiguous();
+        const Tensor wf = to_float_1d(weight), bf = to_float_1d(bias);
+        const auto device = dyc.get_device();
+        hipStream_t stream = c10::hip::getCurrentHIPStream(device);
+        const auto plan = find_plan(gn.key(GROUP_NORM_BWD, device, has_weight, has_bias));
+        const Tensor dx = empty_cl(dyc.sizes(), dyc.scalar_type(), dyc);
+        Tensor sums, workspace;
+        if (has_weight || has_bias) sums = at::detail::empty_cuda({2, gn.c}, at::kFloat, dyc.device(), std::nullopt);
+        if (plan->second.function) workspace = empty_1d(plan->workspace, at::kByte, dyc);
+        const void *px = number(gn.pixels()), *images = number(gn.n);
+        launch(plan->main, stream, {ptr(workspace), ptr(dx), ptr(xc), ptr(ec), ptr(dyc), ptr(sc), ptr(wf), ptr(bf), px, images});
+        if (plan->overwrites)  // (images in stretches: the second launch makes grad_input)
+            launch(plan->second, stream, {ptr(sums), ptr(workspace), ptr(dx), ptr(xc), ptr(ec), ptr(dyc), ptr(sc), ptr(wf),
+                                          ptr(bf), px, images});
+        else if (plan->second.function)
+            launch(plan->second, stream, {ptr(sums), ptr(workspace), images});
+        return {need_x ? dx : Tensor(), need_w ? sums.select(0, 0).to(weight.scalar_type()) : Tensor(),
+                need_b ? sums.select(0, 1).to(bias.scalar_type()) : Tensor(), Tensor()};
+    }
+};
+
+// The launch of an element-wise kernel over n values.
+void launch_values(const Plan& plan, int64_t n, hipStream_t stream, std::initializer_list<const void*> args) {
+    Stage stage = plan.main;
+    const int64_t grid = (n + plan.workspace - 1) / plan.workspace;
+    TORCH_CHECK_VALUE(grid * stage.block[0] < (int64_t(1) << 32), "more workgroups than a launch can have");
+    stage.grid[0] = static_cast<unsigned>(grid);
+    launch(stage, stream, args);
+}
+Key values_key(Kind kind, const Tensor& like, int64_t dtype, int64_t act, bool kept) {
+    return {{kind, like.get_device(), dtype, act, kept, 0, 0, 0, 0, 0, 0, 0}};
+}
+Tensor empty_as(const Tensor& t, at::ScalarType dtype) {  // sizes and strides of a tensor without gaps
+    return at::detail::empty_strided_cuda(t.sizes(), t.strides(), dtype, t.device());
+}
+Tensor dense(const Tensor& t) { return aligned(t.is_non_overlapping_and_dense() ? t : t.contiguous()); }
+
+struct Kept {
+    Tensor codes, exponents;
+};
+Kept empty_kept(const Tensor& x) {
+    return {empty_1d(x.numel(), at::kChar, x), empty_1d(blocks(x.numel()), at::kByte, x)};
+}
+
+// y of x, a tensor without gaps, and x in the 8-bit form where `kept` is given.
+Tensor activation_forward(const Tensor& x, int64_t act, Kept* kept) {
+    const auto plan = find_plan(values_key(ACTIVATION, x, dtype_number(x), act, kept != nullptr));
+    const Tensor y = empty_as(x, x.scalar_type());
+    if (kept) *kept = empty_kept(x);
+    launch_values(*plan, x.numel(), c10::hip::getCurrentHIPStream(x.get_device()),
+                  {ptr(y), kept ? ptr(kept->codes) : nullptr, kept ? ptr(kept->exponents) : nullptr, ptr(x), number(x.numel())});
+    return y;
+}
+
+struct ActivationFunction : torch::autograd::Function<ActivationFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t act) {
+        Kept kept;
+        const Tensor y = activation_forward(dense(x), act, &kept);
+        ctx->save_for_backward({kept.codes, kept.exponents});
+        ctx->saved_data["strides"] = y.strides().vec();
+        ctx->saved_data["v"] = std::vector<int64_t>{act, static_cast<int64_t>(x.scalar_type())};
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->saved_data["v"].toIntVector();
+        const auto strides = ctx->saved_data["strides"].toIntVector();
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &codes = saved[0], &exponents = saved[1], &grad = grads[0];
+        const int64_t n = grad.numel();
+        const bool native = !stands_aside(grad) && grad.scalar_type() == static_cast<at::ScalarType>(v[1]) &&
+                            is_again(codes, grad, {n}, at::kChar) && is_again(exponents, grad, {blocks(n)}, at::kByte);
+        if (!native) {
+            py::gil_scoped_acquire gil;
+            return {py::reinterpret_borrow<py::object>(g_activation_gradient)(grad, codes, exponents, ACTIVATIONS[v[0]], strides)
+                        .cast<Tensor>(), Tensor()};
+        }
+        RECORD_FUNCTION("spio::activation_8bit_backward", tensors({grad, codes, exponents}));
+        Tensor dy = grad;
+        if (dy.strides() != at::IntArrayRef(strides)) {
+            dy = at::detail::empty_strided_cuda(grad.sizes(), strides, grad.scalar_type(), grad.device());
+            dy.copy_(grad);
+        }
+        dy = aligned(dy);
+        const Tensor cc = aligned(codes.contiguous()), ec = exponents.contiguous();
+        const auto plan = find_plan(values_key(ACTIVATION_BWD, dy, dtype_number(dy), v[0], true));
+        const Tensor dx = empty_as(dy, dy.scalar_type());
+        launch_values(*plan, n, c10::hip::getCurrentHIPStream(dy.get_device()), {ptr(dx), ptr(cc), ptr(ec), ptr(dy), number(n)});
+        return {dx, Tensor()};
+    }
+};
+
 // ---- Python boundary ------------------------------------------------------------------------
 
 // Arguments of a Python call by position or keyword; false if they do not fit the names.
@@ -641,7 +861,167 @@ PyObject* layernorm_2d(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObj
     END_HANDLE_TH_ERRORS
 }
 
+// group_norm_2d(inputs, num_groups, weight=None, bias=None, eps=1e-5, activation="none", checkpoint_8bit=False)
+PyObject* group_norm_2d(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    static PyObject* const names[7] = {
+        PyUnicode_InternFromString("inputs"), PyUnicode_InternFromString("num_groups"), PyUnicode_InternFromString("weight"),
+        PyUnicode_InternFromString("bias"), PyUnicode_InternFromString("eps"), PyUnicode_InternFromString("activation"),
+        PyUnicode_InternFromString("checkpoint_8bit")};
+    if (g_bypass.load(std::memory_order_relaxed) != 0 || !eager_mode()) return not_implemented();
+    PyObject* a[7] = {};
+    if (!parse(args, nargs, kwnames, names, a)) return not_implemented();
+    Tensor x, weight, bias;
+    int64_t groups = 0;
+    if (!tensor_arg(a[0], &x) || !a[1] || !int_arg(a[1], &groups) || (a[2] && a[2] != Py_None && !tensor_arg(a[2], &weight)) ||
+        (a[3] && a[3] != Py_None && !tensor_arg(a[3], &bias)) || (a[4] && !PyFloat_CheckExact(a[4])) || (a[6] && !PyBool_Check(a[6])))
+        return not_implemented();
+    if (!is_plain(x) || x.dim() != 4 || dtype_number(x) < 0) return not_implemented();
+    GroupNorm gn{x.size(0), x.size(1), x.size(2), x.size(3), groups, dtype_number(x), a[5] ? activation_number(a[5]) : 0,
+                 a[6] == Py_True, a[4] ? PyFloat_AS_DOUBLE(a[4]) : 1e-5};
+    for (const Tensor& t : {weight, bias})
+        if (t.defined() && (!is_plain(t) || t.dim() != 1 || t.size(0) != gn.c || t.device() != x.device() || dtype_number(t) < 0))
+            return not_implemented();
+    if (gn.n < 1 || gn.h < 1 || gn.w < 1 || gn.c < 8 || gn.c % 8 || gn.c > GROUP_NORM_MAX_CHANNELS || groups < 1 ||
+        gn.c % groups || gn.act < 0 || !(gn.eps > 0))
+        return not_implemented();
+    const bool record = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias));
+    gn.kept = gn.kept && record;
+    Tensor y;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(x.device());
+        RECORD_FUNCTION("spio::group_norm_2d_forward", tensors({x, weight, bias}));
+        if (record) {
+            y = GroupNormFunction::apply(x, optional(weight), optional(bias), gn);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            y = group_norm_forward(gn, to_cl(x), to_float_1d(weight), to_float_1d(bias), /*record=*/false).y;
+        }
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// activation_8bit(inputs, activation="gelu")
+PyObject* activation_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    static PyObject* const names[2] = {PyUnicode_InternFromString("inputs"), PyUnicode_InternFromString("activation")};
+    if (g_bypass.load(std::memory_order_relaxed) != 0 || !eager_mode()) return not_implemented();
+    PyObject* a[2] = {};
+    Tensor x;
+    if (!parse(args, nargs, kwnames, names, a) || !tensor_arg(a[0], &x)) return not_implemented();
+    const int64_t act = a[1] ? activation_number(a[1]) : 3;
+    if (!is_plain(x) || dtype_number(x) < 0 || act < 1 || x.numel() == 0) return not_implemented();
+    Tensor y;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(x.device());
+        RECORD_FUNCTION("spio::activation_8bit_forward", tensors({x}));
+        if (at::GradMode::is_enabled() && x.requires_grad()) {
+            y = ActivationFunction::apply(x, act);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            y = activation_forward(dense(x), act, nullptr);
+        }
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// pack_8bit(inputs): (codes, exponents) of a tensor without gaps
+PyObject* pack_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    if (g_bypass.load(std::memory_order_relaxed) != 0 || !eager_mode() || nargs != 1 || kwnames) return not_implemented();
+    Tensor x;
+    if (!tensor_arg(args[0], &x) || !is_plain(x) || dtype_number(x) < 0 || x.numel() == 0 || !x.is_non_overlapping_and_dense())
+        return not_implemented();
+    Kept kept;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(x.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        RECORD_FUNCTION("spio::pack_8bit", tensors({x}));
+        const auto plan = find_plan(values_key(PACK, x, dtype_number(x), 0, true));
+        const Tensor xa = aligned(x);
+        kept = empty_kept(x);
+        launch_values(*plan, x.numel(), c10::hip::getCurrentHIPStream(x.get_device()),
+                      {ptr(kept.codes), ptr(kept.exponents), ptr(xa), number(x.numel())});
+    }
+    return py::make_tuple(kept.codes, kept.exponents).release().ptr();
+    END_HANDLE_TH_ERRORS
+}
+
+// A tuple of integers, at most 16.
+bool ints_arg(PyObject* o, std::vector<int64_t>* v) {
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) > 16) return false;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o); ++i) {
+        int64_t item = 0;
+        if (!int_arg(PyTuple_GET_ITEM(o, i), &item) || item < 0) return false;
+        v->push_back(item);
+    }
+    return true;
+}
+
+// unpack_8bit(codes, exponents, shape, strides, dtype)
+PyObject* unpack_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    if (g_bypass.load(std::memory_order_relaxed) != 0 || !eager_mode() || nargs != 5 || kwnames) return not_implemented();
+    Tensor codes, exponents;
+    std::vector<int64_t> shape, strides;
+    if (!tensor_arg(args[0], &codes) || !tensor_arg(args[1], &exponents) || !ints_arg(args[2], &shape) ||
+        !ints_arg(args[3], &strides) || !THPDtype_Check(args[4]) || shape.size() != strides.size())
+        return not_implemented();
+    const at::ScalarType dtype = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    const int64_t n = codes.numel();
+    if (!is_plain(codes) || !is_plain(exponents) || codes.dim() != 1 || exponents.dim() != 1 || n == 0 ||
+        codes.scalar_type() != at::kChar || exponents.scalar_type() != at::kByte || exponents.device() != codes.device() ||
+        exponents.numel() != blocks(n) || (dtype != at::kHalf && dtype != at::kBFloat16 && dtype != at::kFloat))
+        return not_implemented();
+    int64_t count = 1;
+    for (int64_t size : shape) {
+        if (size > n) return not_implemented();
+        count *= size;  // (no more than n^2 before it is looked at)
+        if (count > n) return not_implemented();
+    }
+    if (count != n) return not_implemented();
+    Tensor out;
+    bool dense_strides = true;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(codes.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        std::vector<size_t> order;
+        for (size_t i = 0; i < shape.size(); ++i)
+            if (shape[i] != 1) order.push_back(i);
+        std::sort(order.begin(), order.end(), [&](size_t i, size_t j) { return strides[i] < strides[j]; });
+        int64_t expected = 1;
+        for (size_t i : order) {
+            dense_strides = dense_strides && strides[i] == expected;
+            expected *= shape[i];
+        }
+        if (dense_strides) {
+            RECORD_FUNCTION("spio::unpack_8bit", tensors({codes, exponents}));
+            out = at::detail::empty_strided_cuda(shape, strides, dtype, codes.device());
+            const Tensor cc = aligned(codes.contiguous()), ec = exponents.contiguous();
+            const auto plan = find_plan(values_key(UNPACK, out, dtype_number(out), 0, true));
+            launch_values(*plan, n, c10::hip::getCurrentHIPStream(codes.get_device()), {ptr(out), ptr(cc), ptr(ec), number(n)});
+        }
+    }
+    if (!dense_strides) return not_implemented();
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef g_methods[] = {
+    {"group_norm_2d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_norm_2d)),
+     METH_FASTCALL | METH_KEYWORDS, "group_norm_2d on plain GPU tensors, else NotImplemented"},
+    {"activation_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(activation_8bit)),
+     METH_FASTCALL | METH_KEYWORDS, "activation_8bit on plain GPU tensors, else NotImplemented"},
+    {"pack_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack_8bit)), METH_FASTCALL | METH_KEYWORDS,
+     "codes and exponents of a plain GPU tensor without gaps, else NotImplemented"},
+    {"unpack_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(unpack_8bit)), METH_FASTCALL | METH_KEYWORDS,
+     "the tensor of codes, exponents, shape, strides and type, else NotImplemented"},
     {"layernorm_2d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layernorm_2d)),
      METH_FASTCALL | METH_KEYWORDS, "spio::layernorm_2d on plain GPU tensors, else NotImplemented"},
     {"conv2d_gw8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(conv2d_gw8)),
@@ -665,6 +1045,10 @@ PYBIND11_MODULE(_native, m) {
         g_make_plan = make_plan.release().ptr();
         g_backward_op = backward_op.release().ptr();
         g_norm_gradients = norm_gradients.release().ptr();
+    });
+    m.def("configure_kept", [](py::object group_norm_gradients, py::object activation_gradient) {
+        g_group_norm_gradients = group_norm_gradients.release().ptr();
+        g_activation_gradient = activation_gradient.release().ptr();
     });
     m.def("bypass", [](int64_t change) { g_bypass.fetch_add(change); });
     m.def("forget", [] {

@@ -13,6 +13,7 @@ from typing import List, NamedTuple, Tuple
 
 import torch
 
+from .. import native
 from ..kernels.activation_8bit_kernel import (
     BLOCK,
     Activation8bitParams,
@@ -23,7 +24,7 @@ from ..kernels.activation_8bit_kernel import (
 )
 from ..kernels.group_norm_2d_kernel import ACTIVATIONS, DTYPES
 from ..util.math import divup
-from .group_norm_2d_function import aligned
+from .group_norm_2d_function import aligned, refuse_second_derivatives
 
 POINTWISE = tuple(name for name in ACTIVATIONS if name != "none")
 
@@ -84,7 +85,7 @@ def pack_8bit_op(inputs: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     codes, exponents = _empty_kept(x)
     n = x.numel()
     if n:
-        kernel = pack_8bit_kernel_factory.get_kernel(Activation8bitParams(n, DTYPES[x.dtype]), x.device)
+        kernel = pack_8bit_kernel_factory.get_kernel(Activation8bitParams(DTYPES[x.dtype]), x.device)
         kernel(codes, exponents, x, n)
     return codes, exponents
 
@@ -109,7 +110,7 @@ def unpack_8bit_op(codes: torch.Tensor, exponents: torch.Tensor, shape: List[int
     _require_gpu(codes, "unpack_8bit")
     out = torch.empty_strided(tuple(shape), tuple(strides), dtype=dtype, device=codes.device)
     if n:
-        kernel = unpack_8bit_kernel_factory.get_kernel(Activation8bitParams(n, DTYPES[dtype]), codes.device)
+        kernel = unpack_8bit_kernel_factory.get_kernel(Activation8bitParams(DTYPES[dtype]), codes.device)
         kernel(out, aligned(codes.contiguous()), exponents.contiguous(), n)
     return out
 
@@ -123,13 +124,17 @@ def pack_8bit(inputs: torch.Tensor) -> Packed8bit:
     """A float16, bfloat16 or float32 GPU tensor of any shape in the 8-bit form, 33/64 of its size in 16 bits.  A
     tensor with gaps is packed as its contiguous copy.  No gradient passes through."""
     x = dense(inputs.detach())
-    return Packed8bit(*pack_8bit_op(x), tuple(x.shape), tuple(x.stride()), x.dtype)
+    kept = native.call("pack_8bit", x)
+    return Packed8bit(*(pack_8bit_op(x) if kept is NotImplemented else kept), tuple(x.shape), tuple(x.stride()), x.dtype)
 
 
 def unpack_8bit(packed: Packed8bit, dtype: torch.dtype = None) -> torch.Tensor:
     """The tensor that `packed` stands for, in its own type or another one (float16: the largest finite value in
     place of larger ones)."""
     dtype = packed.dtype if dtype is None else dtype
+    out = native.call("unpack_8bit", packed.codes, packed.exponents, packed.shape, packed.strides, dtype)
+    if out is not NotImplemented:
+        return out
     return unpack_8bit_op(packed.codes, packed.exponents, list(packed.shape), list(packed.strides), dtype)
 
 
@@ -153,7 +158,7 @@ def activation_8bit_forward(inputs: torch.Tensor, activation: str,
     codes, exponents = _empty_kept(x, keep)
     n = x.numel()
     if n:
-        params = Activation8bitParams(n, DTYPES[x.dtype], ACTIVATIONS[activation], keep)
+        params = Activation8bitParams(DTYPES[x.dtype], ACTIVATIONS[activation], keep)
         kernel = activation_8bit_kernel_factory.get_kernel(params, x.device)
         kernel(out, *((codes, exponents) if keep else (None, None)), x, n)
     return out, codes, exponents
@@ -177,7 +182,7 @@ def activation_8bit_backward(grad_output: torch.Tensor, codes: torch.Tensor, exp
     dy = aligned(grad_output)
     grad_input = torch.empty_like(dy)
     if n:
-        params = Activation8bitParams(n, DTYPES[dy.dtype], ACTIVATIONS[activation])
+        params = Activation8bitParams(DTYPES[dy.dtype], ACTIVATIONS[activation])
         kernel = activation_8bit_bwd_kernel_factory.get_kernel(params, dy.device)
         kernel(grad_input, aligned(codes.contiguous()), exponents.contiguous(), dy, n)
     return grad_input
@@ -195,6 +200,12 @@ def laid_out(t: torch.Tensor, strides) -> torch.Tensor:
     return torch.empty_strided(t.shape, tuple(strides), dtype=t.dtype, device=t.device).copy_(t)
 
 
+def activation_8bit_gradient(grad_output, codes, exponents, activation, strides):
+    """grad_input of activation_8bit whose input lay in memory by these strides."""
+    refuse_second_derivatives()
+    return activation_8bit_backward(laid_out(grad_output, strides), codes, exponents, activation)
+
+
 def _setup_context(ctx, inputs, output):
     out, codes, exponents = output
     ctx.mark_non_differentiable(codes, exponents)
@@ -208,7 +219,7 @@ def _backward(ctx, grad_output, *_unused):
     if grad_output is None:
         return None, None, None
     codes, exponents = ctx.saved_tensors
-    return activation_8bit_backward(laid_out(grad_output, ctx.strides), codes, exponents, ctx.activation), None, None
+    return activation_8bit_gradient(grad_output, codes, exponents, ctx.activation, ctx.strides), None, None
 
 
 activation_8bit_forward.register_autograd(_backward, setup_context=_setup_context)
@@ -217,5 +228,8 @@ activation_8bit_forward.register_autograd(_backward, setup_context=_setup_contex
 def activation_8bit(inputs: torch.Tensor, activation: str = "gelu") -> torch.Tensor:
     """relu, silu or gelu (of the normal distribution) of a GPU tensor of any shape, in its type; what the backward
     pass needs of the input is kept in 8 bits."""
+    y = native.call("activation_8bit", inputs, activation)
+    if y is not NotImplemented:
+        return y
     keep = torch.is_grad_enabled() and inputs.requires_grad
     return activation_8bit_forward(dense(inputs), activation, keep)[0]

@@ -10,6 +10,7 @@ import torch
 
 from .activation_8bit_function import pack_8bit_op, unpack_8bit_op
 from .conv2d_gw8_function import conv2d_gw8, conv2d_gw8_backward_op
+from .group_norm_2d_function import refuse_second_derivatives
 
 CL = torch.channels_last
 
@@ -49,6 +50,7 @@ def _setup_context(ctx, inputs, output):
 def _backward(ctx, grad_output, *_unused):
     if grad_output is None:
         return (None,) * 5
+    refuse_second_derivatives()
     codes, exponents, weight, bias = ctx.saved_tensors
     n, c, h, w = ctx.shape
     needs = ctx.needs_input_grad

@@ -15,6 +15,7 @@ from typing import Optional, Tuple
 
 import torch
 
+from .. import native
 from ..kernels.group_norm_2d_kernel import (
     ACTIVATIONS,
     DTYPES,
@@ -138,9 +139,17 @@ def _backward_fake(grad_output, inputs, exponents, stats, num_groups, weight, bi
             grad_output.new_empty((2, c), dtype=torch.float32))  # fmt: skip
 
 
+def refuse_second_derivatives():
+    """What is kept in 8 bits has no history: a gradient of a gradient would take it for a constant."""
+    if torch.is_grad_enabled() and not torch.compiler.is_compiling():
+        raise RuntimeError("an input that was kept in 8 bits has no second derivatives (create_graph=True)")
+
+
 def group_norm_2d_gradients(grad_output, inputs, exponents, stats, num_groups, weight, bias, eps, activation, needs_input,
                             needs_weight, needs_bias):  # fmt: skip
     """Gradients of group_norm_2d in the types of the tensors they belong to, None where not needed."""
+    if exponents is not None:
+        refuse_second_derivatives()
     grad_input, sums = group_norm_2d_backward(grad_output, inputs, exponents, stats, num_groups, weight, bias, eps,
                                               activation)  # fmt: skip
     return (
@@ -188,6 +197,9 @@ def group_norm_2d(
     Returns:
         (N, C, H, W) in the inputs' type, channels_last.
     """
+    y = native.call("group_norm_2d", inputs, num_groups, weight, bias, eps, activation, checkpoint_8bit)
+    if y is not NotImplemented:
+        return y
     kept = bool(checkpoint_8bit) and torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (inputs, weight, bias))  # fmt: skip
     return group_norm_2d_forward(inputs, num_groups, weight, bias, eps, activation, kept)[0]

@@ -1,6 +1,6 @@
 """Element-wise kernels with an 8-bit checkpoint (csrc/activation_8bit.hip): parameters and factories.
 
-Specialised by type and activation; the number of values is an argument.  Arguments:
+Specialised by type and activation; the number of values is an argument, and the grid follows from it.  Arguments:
   activation_8bit      (output, codes or None, exponents or None, input, n)
   activation_8bit_bwd  (grad_input, codes, exponents, grad_output, n)
   pack_8bit            (codes, exponents, input, n)
@@ -11,7 +11,6 @@ from dataclasses import dataclass
 
 import torch
 
-from ..util.math import divup
 from .group_norm_2d_kernel import ACTIVATIONS, DTYPE_NAMES, DTYPES
 from .kernel import KernelSpec
 from .kernel_factory import KernelFactory
@@ -23,10 +22,8 @@ BLOCK = 32  # values of a block of the 8-bit form
 
 @dataclass(frozen=True)
 class Activation8bitParams:
-    """`n` values of a type, an activation (numbers of DTYPES and ACTIVATIONS), and whether the forward pass keeps
-    its input."""
+    """Type and activation (numbers of DTYPES and ACTIVATIONS), and whether the forward pass keeps its input."""
 
-    n: int
     dtype: int = 0
     activation: int = 0
     kept: bool = True
@@ -35,7 +32,7 @@ class Activation8bitParams:
         return f"{DTYPE_NAMES[self.dtype]}_{list(ACTIVATIONS)[self.activation]}" + ("_8bit" if self.kept else "")
 
     def validate(self):
-        assert self.n > 0 and 0 <= self.dtype <= 2 and 0 <= self.activation <= 3
+        assert 0 <= self.dtype <= 2 and 0 <= self.activation <= 3
 
 
 @dataclass(frozen=True)
@@ -49,28 +46,28 @@ class Activation8bitConfig:
 def _spec(mode):
     def spec(params: Activation8bitParams, config: Activation8bitConfig, _device_attr=None) -> KernelSpec:
         params.validate()
-        grid = divup(params.n, config.threads * config.units * 8)
-        assert grid * config.threads < 1 << 32, "more workgroups than a launch can have"
         defines = {
             "SPIO_MODE": mode, "SPIO_THREADS": config.threads, "SPIO_UNROLL": config.units,
             "SPIO_DTYPE": params.dtype, "SPIO_ACT": params.activation, "SPIO_KEEP": int(params.kept),
         }  # fmt: skip
-        return KernelSpec(defines, LaunchParams(grid=grid, block=config.threads), SOURCE)
+        return KernelSpec(defines, LaunchParams(grid=1, block=config.threads), SOURCE,
+                          values_per_workgroup=config.threads * config.units * 8)  # fmt: skip
 
     return spec
 
 
 def _test_args(mode):
     def args(params: Activation8bitParams, device):
-        values = torch.randn(params.n, device=device).to(list(DTYPES)[params.dtype])
-        codes = torch.randint(0, 256, (params.n,), device=device, dtype=torch.uint8)
-        exponents = torch.full((divup(params.n, BLOCK),), 126, device=device, dtype=torch.uint8)
+        n = 1 << 24
+        values = torch.randn(n, device=device).to(list(DTYPES)[params.dtype])
+        codes = torch.randint(0, 256, (n,), device=device, dtype=torch.uint8)
+        exponents = torch.full((n // BLOCK,), 126, device=device, dtype=torch.uint8)
         kept = (codes, exponents) if params.kept else (None, None)
         return {
-            0: (torch.empty_like(values), *kept, values, params.n),
-            1: (torch.empty_like(values), codes, exponents, values, params.n),
-            2: (codes, exponents, values, params.n),
-            3: (values, codes, exponents, params.n),
+            0: (torch.empty_like(values), *kept, values, n),
+            1: (torch.empty_like(values), codes, exponents, values, n),
+            2: (codes, exponents, values, n),
+            3: (values, codes, exponents, n),
         }[mode]
 
     return args

@@ -179,7 +179,7 @@ def _get_bwd_kernel_spec(params: GroupNorm2dParams, config: GroupNorm2dConfig, _
     affine = params.has_weight or params.has_bias
     launch = LaunchParams(grid=grid, block=config.threads)
     spec = KernelSpec(dict(_defines(params, config), SPIO_GN_AFFINE=int(affine)), launch, BWD_SOURCE)
-    spec.overwrites_output = True
+    spec.overwrites_output = bool(config.split)  # grad_input and all sums are the second launch's
     adding = divup(2 * params.c, 32) if affine else 0
     rows = params.n * stretches * 2 * params.c * 4 if affine else 0
     if config.split:

@@ -52,7 +52,16 @@ class KernelSpec:
     # True: the kernel (its last stage) stores the tensor at `workspace_arg` whole, so the caller
     # need not zero it; False: the kernel adds into it
     overwrites_output: bool = False
+    # Element-wise kernels: the values a workgroup takes; their number is the last argument, and the grid follows from it
+    values_per_workgroup: int = 0
 
+    def grid(self, args):
+        """Workgroups of a launch with these arguments."""
+        if not self.values_per_workgroup:
+            return self.launch_params.grid
+        grid = divup(args[-1], self.values_per_workgroup)
+        assert 0 < grid and grid * self.launch_params.block[0] < 1 << 32, "more workgroups than a launch can have"
+        return (grid, 1, 1)
 
 
 class LaunchTimer:
@@ -203,7 +212,7 @@ class Kernel:
                 timer.events.setdefault(self, []).append((start, stop))
                 start.record()
             if self.epilogue_function is None:
-                self.function.launch(lp.grid, lp.block, args, lp.shared_mem_bytes, stream)
+                self.function.launch(spec.grid(args), lp.block, args, lp.shared_mem_bytes, stream)
             elif static_workspace:
                 ep = spec.epilogue_launch_params
                 nbytes = spec.workspace_bytes
@@ -250,7 +259,7 @@ class Kernel:
         stream = torch.cuda.current_stream(device).cuda_stream
         if self.epilogue_function is None:
             return self.function.launch_timed(
-                lp.grid, lp.block, prepared, lp.shared_mem_bytes, stream, warmup, iters
+                spec.grid(prepared[0]), lp.block, prepared, lp.shared_mem_bytes, stream, warmup, iters
             )
         ep = spec.epilogue_launch_params
         workspaces = []

@@ -121,16 +121,30 @@ def _make_plan(values):
             kernel = factory.get_kernel(params, device, **direction)
         if kernel is not None:
             kernel = _adapted(kernel, factory, params, device, mode, **direction)
-    else:
+    elif kind < 6:
         n, c, h, w, eps, weight, bias = values[2:9]
         params = kernels.LayerNorm2dParams(n=n, c=c, h=h, w=w, eps=struct.unpack("<d", struct.pack("<q", eps))[0],
                                            has_weight=bool(weight), has_bias=bool(bias))  # fmt: skip
         factory = kernels.layernorm_2d_kernel_factory if kind == 4 else kernels.layernorm_2d_bwd_kernel_factory
         kernel = factory.get_kernel(params, device)
+    elif kind < 8:
+        n, c, h, w, groups, eps, dtype, activation, vectors, kept = values[2:]
+        params = kernels.GroupNorm2dParams(n=n, c=c, h=h, w=w, groups=groups, dtype=dtype, activation=activation,
+                                           eps=struct.unpack("<d", struct.pack("<q", eps))[0], has_weight=bool(vectors & 2),
+                                           has_bias=bool(vectors & 1), kept=bool(kept))  # fmt: skip
+        factory = kernels.group_norm_2d_kernel_factory if kind == 6 else kernels.group_norm_2d_bwd_kernel_factory
+        kernel = factory.get_kernel(params, device)
+    else:
+        dtype, activation, kept = values[2:5]
+        factory = (kernels.activation_8bit_kernel_factory, kernels.activation_8bit_bwd_kernel_factory,
+                   kernels.pack_8bit_kernel_factory, kernels.unpack_8bit_kernel_factory)[kind - 8]  # fmt: skip
+        kernel = factory.get_kernel(kernels.Activation8bitParams(dtype, activation, bool(kept)), device)
     if kernel is None:
         return None
     kernel.in_plans = True
     spec = kernel.kernel_spec
+    if spec.values_per_workgroup:
+        return [_stage(kernel.function, spec.launch_params)], spec.values_per_workgroup, False, kernel
     stages = [_stage(kernel.function, spec.launch_params)]
     if kernel.epilogue_function is not None:
         stages.append(_stage(kernel.epilogue_function, spec.epilogue_launch_params))
@@ -155,6 +169,19 @@ def adopt(op, native_name):
         return
     op.__class__ = NativeOp
     op.native = getattr(_native, native_name)
+
+
+def call(name, *args):
+    """What the native path `name` returns for these arguments; NotImplemented where it stands aside."""
+    if _native is None or torch.compiler.is_compiling():
+        return NotImplemented
+    return getattr(_native, name)(*args)
+
+
+def configure_kept(group_norm_gradients, activation_gradient):
+    """What the backward passes of group_norm_2d and activation_8bit hand over to where they stand aside."""
+    if _native is not None:
+        _native.configure_kept(group_norm_gradients, activation_gradient)
 
 
 def configure(backward_op, norm_gradients):

@@ -114,7 +114,7 @@ def test_every_kind_of_configuration(shape, groups, kept):
             for width in sorted({32, 64, 160, c}):
                 for split in (0, 1):
                     config = GroupNorm2dConfig(threads, units, width, split)
-                    if not is_legal(params, config) or (threads, units) not in ((256, 1), (256, 8), (512, 11), (1024, 3)):
+                    if not is_legal(params, config) or (threads, units) not in ((256, 1), (256, 8), (512, 3), (512, 11), (1024, 3)):
                         continue
                     tried += 1
                     forward = group_norm_2d_kernel_factory.make_kernel(params, config)
@@ -134,7 +134,7 @@ def test_every_kind_of_configuration(shape, groups, kept):
                     _check([y, dx, sums[0], sums[1]], x, dy, groups, weight, bias, "silu", kept, HALF, str(config))
                     for kernel in (forward, backward):
                         kernel.unload()
-    assert tried >= 8
+    assert tried >= 6
 
 
 def _call(x, groups, weight, bias, dy, act="silu", kept=False):

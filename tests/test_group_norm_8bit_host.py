@@ -127,7 +127,13 @@ def test_illegal_configurations_are_refused():
             params_bad = dataclasses.replace(params, **bad)
             group_norm_2d_kernel_factory.get_kernel_spec(params_bad, config, ATTR)
     with pytest.raises(AssertionError):
-        activation_8bit_kernel_factory.get_kernel_spec(Activation8bitParams(0), Activation8bitConfig(), ATTR)
+        activation_8bit_kernel_factory.get_kernel_spec(Activation8bitParams(3), Activation8bitConfig(), ATTR)
+    spec = activation_8bit_kernel_factory.get_kernel_spec(Activation8bitParams(), Activation8bitConfig(256, 4), ATTR)
+    assert [spec.grid((n,))[0] for n in (1, 8192, 8193)] == [1, 1, 2]
+    with pytest.raises(AssertionError):
+        spec.grid((0,))
+    with pytest.raises(AssertionError):
+        spec.grid((1 << 38,))
 
 
 def test_names_leave_out_the_images():
