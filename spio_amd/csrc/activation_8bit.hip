@@ -91,6 +91,7 @@ SPIO_KERNEL_NAME(
     const pw_rsrc rs_codes = pw::buffer(codes + first * 8, kReadsCodes || kWritesCodes ? whole * 8 : 0);
     const pw_rsrc rs_exp = pw::buffer(exponents + first / 4, kReadsCodes || kWritesCodes ? (values + 31) / 32 : 0);
 
+    const pw::Constants constants;
     pw::Unit v[UN];
     pw_uint2 c[UN];
     unsigned ex[UN];
@@ -120,23 +121,23 @@ SPIO_KERNEL_NAME(
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
         const int unit = u * THREADS + tid;
-        float x[8], y[8];
-        if (kReadsValues) pw::unpack(x, v[u]);
         if (kWritesCodes) {
             ex[u] = pw::block_exponent(v[u]);
-            c[u] = pw::encode(x, ex[u]);
+            c[u] = pw::encode(v[u], ex[u]);
             __builtin_amdgcn_raw_buffer_store_b64(c[u], rs_codes, unit * 8, 0, pw::STREAM);
             __builtin_amdgcn_raw_buffer_store_b8((unsigned char)ex[u], rs_exp, tid % 4 == 0 ? unit / 4 : (int)pw::OOB, 0, 0);
         }
         if (kWritesValues) {
-            if (kReadsCodes) {
-                float kept[8];
-                pw::decode(kept, c[u], pw::block_step(ex[u]));
+            float y[8];
+            const float step = kReadsCodes ? pw::block_step(ex[u]) : 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = SPIO_MODE == 1 ? pw::activate_grad(x[e], kept[e]) : finite(kept[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = pw::activate(x[e]);
+            for (int e = 0; e < 8; ++e) {
+                if (SPIO_MODE == 1)
+                    y[e] = pw::activate_grad(v[u], e, pw::code(c[u], e) * step, constants);
+                else if (SPIO_MODE == 3)
+                    y[e] = finite(pw::code(c[u], e) * step);
+                else
+                    y[e] = pw::activate(pw::value(v[u], e));
             }
             v[u] = pw::pack(y);
             pw::store_unit<pw::STREAM>(rs_out, unit * pw::UNIT_BYTES, v[u]);

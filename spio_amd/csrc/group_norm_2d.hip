@@ -18,65 +18,78 @@ namespace {
 
 using namespace gn;
 
-struct Chunk {
-    pw::Unit v[UN];
-    unsigned off[UN];
-    int pixels;         // of the stretch from its first on
-    long long first;    // pixel of the tensor that the offsets start from
+constexpr unsigned STEP = (unsigned)(ROWS * C) * pw::VALUE_BYTES;
+
+// A stretch of an image (all of it where images are whole)
+struct Stretch {
+    int pixels;         // from its first on
+    unsigned off;       // of the lane's first unit; the others follow STEP apart
+    long long first;    // pixel of the tensors that the offsets start from
+    pw_rsrc in;
 };
 
-template <int POLICY>
-PW_DEVICE void load_chunk(Chunk& c, const void* in, const Place& p, long long pixels) {
+PW_DEVICE Stretch stretch_of(const void* in, const Place& p, long long pixels) {
     const long long begin = SPIO_GN_SPLIT ? (long long)p.stretch * SPAN : 0;
     const long long left = pixels - begin;
-    c.pixels = (int)(left < SPAN ? left : SPAN);
-    c.first = p.image * pixels + begin;
-    const pw_rsrc rs = pw::buffer(reinterpret_cast<const unsigned char*>(in) + c.first * (C * pw::VALUE_BYTES),
-                                  (unsigned)c.pixels * (C * pw::VALUE_BYTES));
+    Stretch s;
+    s.pixels = (int)(left < SPAN ? left : SPAN);
+    s.first = p.image * pixels + begin;
+    s.off = p.live ? (unsigned)(p.row * C + p.channel) * pw::VALUE_BYTES : pw::OOB;
+    s.in = pw::buffer(reinterpret_cast<const unsigned char*>(in) + s.first * (C * pw::VALUE_BYTES),
+                      (unsigned)s.pixels * (C * pw::VALUE_BYTES));
+    return s;
+}
+
+// Units [0, COUNT) of it
+template <int COUNT, int POLICY>
+PW_DEVICE void load_units(pw::Unit (&v)[COUNT], const Stretch& s) {
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-        const int pixel = p.row + u * ROWS;
-        c.off[u] = p.live ? (unsigned)(pixel * C + p.channel) * pw::VALUE_BYTES : pw::OOB;
-        c.v[u] = pw::load_unit<POLICY>(rs, c.off[u]);
-    }
+    for (int u = 0; u < COUNT; ++u) v[u] = pw::load_unit<POLICY>(s.in, s.off + u * STEP);
+}
+PW_DEVICE void keep_packed(pw::Unit (&v)[UN]) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) pw::keep_packed(v[u]);
 }
 
 // mean[] and squares[] (sum of squared differences to it) of the groups of a chunk.
-PW_DEVICE void moments(const Chunk& c, const Place& p, float* red, float* mean, float* squares) {
+PW_DEVICE void moments(pw::Unit (&v)[UN], const Stretch& c, const Place& p, const pw::Constants& k, float* red, float* mean, float* squares) {
     float s[KEYS] = {};
 #pragma unroll
     for (int u = 0; u < UN; ++u) {  // what lies behind the last pixel is zero
-        float x[8];
-        pw::unpack(x, c.v[u]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e / KEY_CHANNELS] += x[e];
+        for (int e = 0; e < 8; ++e) s[e / KEY_CHANNELS] = pw::plus(v[u], e, s[e / KEY_CHANNELS], k);
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) asm volatile("" : "+v"(s[i]));  // a unit is worked on when it is there, not when all are
     }
     group_sums(s, p, red, mean);
-    const float count = 1.f / ((float)c.pixels * CG);
+    keep_packed(v);
+    const float count = pw::reciprocal((float)c.pixels * CG);
     float m[KEYS];
 #pragma unroll
-    for (int k = 0; k < KEYS; ++k) {
-        m[k] = mean[group_of(p, k) < GS ? group_of(p, k) : 0] * count;
-        s[k] = 0.f;
+    for (int i = 0; i < KEYS; ++i) {
+        m[i] = mean[group_of(p, i) < GS ? group_of(p, i) : 0] * count;
+        s[i] = 0.f;
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
         if (p.live && p.row + u * ROWS < c.pixels) {
-            float x[8];
-            pw::unpack(x, c.v[u]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float d = x[e] - m[e / KEY_CHANNELS];
+                const float d = pw::plus(v[u], e, -m[e / KEY_CHANNELS], k);
                 s[e / KEY_CHANNELS] = __builtin_fmaf(d, d, s[e / KEY_CHANNELS]);
             }
         }
     }
     group_sums(s, p, red, squares);
+    keep_packed(v);
 }
 
-// out and the checkpoint of a chunk, from the lanes' means and rstds by key
-PW_DEVICE void apply(const Chunk& c, const Place& p, void* out, unsigned char* codes, unsigned char* exponents,
-                     const float (&mean)[KEYS], const float (&rstd)[KEYS], const float (&w)[8], const float (&b)[8]) {
+// out and the checkpoint of a stretch, from the lanes' means and rstds by key.  `v` holds its first COUNT units; the others
+// follow as these are done with.
+template <int COUNT>
+PW_DEVICE void apply(pw::Unit (&v)[COUNT], const Stretch& c, const Place& p, const pw::Constants& k, void* out,
+                     unsigned char* codes, unsigned char* exponents, const float (&mean)[KEYS], const float (&rstd)[KEYS],
+                     const float (&w)[8], const float (&b)[8]) {
     const unsigned bytes = (unsigned)c.pixels * (C * pw::VALUE_BYTES);
     const pw_rsrc rs_out = pw::buffer(reinterpret_cast<unsigned char*>(out) + c.first * (C * pw::VALUE_BYTES), bytes);
     const pw_rsrc rs_codes = pw::buffer(codes + c.first * C, SPIO_GN_KEPT ? (unsigned)c.pixels * C : 0);
@@ -84,29 +97,31 @@ PW_DEVICE void apply(const Chunk& c, const Place& p, void* out, unsigned char* c
     float scale[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) scale[e] = rstd[e / KEY_CHANNELS] * (SPIO_GN_HAS_WEIGHT ? w[e] : 1.f);
+    // (the codes and exponents of lanes without any are stored behind the end of theirs)
+    const unsigned off_codes = p.live ? (unsigned)(p.row * C + p.channel) : pw::OOB;
+    const unsigned off_exp = p.live && p.tid % 4 == 0 ? (unsigned)(p.row * BLOCKS + p.channel / 32) : pw::OOB;
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-        float x[8], y[8];
-        pw::unpack(x, c.v[u]);
+        const pw::Unit x = v[u % COUNT];
+        float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float d = x[e] - mean[e / KEY_CHANNELS];
+            const float d = pw::plus(x, e, -mean[e / KEY_CHANNELS], k);
             y[e] = pw::activate(SPIO_GN_HAS_BIAS ? __builtin_fmaf(d, scale[e], b[e]) : d * scale[e]);
         }
-        pw::store_unit<pw::STREAM>(rs_out, c.off[u], pw::pack(y));
+        pw::store_unit<pw::STREAM>(rs_out, c.off + u * STEP, pw::pack(y));
         if (SPIO_GN_KEPT) {
-            const int pixel = p.row + u * ROWS;
-            const unsigned ex = pw::block_exponent(c.v[u]);
-            const pw_uint2 code = pw::encode(x, ex);
-            __builtin_amdgcn_raw_buffer_store_b64(code, rs_codes, p.live ? pixel * C + p.channel : (int)pw::OOB, 0, pw::STREAM);
-            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)ex, rs_exp,
-                                                 p.live && p.tid % 4 == 0 ? pixel * BLOCKS + p.channel / 32 : (int)pw::OOB, 0, 0);
+            const unsigned ex = pw::block_exponent(x);
+            __builtin_amdgcn_raw_buffer_store_b64(pw::encode(x, ex), rs_codes, (int)(off_codes + u * (ROWS * C)), 0, pw::STREAM);
+            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)ex, rs_exp, (int)(off_exp + u * (ROWS * BLOCKS)), 0, 0);
         }
+        if (u + COUNT < UN) v[u % COUNT] = pw::load_unit<pw::STREAM>(c.in, c.off + (u + COUNT) * STEP);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
 PW_DEVICE float inverse_deviation(float squares, long long pixels) {
-    return __builtin_amdgcn_rsqf(squares * (1.f / ((float)pixels * CG)) + SPIO_GN_EPS);
+    return __builtin_amdgcn_rsqf(squares * (pw::reciprocal((float)pixels * CG)) + SPIO_GN_EPS);
 }
 
 }  // namespace
@@ -123,19 +138,21 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(void* __restrict__ out, unsigned char* __restric
                                 const float* __restrict__ bias, long long pixels, long long) {
     __shared__ float red[RED_FLOATS], sum[GS], squares[GS];
     const Place p = place(__builtin_amdgcn_workgroup_id_x(), 1);
-    Chunk c;
-    load_chunk<pw::STREAM>(c, in, p, pixels);
+    const pw::Constants k;
+    const Stretch c = stretch_of(in, p, pixels);
+    pw::Unit v[UN];
+    load_units<UN, pw::STREAM>(v, c);
     float w[8] = {}, b[8] = {};
     if (SPIO_GN_HAS_WEIGHT) load_vector(w, weight, p);
     if (SPIO_GN_HAS_BIAS) load_vector(b, bias, p);
-    moments(c, p, red, sum, squares);
-    const float count = 1.f / ((float)pixels * CG);
+    moments(v, c, p, k, red, sum, squares);
+    const float count = pw::reciprocal((float)pixels * CG);
     float mean[KEYS], rstd[KEYS];
 #pragma unroll
-    for (int k = 0; k < KEYS; ++k) {
-        const int g = group_of(p, k) < GS ? group_of(p, k) : 0;
-        mean[k] = sum[g] * count;
-        rstd[k] = inverse_deviation(squares[g], pixels);
+    for (int i = 0; i < KEYS; ++i) {
+        const int g = group_of(p, i) < GS ? group_of(p, i) : 0;
+        mean[i] = sum[g] * count;
+        rstd[i] = inverse_deviation(squares[g], pixels);
     }
     if (stats)
         for (int g = p.tid; g < GS && p.slice * GS + g < GROUPS; g += THREADS) {
@@ -143,7 +160,7 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(void* __restrict__ out, unsigned char* __restric
             s[0] = sum[g] * count;
             s[1] = inverse_deviation(squares[g], pixels);
         }
-    apply(c, p, out, codes, exponents, mean, rstd, w, b);
+    apply(v, c, p, k, out, codes, exponents, mean, rstd, w, b);
 }
 
 #else
@@ -154,10 +171,12 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(void*, unsigned char*, unsigned char*, float* __
     __shared__ float red[RED_FLOATS], sum[GS], squares[GS];
     const unsigned stretches = (unsigned)((pixels + SPAN - 1) / SPAN);
     const Place p = place(__builtin_amdgcn_workgroup_id_x(), stretches);
-    Chunk c;
-    load_chunk<0>(c, in, p, pixels);
-    moments(c, p, red, sum, squares);
-    const float count = 1.f / ((float)c.pixels * CG);
+    const pw::Constants k;
+    const Stretch c = stretch_of(in, p, pixels);
+    pw::Unit v[UN];
+    load_units<UN, 0>(v, c);
+    moments(v, c, p, k, red, sum, squares);
+    const float count = pw::reciprocal((float)c.pixels * CG);
     for (int g = p.tid; g < GS && p.slice * GS + g < GROUPS; g += THREADS) {
         float* s = partials + (((long long)p.image * GROUPS + p.slice * GS + g) * stretches + p.stretch) * 2;
         s[0] = sum[g] * count;
@@ -168,13 +187,14 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(void*, unsigned char*, unsigned char*, float* __
 SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
     float* __restrict__ stats, const float* __restrict__ partials, void* __restrict__ out,
     unsigned char* __restrict__ codes, unsigned char* __restrict__ exponents, const void* __restrict__ in,
-    const float* __restrict__ weight, const float* __restrict__ bias, long long pixels, long long images) {
+    const float* __restrict__ weight, const float* __restrict__ bias, long long pixels, long long) {
     __shared__ float means[GS], rstds[GS];
     const unsigned stretches = (unsigned)((pixels + SPAN - 1) / SPAN);
-    // the last stretches first: the first launch read them last
-    const Place p = place((unsigned)images * stretches * SLICES - 1 - __builtin_amdgcn_workgroup_id_x(), stretches);
-    Chunk c;
-    load_chunk<pw::STREAM>(c, in, p, pixels);
+    const Place p = place(__builtin_amdgcn_workgroup_id_x(), stretches);
+    const pw::Constants k;
+    const Stretch c = stretch_of(in, p, pixels);
+    pw::Unit v[DEPTH];
+    load_units<DEPTH, pw::STREAM>(v, c);
     float w[8] = {}, b[8] = {};
     if (SPIO_GN_HAS_WEIGHT) load_vector(w, weight, p);
     if (SPIO_GN_HAS_BIAS) load_vector(b, bias, p);
@@ -217,12 +237,12 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
     sync();
     float mean[KEYS], rstd[KEYS];
 #pragma unroll
-    for (int k = 0; k < KEYS; ++k) {
-        const int g = group_of(p, k) < GS ? group_of(p, k) : 0;
-        mean[k] = means[g];
-        rstd[k] = rstds[g];
+    for (int i = 0; i < KEYS; ++i) {
+        const int g = group_of(p, i) < GS ? group_of(p, i) : 0;
+        mean[i] = means[g];
+        rstd[i] = rstds[g];
     }
-    apply(c, p, out, codes, exponents, mean, rstd, w, b);
+    apply(v, c, p, k, out, codes, exponents, mean, rstd, w, b);
 }
 
 #endif

@@ -21,62 +21,89 @@ namespace {
 
 using namespace gn;
 
-struct Input {  // the norm's input as the backward pass has it
+struct Inputs {  // a unit of the norm's input, as the backward pass has it, and of grad_output
 #if SPIO_GN_KEPT
     pw_uint2 code;
     unsigned exponent;
 #else
-    pw::Unit v;
+    pw::Unit x;
 #endif
+    pw::Unit dy;
 };
 
-struct Chunk {
-    Input x[UN];
-    pw::Unit dy[UN];
-    unsigned off[UN];
-    int pixels;
-    long long first;
+constexpr unsigned STEP = (unsigned)(ROWS * C) * pw::VALUE_BYTES;
+
+// A stretch of an image (all of it where images are whole)
+struct Stretch {
+    int pixels;         // from its first on
+    unsigned off;       // of the lane's first unit; the others follow STEP apart
+    unsigned off_codes, off_exp;
+    long long first;    // pixel of the tensors that the offsets start from
+    pw_rsrc in, exponents, dout;
 };
 
-template <int POLICY>
-PW_DEVICE void load_chunk(Chunk& c, const void* in, const unsigned char* exponents, const void* dout, const Place& p,
-                          long long pixels) {
+PW_DEVICE Stretch stretch_of(const void* in, const unsigned char* exponents, const void* dout, const Place& p,
+                             long long pixels) {
     const long long begin = SPIO_GN_SPLIT ? (long long)p.stretch * SPAN : 0;
     const long long left = pixels - begin;
-    c.pixels = (int)(left < SPAN ? left : SPAN);
-    c.first = p.image * pixels + begin;
     constexpr int IN_BYTES = SPIO_GN_KEPT ? 1 : pw::VALUE_BYTES;
-    const pw_rsrc rs_in = pw::buffer(reinterpret_cast<const unsigned char*>(in) + c.first * (C * IN_BYTES),
-                                     (unsigned)c.pixels * (C * IN_BYTES));
-    const pw_rsrc rs_exp = pw::buffer(exponents + c.first * BLOCKS, SPIO_GN_KEPT ? (unsigned)c.pixels * BLOCKS : 0);
-    const pw_rsrc rs_dout = pw::buffer(reinterpret_cast<const unsigned char*>(dout) + c.first * (C * pw::VALUE_BYTES),
-                                       (unsigned)c.pixels * (C * pw::VALUE_BYTES));
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-        const int pixel = p.row + u * ROWS;
-        c.off[u] = p.live ? (unsigned)(pixel * C + p.channel) * pw::VALUE_BYTES : pw::OOB;
+    Stretch s;
+    s.pixels = (int)(left < SPAN ? left : SPAN);
+    s.first = p.image * pixels + begin;
+    s.off = p.live ? (unsigned)(p.row * C + p.channel) * pw::VALUE_BYTES : pw::OOB;
+    s.off_codes = p.live ? (unsigned)(p.row * C + p.channel) : pw::OOB;
+    s.off_exp = p.live ? (unsigned)(p.row * BLOCKS + p.channel / 32) : pw::OOB;
+    s.in = pw::buffer(reinterpret_cast<const unsigned char*>(in) + s.first * (C * IN_BYTES), (unsigned)s.pixels * (C * IN_BYTES));
+    s.exponents = pw::buffer(exponents + s.first * BLOCKS, SPIO_GN_KEPT ? (unsigned)s.pixels * BLOCKS : 0);
+    s.dout = pw::buffer(reinterpret_cast<const unsigned char*>(dout) + s.first * (C * pw::VALUE_BYTES),
+                        (unsigned)s.pixels * (C * pw::VALUE_BYTES));
+    return s;
+}
+
+template <int POLICY>
+PW_DEVICE Inputs load_inputs(const Stretch& s, int u) {
+    Inputs in;
 #if SPIO_GN_KEPT
-        c.x[u].code = __builtin_amdgcn_raw_buffer_load_b64(rs_in, p.live ? pixel * C + p.channel : (int)pw::OOB, 0, POLICY);
-        c.x[u].exponent = __builtin_amdgcn_raw_buffer_load_b8(
-            rs_exp, p.live ? pixel * BLOCKS + p.channel / 32 : (int)pw::OOB, 0, 0);
+    in.code = __builtin_amdgcn_raw_buffer_load_b64(s.in, (int)(s.off_codes + u * (ROWS * C)), 0, POLICY);
+    in.exponent = __builtin_amdgcn_raw_buffer_load_b8(s.exponents, (int)(s.off_exp + u * (ROWS * BLOCKS)), 0, 0);
 #else
-        c.x[u].v = pw::load_unit<POLICY>(rs_in, c.off[u]);
+    in.x = pw::load_unit<POLICY>(s.in, s.off + u * STEP);
 #endif
-        c.dy[u] = pw::load_unit<POLICY>(rs_dout, c.off[u]);
+    in.dy = pw::load_unit<POLICY>(s.dout, s.off + u * STEP);
+    return in;
+}
+
+// How many of a stretch's units a lane has in registers: all where it works on them twice.
+constexpr int HELD = SPIO_GN_SPLIT ? DEPTH : UN;
+
+template <int POLICY>
+PW_DEVICE void load_first(Inputs (&in)[HELD], const Stretch& s) {
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) in[u] = load_inputs<POLICY>(s, u);
+}
+// The next one in place of one that is done with
+template <int POLICY>
+PW_DEVICE void load_next(Inputs (&in)[HELD], const Stretch& s, int u) {
+    if (u + HELD < UN) in[u % HELD] = load_inputs<POLICY>(s, u + HELD);
+    __builtin_amdgcn_sched_barrier(0);  // a unit is worked on when it is there, not when all are
+}
+
+PW_DEVICE void keep_packed(Inputs (&in)[HELD]) {
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) {
+#if SPIO_GN_KEPT
+        asm volatile("" : "+v"(in[u].code), "+v"(in[u].exponent));
+#else
+        pw::keep_packed(in[u].x);
+#endif
+        pw::keep_packed(in[u].dy);
     }
 }
 
-PW_DEVICE void input_values(float (&x)[8], const Input& in) {
-#if SPIO_GN_KEPT
-    pw::decode(x, in.code, pw::block_step(in.exponent));
-#else
-    pw::unpack(x, in.v);
-#endif
-}
-
-struct Lane {  // a lane's eight channels
-    float w[8], b[8];
+struct Lane {  // a lane's eight channels: z = (x - mean) * scale + bias
+    float w[8], scale[8], b[8];
     float mean[KEYS], rstd[KEYS];
+    pw::Constants k;
 };
 
 PW_DEVICE void load_lane(Lane& l, const float* stats, const float* weight, const float* bias, const Place& p) {
@@ -91,46 +118,57 @@ PW_DEVICE void load_lane(Lane& l, const float* stats, const float* weight, const
 #pragma unroll
         for (int e = 0; e < 8; ++e) l.b[e] = 0.f;
 #pragma unroll
-    for (int k = 0; k < KEYS; ++k) {
-        const int g = p.slice * GS + group_of(p, k);
+    for (int i = 0; i < KEYS; ++i) {
+        const int g = p.slice * GS + group_of(p, i);
         const float* s = stats + ((long long)p.image * GROUPS + (p.live ? g : 0)) * 2;
-        l.mean[k] = s[0];
-        l.rstd[k] = s[1];
+        l.mean[i] = s[0];
+        l.rstd[i] = s[1];
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l.scale[e] = l.w[e] * l.rstd[e / KEY_CHANNELS];
 }
 
-// xhat and dz of a unit (what lies behind the last pixel has dy = 0, and with it dz)
-PW_DEVICE void work(float (&xhat)[8], float (&dz)[8], const Chunk& c, int u, const Lane& l) {
-    float x[8], dy[8];
-    input_values(x, c.x[u]);
-    pw::unpack(dy, c.dy[u]);
+// x - mean and dz of a unit (what lies behind the last pixel has dy = 0, and with it dz)
+PW_DEVICE void work(float (&d)[8], float (&dz)[8], const Inputs& in, const Lane& l) {
+#if SPIO_GN_KEPT
+    const float step = pw::block_step(in.exponent);
+#endif
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        xhat[e] = (x[e] - l.mean[e / KEY_CHANNELS]) * l.rstd[e / KEY_CHANNELS];
-        dz[e] = pw::activate_grad(dy[e], __builtin_fmaf(xhat[e], l.w[e], l.b[e]));
+#if SPIO_GN_KEPT
+        d[e] = __builtin_fmaf(pw::code(in.code, e), step, -l.mean[e / KEY_CHANNELS]);
+#else
+        d[e] = pw::plus(in.x, e, -l.mean[e / KEY_CHANNELS], l.k);
+#endif
+        const float z = SPIO_GN_HAS_BIAS ? __builtin_fmaf(d[e], l.scale[e], l.b[e]) : d[e] * l.scale[e];
+        dz[e] = pw::activate_grad(in.dy, e, z, l.k);
     }
 }
 
-// The chunk's sums of dz and of dz * xhat: [which][channel of the slice] in `red`, and in `row`, those of dz * xhat first.
+// The stretch's sums of dz and of dz * xhat: [which][channel of the slice] in `red`, and in `row`, those of dz * xhat first.
 constexpr int WIDTH = SUP * 8;
 constexpr int COLUMNS = 2 * WIDTH;
 constexpr int PARTS = THREADS / COLUMNS > 1 ? THREADS / COLUMNS : 1;  // threads that share a column
 constexpr int RED = SUM_ROWS * COLUMNS > PARTS * COLUMNS ? SUM_ROWS * COLUMNS : PARTS * COLUMNS;
 
-PW_DEVICE void channel_sums(const Chunk& c, const Place& p, const Lane& l, float* red, float* row) {
+template <int POLICY>
+PW_DEVICE void channel_sums(Inputs (&in)[HELD], const Stretch& c, const Place& p, const Lane& l, float* red, float* row) {
     float s1[8] = {}, s2[8] = {};
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-        if (p.live && p.row + u * ROWS < c.pixels) {
-            float xhat[8], dz[8];
-            work(xhat, dz, c, u, l);
+        float d[8], dz[8];
+        work(d, dz, in[u % HELD], l);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                s1[e] += dz[e];
-                s2[e] = __builtin_fmaf(dz[e], xhat[e], s2[e]);
-            }
+        for (int e = 0; e < 8; ++e) {
+            s1[e] += dz[e];
+            s2[e] = __builtin_fmaf(dz[e], d[e], s2[e]);
+            asm volatile("" : "+v"(s1[e]), "+v"(s2[e]));  // (now: all units' sums would be put off behind the last load)
         }
+        load_next<POLICY>(in, c, u);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s2[e] *= l.rstd[e / KEY_CHANNELS];
+    if (!SPIO_GN_SPLIT) keep_packed(in);
     if (kFold) {
 #pragma unroll
         for (int m = SUP; m < 64; m <<= 1)
@@ -207,28 +245,29 @@ PW_DEVICE void group_pairs(const Place& p, const float* red, float* pairs, const
     sync();
 }
 
-PW_DEVICE void apply(const Chunk& c, const Place& p, const Lane& l, void* din, const float* pairs, long long pixels) {
+PW_DEVICE void apply(Inputs (&in)[HELD], const Stretch& c, const Place& p, const Lane& l, void* din, const float* pairs, long long pixels) {
     const pw_rsrc rs = pw::buffer(reinterpret_cast<unsigned char*>(din) + c.first * (C * pw::VALUE_BYTES),
                                   (unsigned)c.pixels * (C * pw::VALUE_BYTES));
-    const float count = 1.f / ((float)pixels * CG);
-    float m1[KEYS], m2[KEYS];
+    const float count = pw::reciprocal((float)pixels * CG);
+    // rstd * (dz * w - m1 - xhat * m2) = dz * scale + c1 + (x - mean) * c2
+    float c1[KEYS], c2[KEYS];
 #pragma unroll
-    for (int k = 0; k < KEYS; ++k) {
-        const int g = group_of(p, k) < GS ? group_of(p, k) : 0;
-        m1[k] = pairs[g] * count;
-        m2[k] = pairs[GS + g] * count;
+    for (int i = 0; i < KEYS; ++i) {
+        const int g = group_of(p, i) < GS ? group_of(p, i) : 0;
+        c1[i] = -l.rstd[i] * (pairs[g] * count);
+        c2[i] = -l.rstd[i] * l.rstd[i] * (pairs[GS + g] * count);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-        float xhat[8], dz[8], dx[8];
-        work(xhat, dz, c, u, l);
+        float d[8], dz[8], dx[8];
+        work(d, dz, in[u % HELD], l);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int k = e / KEY_CHANNELS;
-            const float g = SPIO_GN_HAS_WEIGHT ? __builtin_fmaf(dz[e], l.w[e], -m1[k]) : dz[e] - m1[k];
-            dx[e] = l.rstd[k] * __builtin_fmaf(xhat[e], -m2[k], g);
+            const int i = e / KEY_CHANNELS;
+            dx[e] = __builtin_fmaf(dz[e], l.scale[e], __builtin_fmaf(d[e], c2[i], c1[i]));
         }
-        pw::store_unit<pw::STREAM>(rs, c.off[u], pw::pack(dx));
+        pw::store_unit<pw::STREAM>(rs, c.off + u * STEP, pw::pack(dx));
+        load_next<pw::STREAM>(in, c, u);
     }
 }
 
@@ -275,13 +314,14 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(float* __restrict__ rows, void* __restrict__ din
                                 const float* __restrict__ bias, long long pixels, long long) {
     __shared__ float red[RED], pairs[2 * GS];
     const Place p = place(__builtin_amdgcn_workgroup_id_x(), 1);
-    Chunk c;
-    load_chunk<pw::STREAM>(c, in, exponents, dout, p, pixels);
+    const Stretch c = stretch_of(in, exponents, dout, p, pixels);
+    Inputs held[HELD];
+    load_first<pw::STREAM>(held, c);
     Lane l;
     load_lane(l, stats, weight, bias, p);
-    channel_sums(c, p, l, red, rows + (long long)p.image * (2 * C));
+    channel_sums<pw::STREAM>(held, c, p, l, red, rows + (long long)p.image * (2 * C));
     group_pairs(p, red, pairs, weight);
-    apply(c, p, l, din, pairs, pixels);
+    apply(held, c, p, l, din, pairs, pixels);
 }
 
 #if SPIO_GN_AFFINE
@@ -302,11 +342,12 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(float* __restrict__ rows, void*, const void* __r
     __shared__ float red[RED], pairs[2 * GS];
     const unsigned stretches = (unsigned)((pixels + SPAN - 1) / SPAN);
     const Place p = place(__builtin_amdgcn_workgroup_id_x(), stretches);
-    Chunk c;
-    load_chunk<0>(c, in, exponents, dout, p, pixels);
+    const Stretch c = stretch_of(in, exponents, dout, p, pixels);
+    Inputs held[HELD];
+    load_first<0>(held, c);
     Lane l;
     load_lane(l, stats, weight, bias, p);
-    channel_sums(c, p, l, red, rows + ((long long)p.image * stretches + p.stretch) * (2 * C));
+    channel_sums<0>(held, c, p, l, red, rows + ((long long)p.image * stretches + p.stretch) * (2 * C));
     group_pairs(p, red, pairs, weight);
     float* out = rows + (SPIO_GN_AFFINE ? images * stretches * (2 * C) : 0);
     for (int i = p.tid; i < 2 * GS; i += THREADS) {
@@ -326,10 +367,10 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
         add_rows(sums, rows, images * stretches, (int)block, pairs);
         return;
     }
-    // the last stretches first: the first launch read them last
-    const Place p = place((unsigned)images * stretches * SLICES - 1 - (block - ADDING), stretches);
-    Chunk c;
-    load_chunk<pw::STREAM>(c, in, exponents, dout, p, pixels);
+    const Place p = place(block - ADDING, stretches);
+    const Stretch c = stretch_of(in, exponents, dout, p, pixels);
+    Inputs held[HELD];
+    load_first<pw::STREAM>(held, c);
     Lane l;
     load_lane(l, stats, weight, bias, p);
     const float* parts = rows + (SPIO_GN_AFFINE ? images * stretches * (2 * C) : 0);
@@ -355,7 +396,7 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
         }
     }
     sync();
-    apply(c, p, l, din, pairs, pixels);
+    apply(held, c, p, l, din, pairs, pixels);
 }
 
 #endif

@@ -55,6 +55,11 @@ constexpr int WAVES = THREADS / 64;
 constexpr int BLOCKS = (C + 31) / 32;           // exponents of a pixel
 static_assert(C % 8 == 0 && C % GROUPS == 0 && SLICE % 8 == 0 && SLICE % CG == 0 && SLICE <= C, "bad geometry");
 static_assert(SLICE == C || SLICE % 32 == 0, "a block lies in one slice");
+// Units that a lane has under way where it does not hold on to them
+#ifndef SPIO_GN_DEPTH
+#define SPIO_GN_DEPTH 3
+#endif
+constexpr int DEPTH = SPIO_GN_DEPTH < UN ? SPIO_GN_DEPTH : UN;
 static_assert(THREADS % 64 == 0 && ROWS >= 1, "bad geometry");
 
 // A lane's eight channels as the groups divide them: KEYS values for it, KEY_CHANNELS channels each, all of one group.
@@ -101,10 +106,17 @@ PW_DEVICE Place place(unsigned block, unsigned stretches) {
 
 // Sums over the workgroup of a lane's values for its KEYS keys: `sums[group of the slice]`, in the same order
 // always.  Lanes that are not live have zeros.  `red` may be used again after the next barrier.
-constexpr int RED_FLOATS = SUM_ROWS * SUP * KEYS;
+// (rows an odd number of 16 bytes apart: lanes that read one column of several rows meet different banks)
+constexpr int RED_PITCH = ((SUP * KEYS + 3) / 4 | 1) * 4;
+constexpr int RED_FLOATS = SUM_ROWS * RED_PITCH;
 constexpr int group_lanes() {
     int lanes = 64;
     while (lanes > 1 && lanes * GS > THREADS) lanes /= 2;
+    return lanes;
+}
+constexpr int key_lanes() {
+    int lanes = 1;
+    while (2 * lanes <= GROUP_KEYS && group_lanes() / lanes > SUM_ROWS) lanes *= 2;
     return lanes;
 }
 PW_DEVICE void group_sums(float (&v)[KEYS], const Place& p, float* red, float* sums) {
@@ -115,18 +127,25 @@ PW_DEVICE void group_sums(float (&v)[KEYS], const Place& p, float* red, float* s
             for (int k = 0; k < KEYS; ++k) v[k] += lane_xor(v[k], m);
         if ((p.tid & 63) < SUP)
 #pragma unroll
-            for (int k = 0; k < KEYS; ++k) red[(p.tid >> 6) * (SUP * KEYS) + p.sub * KEYS + k] = v[k];
+            for (int k = 0; k < KEYS; ++k) red[(p.tid >> 6) * RED_PITCH + p.sub * KEYS + k] = v[k];
     } else if (p.row < ROWS) {
 #pragma unroll
-        for (int k = 0; k < KEYS; ++k) red[p.row * (SUP * KEYS) + p.sub * KEYS + k] = v[k];
+        for (int k = 0; k < KEYS; ++k) red[p.row * RED_PITCH + p.sub * KEYS + k] = v[k];
     }
     sync();
+    // the lanes of a group share its rows, and its keys where these are fewer
     constexpr int LANES = group_lanes();
+    constexpr int BY_KEY = key_lanes();
+    constexpr int BY_ROW = LANES / BY_KEY;
     const int part = p.tid % LANES;
     for (int g = p.tid / LANES; g < GS; g += THREADS / LANES) {
         float s = 0.f;
-        for (int e = part; e < SUM_ROWS * GROUP_KEYS; e += LANES)
-            s += red[e / GROUP_KEYS * (SUP * KEYS) + g * GROUP_KEYS + e % GROUP_KEYS];
+        for (int r = part / BY_KEY; r < SUM_ROWS; r += BY_ROW) {
+            const float* from = red + r * RED_PITCH + g * GROUP_KEYS + part % BY_KEY;
+#pragma unroll 8
+            for (int e = 0; e < GROUP_KEYS; e += BY_KEY)
+                if (GROUP_KEYS % BY_KEY == 0 || e + part % BY_KEY < GROUP_KEYS) s += from[e];
+        }
 #pragma unroll
         for (int m = 1; m < LANES; m <<= 1) s += lane_xor(s, m);
         if (part == 0) sums[g] = s;

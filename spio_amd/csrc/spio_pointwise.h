@@ -64,41 +64,63 @@ PW_DEVICE void store_unit(pw_rsrc rs, unsigned off, const Unit& u) {
     for (int i = 0; i < QUADS; ++i) __builtin_amdgcn_raw_buffer_store_b128(u.q[i], rs, (int)(off + 16 * i), 0, POLICY);
 }
 
+// What is done with a unit behind this starts from its registers again: values converted ahead of it would take two to
+// four times as many in between.
+PW_DEVICE void keep_packed(Unit& u) {
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) asm volatile("" : "+v"(u.q[i]));
+}
+
+typedef _Float16 pw_half2 __attribute__((ext_vector_type(2)));
+typedef _Float16 pw_half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pw_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float pw_float2 __attribute__((ext_vector_type(2)));
+
+PW_DEVICE float value(const Unit& u, int e) {
+    if (SPIO_DTYPE == 2) return as_float(u.q[e / 4 % QUADS][e % 4]);
+    if (SPIO_DTYPE == 1) return as_float(e % 2 ? u.q[0][e / 2] & 0xffff0000u : u.q[0][e / 2] << 16);
+    return (float)__builtin_bit_cast(pw_half8, u.q[0])[e];
+}
 PW_DEVICE void unpack(float (&v)[8], const Unit& u) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if (SPIO_DTYPE == 2) {
-            v[e] = as_float(u.q[e / 4 % QUADS][e % 4]);
-        } else {
-            const unsigned w = u.q[0][e / 2];
-            if (SPIO_DTYPE == 1)
-                v[e] = as_float(e % 2 ? w & 0xffff0000u : w << 16);
-            else
-                v[e] = (float)__builtin_bit_cast(_Float16, (unsigned short)(e % 2 ? w >> 16 : w));
-        }
-    }
+    for (int e = 0; e < 8; ++e) v[e] = value(u, e);
 }
+// The vector units are what most of these kernels wait for, so instructions count: a float16 value enters a
+// mixed-precision multiply-add instead of being converted, in products with a 1 and sums with a -0 that the compiler
+// does not know for such.
+struct Constants {
+    float one = 1.f, zero = -0.f;
+    PW_DEVICE Constants() { asm("" : "+s"(one), "+s"(zero)); }
+};
+PW_DEVICE float plus(const Unit& u, int e, float c, const Constants& k) {  // value + c
+    return SPIO_DTYPE == 0 ? __builtin_fmaf(value(u, e), k.one, c) : value(u, e) + c;
+}
+PW_DEVICE float times(const Unit& u, int e, float f, const Constants& k) {  // value * f
+    return SPIO_DTYPE == 0 ? __builtin_fmaf(value(u, e), f, k.zero) : value(u, e) * f;
+}
+
 // Rounds to nearest, ties to even.
 PW_DEVICE Unit pack(const float (&v)[8]) {
     Unit u;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
+        const pw_float2 pair = {v[e], v[e + 1]};
         if (SPIO_DTYPE == 2) {
             u.q[e / 4 % QUADS][e % 4] = as_bits(v[e]);
             u.q[e / 4 % QUADS][e % 4 + 1] = as_bits(v[e + 1]);
+        } else if (SPIO_DTYPE == 1) {
+            u.q[0][e / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(pair, pw_bf16x2));
         } else {
-            unsigned short a, b;
-            if (SPIO_DTYPE == 1) {
-                a = __builtin_bit_cast(unsigned short, (__bf16)v[e]);
-                b = __builtin_bit_cast(unsigned short, (__bf16)v[e + 1]);
-            } else {
-                a = __builtin_bit_cast(unsigned short, (_Float16)v[e]);
-                b = __builtin_bit_cast(unsigned short, (_Float16)v[e + 1]);
-            }
-            u.q[0][e / 2] = (unsigned)a | (unsigned)b << 16;
+            u.q[0][e / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(pair, pw_half2));
         }
     }
     return u;
+}
+
+// 1 / v to the last place or nearly
+PW_DEVICE float reciprocal(float v) {
+    const float r = __builtin_amdgcn_rcpf(v);
+    return __builtin_fmaf(__builtin_fmaf(-v, r, 1.f), r, r);
 }
 
 // ---- activations ----
@@ -140,19 +162,19 @@ PW_DEVICE float activate(float z) {
     return z;
 }
 
-// dy times the activation's derivative at z
-PW_DEVICE float activate_grad(float dy, float z) {
-    if (SPIO_ACT == 1) return z > 0.f ? dy : 0.f;
+// value e of dy times the activation's derivative at z
+PW_DEVICE float activate_grad(const Unit& dy, int e, float z, const Constants& k) {
+    if (SPIO_ACT == 1) return z > 0.f ? value(dy, e) : 0.f;
     if (SPIO_ACT == 2) {
         const float s = sigmoid(z);
-        return dy * __builtin_fmaf(z * s, 1.f - s, s);
+        return times(dy, e, __builtin_fmaf(s, __builtin_fmaf(-z, s, z), s), k);  // s + s z (1 - s)
     }
     if (SPIO_ACT == 3) {
         float density, cdf;
         normal(z, density, cdf);
-        return dy * __builtin_fmaf(z, density, cdf);
+        return times(dy, e, __builtin_fmaf(z, density, cdf), k);
     }
-    return dy;
+    return value(dy, e);
 }
 
 // ---- 8-bit form ----
@@ -195,15 +217,19 @@ PW_DEVICE unsigned block_exponent(const Unit& u) {
     return m >= 0x7f800000u ? 255 : in_range;
 }
 // The codes of a unit, by a product and a sum whose low byte is the integer (1.5 * 2^23 has a unit of one there).
-PW_DEVICE pw_uint2 encode(const float (&v)[8], unsigned exponent) {
+PW_DEVICE pw_uint2 encode(Unit u, unsigned exponent) {
     const float inverse = as_float((260u - exponent) << 23);
-    constexpr float limit = 0x1.fcp127f;  // 127 steps of the largest exponent: the few values behind it are held as that
+    if (SPIO_DTYPE != 0 && __builtin_amdgcn_ballot_w64(exponent == 254)) {
+        // values behind 127 steps of the largest exponent are held as that
+        constexpr float limit = 0x1.fcp127f;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_fmed3f(value(u, e), -limit, limit);
+        u = pack(x);
+    }
     unsigned r[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float x = SPIO_DTYPE == 0 ? v[e] : __builtin_amdgcn_fmed3f(v[e], -limit, limit);
-        r[e] = as_bits(__builtin_fmaf(x, inverse, 12582912.f));
-    }
+    for (int e = 0; e < 8; ++e) r[e] = as_bits(__builtin_fmaf(value(u, e), inverse, 12582912.f));
     pw_uint2 codes;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -217,15 +243,11 @@ PW_DEVICE pw_uint2 encode(const float (&v)[8], unsigned exponent) {
 // The step of an exponent byte; NaN for that of a block without a value.
 PW_DEVICE float block_step(unsigned exponent) {
     const unsigned e = exponent < 7 ? 7 : exponent;
-    return exponent == 255 ? as_float(0x7fc00000u) : as_float((e - 6) << 23);
+    unsigned bits = exponent == 255 ? 0x7fc00000u : (e - 6) << 23;
+    asm("" : "+v"(bits));  // (the choice would be made of every value's product instead)
+    return as_float(bits);
 }
-PW_DEVICE void decode(float (&v)[8], const pw_uint2& codes, float step) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const unsigned w = codes[e / 4] ^ 0x80808080u;  // code + 128 as an unsigned byte
-        v[e] = ((float)(w >> 8 * (e % 4) & 0xff) - 128.f) * step;  // (128 steps can be too large a number)
-    }
-}
+PW_DEVICE float code(const pw_uint2& codes, int e) { return (float)(signed char)(codes[e / 4] >> 8 * (e % 4)); }
 
 }  // namespace pw
 

@@ -109,41 +109,86 @@ def _span(params: GroupNorm2dParams, config: GroupNorm2dConfig) -> int:
     return config.threads // _lane_units(params, config.slice) * config.units
 
 
-def _choose(params: GroupNorm2dParams, cus: int, most: int, bwd: bool) -> GroupNorm2dConfig:
-    """`most`: units that a lane holds without its registers running out at 1024 threads."""
+# How a configuration is chosen.  The times of its two kinds were fitted to sweeps of 20 shapes in both directions (1 to
+# 256 images, 64 to 1280 channels, 7x7 to 224x224): a launch, and for every round of workgroups over the device what the
+# units of a workgroup take.  us = LAUNCH + PER_UNIT * rounds * threads * units for whole images, us = LAUNCH +
+# PER_UNIT * units of the tensor / compute units in stretches, where the input is read twice; both for 16-byte units.
+# Whole images win where there are enough of them, us whole and in stretches: forward 128n 384c 14x14 9.5 and 12, 64n
+# 128c 28x28 9.6 and 11.3, 8n 1280c 8x8 5.6 and 6.9, but 4n 256c 32x32 8.5 and 7.1, 64n 192c 20x20 with one group 9.4 and 8.9;
+# backward 128n 384c 14x14 16.8 and 19.4, 32n 192c 28x28 float32 18.2 and 21.0, but 64n 128c 28x28 17.3 and 15.1.
+_WHOLE = {False: (3.2, 1.1e-3), True: (5.4, 1.8e-3)}  # forward; backward, whose sums over images are a launch
+_STRETCHES = {False: (6.0, 1.8e-3), True: (6.0, 2.75e-3)}
+
+
+def _best_whole(params: GroupNorm2dParams, cus: int, bwd: bool):
+    """(cost, configuration) that holds whole images, or None; the cost is rounds * threads * units."""
+    wide = params.dtype == 2
+    value = 4 if wide else 2
+    # units in a lane's registers, of which 1024 threads have 128 each: 8 backward and 4 forward (16-bit types)
+    most = ((8, 3) if wide else (13, 5)) if bwd else ((12, 6) if wide else (16, 12))
     granule = _granule(params)
-    widths = [w for w in range(granule, params.c, granule)] + [params.c]
     best = None
-    for width in widths:
+    for width in [*range(granule, params.c, granule), params.c]:
         lanes = _lane_units(params, width)
-        for threads in (256, 512, 1024):
+        groups = params.n * divup(params.c, width)
+        # lines that two workgroups share cost: 128n 384c 14x14 in slices of 96 channels 10.4 us, of 192 9.5;
+        # 64n 128c 28x28 with a checkpoint in slices of 32 channels 15.6 us, of 64, half as many workgroups, 11.4
+        split_line = 1.0 if width == params.c or width * value % 128 == 0 else 1.25 if width * value > 128 else 2.2
+        for threads in (256, 512, 1024) if groups >= 2 * cus else (512, 256, 1024):
             if threads < lanes:
                 continue
             units = divup(params.pixels, threads // lanes)
-            if units <= (8 if threads < 1024 else most):
-                groups = params.n * divup(params.c, width)
-                key = (groups >= 2 * cus, width if groups >= 2 * cus else -width, -threads)
-                if best is None or key > best[0]:
-                    best = (key, GroupNorm2dConfig(threads, units, width, 0))
-                break
-    if best is not None:
-        return best[1]
-    return GroupNorm2dConfig(512, min(8, most), params.c, 1)
+            if units > most[threads == 1024]:
+                continue
+            cost = divup(groups, cus) * threads * units * split_line
+            if best is None or cost < best[0]:
+                best = (cost, GroupNorm2dConfig(threads, units, width, 0))
+    return best
+
+
+def _best_stretches(params: GroupNorm2dParams, cus: int, bwd: bool) -> GroupNorm2dConfig:
+    """The stretch that leaves the least of the last round of workgroups idle; a workgroup costs what 512 units do
+    besides its own.  (us: forward 16n 24c 144x144 432 workgroups 20.1, 336 23.4; 8n 320c 64x64 232 15.7, 344 18.3.)
+    The forward pass holds its units, the backward pass lets them follow each other."""
+    if bwd:
+        kinds = [(256, u) for u in (16, 12, 8, 4, 2)] + [(512, u) for u in (16, 8, 4, 2)]
+    else:
+        most = 8 if params.dtype == 2 else 12
+        kinds = [(512, u) for u in (8, 6, 12, 4, 2) if u <= most] + [(256, u) for u in (8, 12, 4, 2) if u <= most]
+    best = None
+    for threads, units in kinds:
+        lanes = _lane_units(params, params.c)
+        if threads < lanes:
+            continue
+        grid = params.n * divup(params.pixels, threads // lanes * units)
+        cost = divup(grid, cus) * (threads * units + 512)
+        if best is None or cost < best[0]:
+            best = (cost, GroupNorm2dConfig(threads, units, params.c, 1))
+    return best[1]
+
+
+def _choose(params: GroupNorm2dParams, device_attr, bwd: bool) -> List[GroupNorm2dConfig]:
+    cus = getattr(device_attr, "multiprocessor_count", 256) or 256
+    whole = _best_whole(params, cus, bwd)
+    if whole is not None:
+        size = 2 if params.dtype == 2 else 1
+        total = params.n * params.pixels * params.c / 8 / cus
+        launch, per_unit = _WHOLE[bwd]
+        launches, per_unit_twice = _STRETCHES[bwd]
+        if launch + per_unit * size * whole[0] <= launches + per_unit_twice * size * total:
+            return [whole[1]]
+    return [_best_stretches(params, cus, bwd)]
 
 
 def _get_configs(params: GroupNorm2dParams, device_attr=None) -> List[GroupNorm2dConfig]:
-    cus = getattr(device_attr, "multiprocessor_count", 256) or 256
-    return [_choose(params, cus, 6 if params.dtype == 2 else 12, False)]
+    return _choose(params, device_attr, False)
 
 
 def _get_bwd_configs(params: GroupNorm2dParams, device_attr=None) -> List[GroupNorm2dConfig]:
-    cus = getattr(device_attr, "multiprocessor_count", 256) or 256
-    return [_choose(params, cus, 3 if params.dtype == 2 else 6, True)]
+    return _choose(params, device_attr, True)
 
 
 def _defines(params: GroupNorm2dParams, config: GroupNorm2dConfig):
-    params.validate()
-    assert is_legal(params, config), f"illegal configuration {config} of {params}"
     return {
         "SPIO_GN_C": params.c, "SPIO_GN_GROUPS": params.groups, "SPIO_GN_SLICE": config.slice,
         "SPIO_GN_THREADS": config.threads, "SPIO_GN_UNITS": config.units, "SPIO_GN_SPLIT": config.split,
@@ -155,6 +200,8 @@ def _defines(params: GroupNorm2dParams, config: GroupNorm2dConfig):
 
 def _grid(params: GroupNorm2dParams, config: GroupNorm2dConfig):
     """(workgroups, stretches of an image)"""
+    params.validate()
+    assert is_legal(params, config), f"illegal configuration {config} of {params}"
     stretches = divup(params.pixels, _span(params, config)) if config.split else 1
     grid = params.n * stretches * divup(params.c, config.slice)
     assert (grid + 2 * params.c) * config.threads < 1 << 32, "more workgroups than a launch can have"
