@@ -731,6 +731,70 @@ struct ActivationFunction : torch::autograd::Function<ActivationFunction> {
     }
 };
 
+// ---- convolution with its input kept in 8 bits ----
+
+Kept pack(const Tensor& x) {  // a tensor without gaps, on 16 bytes
+    const auto plan = find_plan(values_key(PACK, x, dtype_number(x), 0, true));
+    Kept kept = empty_kept(x);
+    launch_values(*plan, x.numel(), c10::hip::getCurrentHIPStream(x.get_device()),
+                  {ptr(kept.codes), ptr(kept.exponents), ptr(x), number(x.numel())});
+    return kept;
+}
+void unpack(const Tensor& out, const Tensor& codes, const Tensor& exponents) {
+    const Tensor cc = aligned(codes.contiguous()), ec = exponents.contiguous();
+    const auto plan = find_plan(values_key(UNPACK, out, dtype_number(out), 0, true));
+    launch_values(*plan, out.numel(), c10::hip::getCurrentHIPStream(out.get_device()),
+                  {ptr(out), ptr(cc), ptr(ec), number(out.numel())});
+}
+
+PyObject* g_conv_kept_gradients = nullptr;  // Python: the gradients through the operators
+
+struct ConvKeptFunction : torch::autograd::Function<ConvKeptFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                          const std::optional<Tensor>& bias_arg, const Conv& cv) {
+        const Tensor bias = bias_arg.value_or(Tensor());
+        const auto o = conv_forward(cv, x, w, to_float_1d(bias), /*keep=*/true);
+        const Kept kept = pack(aligned(o.x));
+        ctx->save_for_backward({kept.codes, kept.exponents, w, bias});
+        ctx->saved_data["v"] = std::vector<int64_t>{
+            cv.n, cv.c, cv.h, cv.w, cv.r, cv.s, cv.py, cv.px, cv.bias, static_cast<int64_t>(x.scalar_type()),
+            static_cast<int64_t>(w.scalar_type()),
+            bias.defined() ? static_cast<int64_t>(bias.scalar_type()) : static_cast<int64_t>(at::kFloat)};
+        return o.y.to(x.scalar_type());
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->saved_data["v"].toIntVector();
+        const Conv cv{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8] != 0};
+        auto type = [&](int i) { return static_cast<at::ScalarType>(v[i]); };
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &codes = saved[0], &exponents = saved[1], &w = saved[2], &bias = saved[3], &grad = grads[0];
+        const int64_t n = cv.n * cv.c * cv.h * cv.w;
+        const bool native = !stands_aside(grad) && is_again(codes, grad, {n}, at::kChar) &&
+                            is_again(exponents, grad, {blocks(n)}, at::kByte) &&
+                            is_again(w, grad, {cv.c, 8, cv.r, cv.s}, type(10));
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+                   need_b = cv.bias && ctx->needs_input_grad(2);
+        if (!native) {
+            py::gil_scoped_acquire gil;
+            py::tuple r = py::reinterpret_borrow<py::object>(g_conv_kept_gradients)(
+                grad, codes, exponents, w, bias.defined() ? py::cast(bias) : py::object(py::none()),
+                std::vector<int64_t>{cv.n, cv.c, cv.h, cv.w}, cv.py, cv.px, need_x, need_w, need_b);
+            auto get = [&](int i) { return r[i].is_none() ? Tensor() : r[i].cast<Tensor>().to(type(9 + i)); };
+            return {get(0), get(1), get(2), Tensor()};
+        }
+        RECORD_FUNCTION("spio::conv2d_gw8_backward", tensors({codes, w, bias, grad}));
+        Tensor x;
+        if (need_w) {
+            x = empty_cl({cv.n, cv.c, cv.h, cv.w}, at::kHalf, grad);
+            unpack(x, codes, exponents);
+        }
+        const ConvGrads g = conv_backward(cv, x, to_half_cl(w), grad, need_x, need_w, need_b, type(9), type(10));
+        auto typed = [&](const Tensor& t, int i) { return t.defined() ? t.to(type(i)) : t; };
+        return {typed(g.x, 9), typed(g.w, 10), typed(g.b, 11), Tensor()};
+    }
+};
+
 // ---- Python boundary ------------------------------------------------------------------------
 
 // Arguments of a Python call by position or keyword; false if they do not fit the names.
@@ -771,9 +835,10 @@ PyObject* not_implemented() { Py_RETURN_NOTIMPLEMENTED; }
 // Paddings above this are the Python operator's to refuse: twice one near 2^63 would wrap around to a small image.
 constexpr int64_t MAX_PADDING = 1 << 24;
 
-// conv2d_gw8(inputs, weight, bias=None, stride=1, padding_y=0, padding_x=0, dilation=1, groups=1)
-PyObject* conv2d_gw8(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
-    HANDLE_TH_ERRORS
+// conv2d_gw8(inputs, weight, bias=None, stride=1, padding_y=0, padding_x=0, dilation=1, groups=1), with `Function` for calls
+// whose gradients are recorded
+template <class Function>
+PyObject* convolution(PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames, const char* name) {
     static PyObject* const names[8] = {
         PyUnicode_InternFromString("inputs"),    PyUnicode_InternFromString("weight"),
         PyUnicode_InternFromString("bias"),      PyUnicode_InternFromString("stride"),
@@ -809,17 +874,27 @@ PyObject* conv2d_gw8(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObjec
     {
         py::gil_scoped_release no_gil;
         c10::DeviceGuard device(x.device());
-        RECORD_FUNCTION("spio::conv2d_gw8", tensors({x, w, bias}));
+        RECORD_FUNCTION(name, tensors({x, w, bias}));
         // the casts and copies inside are the operator's own, whatever autocast thinks of them
         c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
         if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(bias))) {
-            y = ConvFunction::apply(x, w, optional(bias), cv);
+            y = Function::apply(x, w, optional(bias), cv);
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
             y = conv_forward(cv, x, w, to_float_1d(bias), /*keep=*/false).y.to(x.scalar_type());
         }
     }
     return THPVariable_Wrap(y);
+}
+PyObject* conv2d_gw8(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    return convolution<ConvFunction>(args, nargs, kwnames, "spio::conv2d_gw8");
+    END_HANDLE_TH_ERRORS
+}
+// The same with its input kept in 8 bits
+PyObject* conv2d_gw8_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    return convolution<ConvKeptFunction>(args, nargs, kwnames, "spio::conv2d_gw8_8bit_forward");
     END_HANDLE_TH_ERRORS
 }
 
@@ -942,11 +1017,7 @@ PyObject* pack_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject
         c10::DeviceGuard device(x.device());
         at::AutoDispatchBelowADInplaceOrView below;
         RECORD_FUNCTION("spio::pack_8bit", tensors({x}));
-        const auto plan = find_plan(values_key(PACK, x, dtype_number(x), 0, true));
-        const Tensor xa = aligned(x);
-        kept = empty_kept(x);
-        launch_values(*plan, x.numel(), c10::hip::getCurrentHIPStream(x.get_device()),
-                      {ptr(kept.codes), ptr(kept.exponents), ptr(xa), number(x.numel())});
+        kept = pack(aligned(x));
     }
     return py::make_tuple(kept.codes, kept.exponents).release().ptr();
     END_HANDLE_TH_ERRORS
@@ -1003,9 +1074,7 @@ PyObject* unpack_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObje
         if (dense_strides) {
             RECORD_FUNCTION("spio::unpack_8bit", tensors({codes, exponents}));
             out = at::detail::empty_strided_cuda(shape, strides, dtype, codes.device());
-            const Tensor cc = aligned(codes.contiguous()), ec = exponents.contiguous();
-            const auto plan = find_plan(values_key(UNPACK, out, dtype_number(out), 0, true));
-            launch_values(*plan, n, c10::hip::getCurrentHIPStream(codes.get_device()), {ptr(out), ptr(cc), ptr(ec), number(n)});
+            unpack(out, codes, exponents);
         }
     }
     if (!dense_strides) return not_implemented();
@@ -1018,6 +1087,8 @@ PyMethodDef g_methods[] = {
      METH_FASTCALL | METH_KEYWORDS, "group_norm_2d on plain GPU tensors, else NotImplemented"},
     {"activation_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(activation_8bit)),
      METH_FASTCALL | METH_KEYWORDS, "activation_8bit on plain GPU tensors, else NotImplemented"},
+    {"conv2d_gw8_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(conv2d_gw8_8bit)),
+     METH_FASTCALL | METH_KEYWORDS, "conv2d_gw8 with its input kept in 8 bits on plain GPU tensors, else NotImplemented"},
     {"pack_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pack_8bit)), METH_FASTCALL | METH_KEYWORDS,
      "codes and exponents of a plain GPU tensor without gaps, else NotImplemented"},
     {"unpack_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(unpack_8bit)), METH_FASTCALL | METH_KEYWORDS,
@@ -1046,9 +1117,10 @@ PYBIND11_MODULE(_native, m) {
         g_backward_op = backward_op.release().ptr();
         g_norm_gradients = norm_gradients.release().ptr();
     });
-    m.def("configure_kept", [](py::object group_norm_gradients, py::object activation_gradient) {
+    m.def("configure_kept", [](py::object group_norm_gradients, py::object activation_gradient, py::object conv_gradients) {
         g_group_norm_gradients = group_norm_gradients.release().ptr();
         g_activation_gradient = activation_gradient.release().ptr();
+        g_conv_kept_gradients = conv_gradients.release().ptr();
     });
     m.def("bypass", [](int64_t change) { g_bypass.fetch_add(change); });
     m.def("forget", [] {

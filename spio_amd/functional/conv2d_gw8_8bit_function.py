@@ -8,6 +8,7 @@ from typing import Optional, Tuple
 
 import torch
 
+from .. import native
 from .activation_8bit_function import pack_8bit_op, unpack_8bit_op
 from .conv2d_gw8_function import conv2d_gw8, conv2d_gw8_backward_op
 from .group_norm_2d_function import refuse_second_derivatives
@@ -47,20 +48,26 @@ def _setup_context(ctx, inputs, output):
     ctx.shape, ctx.dtype = x.shape, x.dtype
 
 
-def _backward(ctx, grad_output, *_unused):
-    if grad_output is None:
-        return (None,) * 5
+def conv2d_gw8_8bit_gradients(grad_output, codes, exponents, weight, bias, shape, padding_y, padding_x, needs_input,
+                              needs_weight, needs_bias):  # fmt: skip
+    """Gradients of conv2d_gw8_8bit in conv2d_gw8's types, None where not needed."""
     refuse_second_derivatives()
-    codes, exponents, weight, bias = ctx.saved_tensors
-    n, c, h, w = ctx.shape
-    needs = ctx.needs_input_grad
-    needs_weight, needs_bias = needs[1], bias is not None and needs[2]
+    n, c, h, w = shape
     if needs_weight:
         x = unpack_8bit_op(codes, exponents, [n, c, h, w], [h * w * c, 1, w * c, c], torch.float16)
     else:  # the operator asks for its sizes only
         x = torch.empty((n, c, h, w), dtype=torch.float16, device=grad_output.device, memory_format=CL)
-    dx, dw, db = conv2d_gw8_backward_op(x, _half(weight), None if bias is None else bias.float(), _half(grad_output),
-                                        *ctx.padding, needs[0], needs_weight, needs_bias)  # fmt: skip
+    return conv2d_gw8_backward_op(x, _half(weight), None if bias is None else bias.float(), _half(grad_output),
+                                  padding_y, padding_x, needs_input, needs_weight, needs_bias)  # fmt: skip
+
+
+def _backward(ctx, grad_output, *_unused):
+    if grad_output is None:
+        return (None,) * 5
+    codes, exponents, weight, bias = ctx.saved_tensors
+    needs = ctx.needs_input_grad
+    dx, dw, db = conv2d_gw8_8bit_gradients(grad_output, codes, exponents, weight, bias, tuple(ctx.shape), *ctx.padding,
+                                           needs[0], needs[1], bias is not None and needs[2])  # fmt: skip
     return (None if dx is None else dx.to(ctx.dtype), None if dw is None else dw.to(weight.dtype),
             None if db is None else db.to(bias.dtype), None, None)  # fmt: skip
 
@@ -76,6 +83,9 @@ def conv2d_gw8_8bit(
     Where no grad_weight is wanted it is conv2d_gw8."""
     if not (torch.is_grad_enabled() and weight.requires_grad):
         return conv2d_gw8(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)
+    y = native.call("conv2d_gw8_8bit", inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)
+    if y is not NotImplemented:
+        return y
     if not torch.is_autocast_enabled("cuda"):
         assert inputs.dtype == torch.float16 and weight.dtype == torch.float16
         assert bias is None or bias.dtype == torch.float32

@@ -178,10 +178,11 @@ def call(name, *args):
     return getattr(_native, name)(*args)
 
 
-def configure_kept(group_norm_gradients, activation_gradient):
-    """What the backward passes of group_norm_2d and activation_8bit hand over to where they stand aside."""
+def configure_kept(group_norm_gradients, activation_gradient, conv_gradients):
+    """What the backward passes of group_norm_2d, activation_8bit and conv2d_gw8_8bit hand over to where they stand
+    aside."""
     if _native is not None:
-        _native.configure_kept(group_norm_gradients, activation_gradient)
+        _native.configure_kept(group_norm_gradients, activation_gradient, conv_gradients)
 
 
 def configure(backward_op, norm_gradients):
