@@ -206,16 +206,26 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
     for (int g = p.tid / LANES; g < GS; g += THREADS / LANES) {
         float n = 0.f, m = 0.f, q = 0.f;
         auto join = [&](float n2, float m2, float q2) {
-            const float total = n + n2, share = total > 0.f ? n2 / total : 0.f, d = m2 - m;
+            const float total = n + n2, share = total > 0.f ? n2 * pw::reciprocal(total) : 0.f, d = m2 - m;
             q += q2 + d * d * n * share;
             m += d * share;
             n = total;
         };
         if (p.slice * GS + g < GROUPS) {
             const float* s = partials + ((long long)p.image * GROUPS + p.slice * GS + g) * stretches * 2;
-            for (unsigned i = part; i < stretches; i += LANES) {
-                const long long left = pixels - (long long)i * SPAN;
-                join((float)(left < SPAN ? left : SPAN) * CG, s[2 * i], s[2 * i + 1]);
+            for (unsigned first = part; first < stretches; first += LANES * 4) {  // four loads under way
+                float m2[4], q2[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned i = first + j * LANES;
+                    m2[j] = i < stretches ? s[2 * i] : 0.f;
+                    q2[j] = i < stretches ? s[2 * i + 1] : 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const long long left = pixels - (long long)(first + j * LANES) * SPAN;
+                    join((float)(left < 0 ? 0 : left < SPAN ? left : SPAN) * CG, m2[j], q2[j]);
+                }
             }
         }
         // (both lanes of a pair come to the same sums but for their order: the lower one's is passed on in the end)

@@ -75,6 +75,9 @@ PW_DEVICE Inputs load_inputs(const Stretch& s, int u) {
 
 // How many of a stretch's units a lane has in registers: all where it works on them twice.
 constexpr int HELD = SPIO_GN_SPLIT ? DEPTH : UN;
+// ... with dz in place of grad_output: that takes more registers, but an activation's derivative takes more
+// instructions than all the rest of the second pass (silu, us: 128n 384c 14x14 16.8 -> 14.7, 64n 128c 28x28 17.3 -> 13.8).
+constexpr bool kHoldsDz = !SPIO_GN_SPLIT && SPIO_ACT;
 
 template <int POLICY>
 PW_DEVICE void load_first(Inputs (&in)[HELD], const Stretch& s) {
@@ -96,7 +99,7 @@ PW_DEVICE void keep_packed(Inputs (&in)[HELD]) {
 #else
         pw::keep_packed(in[u].x);
 #endif
-        pw::keep_packed(in[u].dy);
+        if (!kHoldsDz) pw::keep_packed(in[u].dy);
     }
 }
 
@@ -129,7 +132,7 @@ PW_DEVICE void load_lane(Lane& l, const float* stats, const float* weight, const
 }
 
 // x - mean and dz of a unit (what lies behind the last pixel has dy = 0, and with it dz)
-PW_DEVICE void work(float (&d)[8], float (&dz)[8], const Inputs& in, const Lane& l) {
+PW_DEVICE void centre(float (&d)[8], const Inputs& in, const Lane& l) {
 #if SPIO_GN_KEPT
     const float step = pw::block_step(in.exponent);
 #endif
@@ -140,6 +143,12 @@ PW_DEVICE void work(float (&d)[8], float (&dz)[8], const Inputs& in, const Lane&
 #else
         d[e] = pw::plus(in.x, e, -l.mean[e / KEY_CHANNELS], l.k);
 #endif
+    }
+}
+PW_DEVICE void work(float (&d)[8], float (&dz)[8], const Inputs& in, const Lane& l) {
+    centre(d, in, l);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
         const float z = SPIO_GN_HAS_BIAS ? __builtin_fmaf(d[e], l.scale[e], l.b[e]) : d[e] * l.scale[e];
         dz[e] = pw::activate_grad(in.dy, e, z, l.k);
     }
@@ -152,12 +161,16 @@ constexpr int PARTS = THREADS / COLUMNS > 1 ? THREADS / COLUMNS : 1;  // threads
 constexpr int RED = SUM_ROWS * COLUMNS > PARTS * COLUMNS ? SUM_ROWS * COLUMNS : PARTS * COLUMNS;
 
 template <int POLICY>
-PW_DEVICE void channel_sums(Inputs (&in)[HELD], const Stretch& c, const Place& p, const Lane& l, float* red, float* row) {
+PW_DEVICE void channel_sums(Inputs (&in)[HELD], float (&held)[UN][8], const Stretch& c, const Place& p, const Lane& l,
+                            float* red, float* row) {
     float s1[8] = {}, s2[8] = {};
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
         float d[8], dz[8];
         work(d, dz, in[u % HELD], l);
+        if (kHoldsDz)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) held[u][e] = dz[e];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             s1[e] += dz[e];
@@ -245,7 +258,7 @@ PW_DEVICE void group_pairs(const Place& p, const float* red, float* pairs, const
     sync();
 }
 
-PW_DEVICE void apply(Inputs (&in)[HELD], const Stretch& c, const Place& p, const Lane& l, void* din, const float* pairs, long long pixels) {
+PW_DEVICE void apply(Inputs (&in)[HELD], const float (&held)[UN][8], const Stretch& c, const Place& p, const Lane& l, void* din, const float* pairs, long long pixels) {
     const pw_rsrc rs = pw::buffer(reinterpret_cast<unsigned char*>(din) + c.first * (C * pw::VALUE_BYTES),
                                   (unsigned)c.pixels * (C * pw::VALUE_BYTES));
     const float count = pw::reciprocal((float)pixels * CG);
@@ -260,7 +273,13 @@ PW_DEVICE void apply(Inputs (&in)[HELD], const Stretch& c, const Place& p, const
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
         float d[8], dz[8], dx[8];
-        work(d, dz, in[u % HELD], l);
+        if (kHoldsDz) {
+            centre(d, in[u % HELD], l);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dz[e] = held[u][e];
+        } else {
+            work(d, dz, in[u % HELD], l);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int i = e / KEY_CHANNELS;
@@ -315,13 +334,14 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(float* __restrict__ rows, void* __restrict__ din
     __shared__ float red[RED], pairs[2 * GS];
     const Place p = place(__builtin_amdgcn_workgroup_id_x(), 1);
     const Stretch c = stretch_of(in, exponents, dout, p, pixels);
-    Inputs held[HELD];
-    load_first<pw::STREAM>(held, c);
+    Inputs units[HELD];
+    load_first<pw::STREAM>(units, c);
+    float dz[UN][8];
     Lane l;
     load_lane(l, stats, weight, bias, p);
-    channel_sums<pw::STREAM>(held, c, p, l, red, rows + (long long)p.image * (2 * C));
+    channel_sums<pw::STREAM>(units, dz, c, p, l, red, rows + (long long)p.image * (2 * C));
     group_pairs(p, red, pairs, weight);
-    apply(held, c, p, l, din, pairs, pixels);
+    apply(units, dz, c, p, l, din, pairs, pixels);
 }
 
 #if SPIO_GN_AFFINE
@@ -343,11 +363,12 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(float* __restrict__ rows, void*, const void* __r
     const unsigned stretches = (unsigned)((pixels + SPAN - 1) / SPAN);
     const Place p = place(__builtin_amdgcn_workgroup_id_x(), stretches);
     const Stretch c = stretch_of(in, exponents, dout, p, pixels);
-    Inputs held[HELD];
-    load_first<0>(held, c);
+    Inputs units[HELD];
+    load_first<0>(units, c);
+    float dz[UN][8];
     Lane l;
     load_lane(l, stats, weight, bias, p);
-    channel_sums<0>(held, c, p, l, red, rows + ((long long)p.image * stretches + p.stretch) * (2 * C));
+    channel_sums<0>(units, dz, c, p, l, red, rows + ((long long)p.image * stretches + p.stretch) * (2 * C));
     group_pairs(p, red, pairs, weight);
     float* out = rows + (SPIO_GN_AFFINE ? images * stretches * (2 * C) : 0);
     for (int i = p.tid; i < 2 * GS; i += THREADS) {
@@ -369,8 +390,9 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
     }
     const Place p = place(block - ADDING, stretches);
     const Stretch c = stretch_of(in, exponents, dout, p, pixels);
-    Inputs held[HELD];
-    load_first<pw::STREAM>(held, c);
+    Inputs units[HELD];
+    load_first<pw::STREAM>(units, c);
+    float dz[UN][8];
     Lane l;
     load_lane(l, stats, weight, bias, p);
     const float* parts = rows + (SPIO_GN_AFFINE ? images * stretches * (2 * C) : 0);
@@ -380,9 +402,19 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
         float a = 0.f, b = 0.f;
         if (p.slice * GS + g < GROUPS) {
             const float* s = parts + ((long long)p.image * 2 * GROUPS + p.slice * GS + g) * stretches;
-            for (unsigned i = part; i < stretches; i += LANES) {
-                a += s[i];
-                b += s[(long long)GROUPS * stretches + i];
+            for (unsigned first = part; first < stretches; first += LANES * 4) {  // four loads under way
+                float a4[4], b4[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned i = first + j * LANES;
+                    a4[j] = i < stretches ? s[i] : 0.f;
+                    b4[j] = i < stretches ? s[(long long)GROUPS * stretches + i] : 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a += a4[j];
+                    b += b4[j];
+                }
             }
         }
 #pragma unroll
@@ -396,7 +428,7 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
         }
     }
     sync();
-    apply(held, c, p, l, din, pairs, pixels);
+    apply(units, dz, c, p, l, din, pairs, pixels);
 }
 
 #endif

@@ -130,34 +130,43 @@ PW_DEVICE float sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
 }
 
-// The normal distribution at z: `density` and `cdf`.  The upper tail is density * R(|z|), and R falls smoothly from
-// sqrt(pi/2) like 1/|z|: a polynomial in t = 1 / (1 + p|z|), fitted to its values (scipy's erfcx) at Chebyshev points of t
-// for |z| <= 14 by reweighted least squares, relative error 1.5e-7.  (Two degrees less, 4.6e-6, would do for results in 16
-// bits, but sums of many of them showed it: grad_bias of 16n 24c 144x144 was off by 1.6e-6 of its norm for 4e-7.)
-PW_DEVICE void normal(float z, float& density, float& cdf) {
+// The normal distribution at z: exp(-z^2 / 2) and the upper tail at |z|, which is that times R(|z|); R falls smoothly from
+// a half like 1/|z|: a polynomial in t = 1 / (1 + p|z|), fitted to its values (scipy's erfcx) at Chebyshev points of t for
+// |z| <= 14 by reweighted least squares.  Relative error of the tail 1.5e-7, or 4.6e-6 with two degrees less, which is for
+// single results in 16 bits: sums of many show it (grad_bias of 16n 24c 144x144 was off by 1.6e-6 of its norm for 4e-7).
+template <bool SHORT>
+PW_DEVICE void normal(float z, float& e, float& tail) {
     const float a = __builtin_fabsf(z);
-    const float e = __builtin_amdgcn_exp2f(a * a * -0.721347520f);  // exp(-z^2 / 2)
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3f, 1.f));
-    float r = 0.03567488f;
-    r = __builtin_fmaf(r, t, -0.1572035f);
-    r = __builtin_fmaf(r, t, 0.2063542f);
-    r = __builtin_fmaf(r, t, -0.05368425f);
-    r = __builtin_fmaf(r, t, 0.12856192f);
-    r = __builtin_fmaf(r, t, 0.09991341f);
-    r = __builtin_fmaf(r, t, 0.12075397f);
-    r = __builtin_fmaf(r, t, 0.1196293f);
-    const float tail = e * (r * t);
-    cdf = z < 0.f ? tail : 1.f - tail;
-    density = e * 0.398942280f;
+    e = __builtin_amdgcn_exp2f(a * a * -0.721347520f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, SHORT ? 0.31f : 0.3f, 1.f));
+    float r;
+    if (SHORT) {
+        r = -0.07392936f;
+        r = __builtin_fmaf(r, t, 0.18045098f);
+        r = __builtin_fmaf(r, t, 0.01574401f);
+        r = __builtin_fmaf(r, t, 0.13343013f);
+        r = __builtin_fmaf(r, t, 0.1204412f);
+        r = __builtin_fmaf(r, t, 0.12386071f);
+    } else {
+        r = 0.03567488f;
+        r = __builtin_fmaf(r, t, -0.1572035f);
+        r = __builtin_fmaf(r, t, 0.2063542f);
+        r = __builtin_fmaf(r, t, -0.05368425f);
+        r = __builtin_fmaf(r, t, 0.12856192f);
+        r = __builtin_fmaf(r, t, 0.09991341f);
+        r = __builtin_fmaf(r, t, 0.12075397f);
+        r = __builtin_fmaf(r, t, 0.1196293f);
+    }
+    tail = e * (r * t);
 }
 
 PW_DEVICE float activate(float z) {
     if (SPIO_ACT == 1) return z < 0.f ? 0.f : z;  // (NaN stays)
     if (SPIO_ACT == 2) return z * sigmoid(z);
     if (SPIO_ACT == 3) {
-        float density, cdf;
-        normal(z, density, cdf);
-        return z * cdf;
+        float e, tail;
+        normal<SPIO_DTYPE != 2>(z, e, tail);
+        return z * (z < 0.f ? tail : 1.f - tail);
     }
     return z;
 }
@@ -170,9 +179,9 @@ PW_DEVICE float activate_grad(const Unit& dy, int e, float z, const Constants& k
         return times(dy, e, __builtin_fmaf(s, __builtin_fmaf(-z, s, z), s), k);  // s + s z (1 - s)
     }
     if (SPIO_ACT == 3) {
-        float density, cdf;
-        normal(z, density, cdf);
-        return times(dy, e, __builtin_fmaf(z, density, cdf), k);
+        float density, tail;
+        normal<false>(z, density, tail);
+        return times(dy, e, __builtin_fmaf(z, density * 0.398942280f, z < 0.f ? tail : 1.f - tail), k);
     }
     return value(dy, e);
 }

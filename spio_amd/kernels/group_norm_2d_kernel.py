@@ -115,9 +115,10 @@ def _span(params: GroupNorm2dParams, config: GroupNorm2dConfig) -> int:
 # PER_UNIT * units of the tensor / compute units in stretches, where the input is read twice; both for 16-byte units.
 # Whole images win where there are enough of them, us whole and in stretches: forward 128n 384c 14x14 9.5 and 12, 64n
 # 128c 28x28 9.6 and 11.3, 8n 1280c 8x8 5.6 and 6.9, but 4n 256c 32x32 8.5 and 7.1, 64n 192c 20x20 with one group 9.4 and 8.9;
-# backward 128n 384c 14x14 16.8 and 19.4, 32n 192c 28x28 float32 18.2 and 21.0, but 64n 128c 28x28 17.3 and 15.1.
-_WHOLE = {False: (3.2, 1.1e-3), True: (5.4, 1.8e-3)}  # forward; backward, whose sums over images are a launch
-_STRETCHES = {False: (6.0, 1.8e-3), True: (6.0, 2.75e-3)}
+# backward 128n 384c 14x14 14.7 and 19.4, 32n 192c 28x28 float32 17.9 and 21.2, 64n 128c 28x28 13.8 and 14.7, but 4n 256c
+# 32x32 15 and 7.6.
+_WHOLE = {False: (3.2, 1.1e-3), True: (5.4, 1.3e-3)}  # forward; backward, whose sums over images are a launch
+_STRETCHES = {False: (6.0, 1.8e-3), True: (6.4, 2.75e-3)}
 
 
 def _best_whole(params: GroupNorm2dParams, cus: int, bwd: bool):
@@ -132,8 +133,11 @@ def _best_whole(params: GroupNorm2dParams, cus: int, bwd: bool):
         lanes = _lane_units(params, width)
         groups = params.n * divup(params.c, width)
         # lines that two workgroups share cost: 128n 384c 14x14 in slices of 96 channels 10.4 us, of 192 9.5;
-        # 64n 128c 28x28 with a checkpoint in slices of 32 channels 15.6 us, of 64, half as many workgroups, 11.4
+        # 64n 128c 28x28 with a checkpoint in slices of 32 channels 15.6 us, of 64, half as many workgroups, 11.4.  Not
+        # where the caches hold it all: 10n 112c 10x10 in slices of 32 channels 3.8 us, of 64 5.3.
         split_line = 1.0 if width == params.c or width * value % 128 == 0 else 1.25 if width * value > 128 else 2.2
+        if params.n * params.pixels * params.c * value < 8 << 20:
+            split_line = 1.0
         for threads in (256, 512, 1024) if groups >= 2 * cus else (512, 256, 1024):
             if threads < lanes:
                 continue
