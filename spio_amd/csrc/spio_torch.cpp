@@ -32,6 +32,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <limits>
 #include <memory>
 #include <mutex>
 #include <shared_mutex>
@@ -958,7 +959,7 @@ PyObject* group_norm_2d(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyOb
         if (t.defined() && (!is_plain(t) || t.dim() != 1 || t.size(0) != gn.c || t.device() != x.device() || dtype_number(t) < 0))
             return not_implemented();
     if (gn.n < 1 || gn.h < 1 || gn.w < 1 || gn.c < 8 || gn.c % 8 || gn.c > GROUP_NORM_MAX_CHANNELS || groups < 1 ||
-        gn.c % groups || gn.act < 0 || !(gn.eps > 0))
+        gn.c % groups || gn.act < 0 || !(gn.eps > 0) || gn.eps > std::numeric_limits<double>::max())
         return not_implemented();
     const bool record = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias));
     gn.kept = gn.kept && record;
@@ -1051,9 +1052,8 @@ PyObject* unpack_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObje
         return not_implemented();
     int64_t count = 1;
     for (int64_t size : shape) {
-        if (size > n) return not_implemented();
-        count *= size;  // (no more than n^2 before it is looked at)
-        if (count > n) return not_implemented();
+        if (size < 1 || count > n / size) return not_implemented();
+        count *= size;
     }
     if (count != n) return not_implemented();
     Tensor out;

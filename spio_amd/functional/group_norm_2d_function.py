@@ -51,7 +51,7 @@ def _check(inputs, num_groups, weight, bias, eps, activation):
     c = inputs.shape[1]
     assert num_groups > 0 and c % num_groups == 0, "channels must be a multiple of num_groups"
     assert c > 0 and c % 8 == 0, "channels must be a multiple of 8 (16-byte units)"
-    assert eps > 0, "eps must be positive"
+    assert 0 < eps < float("inf"), "eps must be positive and finite"
     for t in (weight, bias):
         assert t is None or (t.dim() == 1 and t.shape[0] == c and t.is_floating_point()), "weight and bias are [C]"
         assert t is None or t.device == inputs.device, "weight and bias must be on the inputs' device"

@@ -48,7 +48,9 @@ class GroupNorm2dParams:
     kept: bool = False
 
     def encode(self) -> str:
-        """What the compiled code depends on, in characters of an identifier (eps as in LayerNorm2dParams)."""
+        """What the compiled code depends on besides the configuration, in characters of an identifier (eps as in
+        LayerNorm2dParams).  Recorded choices are filed under it, so that one for images of another size may be found:
+        the factories have no other configuration than the chosen one, and such a record is passed over."""
         eps = repr(float(self.eps)).replace(".", "p").replace("-", "m").replace("+", "")
         flags = ("w" if self.has_weight else "nw") + ("b" if self.has_bias else "nb") + ("_8bit" if self.kept else "")
         act = list(ACTIVATIONS)[self.activation]
@@ -58,7 +60,7 @@ class GroupNorm2dParams:
         assert self.n > 0 and self.h > 0 and self.w > 0
         assert self.c % 8 == 0 and 0 < self.c <= MAX_CHANNELS, f"channels must be a multiple of 8 up to {MAX_CHANNELS}"
         assert self.groups > 0 and self.c % self.groups == 0, "channels must be a multiple of the groups"
-        assert 0 <= self.dtype <= 2 and 0 <= self.activation <= 3 and self.eps > 0
+        assert 0 <= self.dtype <= 2 and 0 <= self.activation <= 3 and 0 < self.eps < float("inf")
         assert self.pixels < 1 << 31, "at most 2^31 pixels an image"
 
     @property
@@ -294,7 +296,6 @@ group_norm_2d_kernel_factory = KernelFactory(
     kernel_spec=_get_kernel_spec,
     make_test_args=_make_test_args,
     args_checker=None,
-    is_legal=is_legal,
 )
 
 group_norm_2d_bwd_kernel_factory = KernelFactory(
@@ -306,5 +307,4 @@ group_norm_2d_bwd_kernel_factory = KernelFactory(
     kernel_spec=_get_bwd_kernel_spec,
     make_test_args=_make_bwd_test_args,
     args_checker=None,
-    is_legal=is_legal,
 )

@@ -32,7 +32,7 @@ class GroupNorm2d(nn.GroupNorm):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:  # pylint: disable=arguments-renamed
         if (x.is_cuda and x.dim() == 4 and x.dtype in DTYPES and x.shape[1] == self.num_channels
-                and x.shape[1] % 8 == 0 and x.shape[1] <= MAX_CHANNELS and self.eps > 0):  # fmt: skip
+                and x.shape[1] % 8 == 0 and x.shape[1] <= MAX_CHANNELS and 0 < self.eps < float("inf")):  # fmt: skip
             return group_norm_2d(x, self.num_groups, self.weight, self.bias, self.eps, self.activation,
                                  self.checkpoint_8bit)  # fmt: skip
         y = F.group_norm(x, self.num_groups, self.weight, self.bias, self.eps)

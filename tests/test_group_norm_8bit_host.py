@@ -44,6 +44,8 @@ def test_cpu_tensors_are_refused():
     lambda x: group_norm_2d(x[:, :4], 2),
     lambda x: group_norm_2d(x.double(), 4),
     lambda x: group_norm_2d(x, 4, eps=0.0),
+    lambda x: group_norm_2d(x, 4, eps=float("inf")),
+    lambda x: group_norm_2d(x, 4, eps=float("nan")),
     lambda x: group_norm_2d(x, 4, activation="tanh"),
     lambda x: group_norm_2d(x, 4, torch.ones(15)),
     lambda x: group_norm_2d(x, 4, None, torch.ones(16, 1)),
@@ -168,3 +170,20 @@ def test_the_8_bit_form_is_within_half_a_step():
     step = torch.exp2(exponents.double() - 133).repeat_interleave(32, -1)[:, :77]
     assert ((values(codes, exponents) - x.double()).abs() <= step / 2).all()
     assert exponents.shape == (50, 3) and codes.abs().max() <= 127
+
+
+def test_a_record_for_other_images_is_passed_over(monkeypatch):
+    """The kernels' names leave out the images: a configuration that is recorded under one is used only where it is
+    the chosen one."""
+    from spio_amd.kernels import tuner as tuner_object
+
+    small, large = GroupNorm2dParams(1, 64, 8, 8, 8), GroupNorm2dParams(8, 64, 100, 100, 8)
+    (wrong,), (right,) = (group_norm_2d_kernel_factory.configs(p, ATTR) for p in (large, small))
+    assert wrong != right and is_legal(small, wrong)
+    used = []
+    monkeypatch.setattr("spio_amd.kernels.kernel_cache.compile_and_load_kernel",
+                        lambda factory, params, config, *args, **kwargs: used.append(config))
+    monkeypatch.setattr(tuner_object, "lookup", lambda attr, name: {"config": dataclasses.asdict(wrong)})
+    monkeypatch.setenv("SPIO_TUNE", "1")
+    tuner_object.best_kernel(group_norm_2d_kernel_factory, small, 0, ATTR)
+    assert used == [right]

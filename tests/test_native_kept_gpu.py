@@ -268,6 +268,72 @@ def test_pack_and_unpack():
                     unpack_8bit(bad)
 
 
+def test_vectors_off_16_bytes():
+    """float32 vectors are read where they are: four bytes behind a border too."""
+    leaves, call = _norm()
+    expected = _run(leaves, call)
+    off = [torch.cat([t.detach()[:1], t.detach()])[1:].requires_grad_() for t in leaves[1:]]
+    assert all(t.data_ptr() % 16 == 4 for t in off)
+    _same(_run([leaves[0], *off], call), expected)
+
+
+def test_inference_mode():
+    leaves, call = _norm(kept=True)
+    expected = call(*leaves)
+    with torch.inference_mode():
+        x = leaves[0].detach().clone()
+        assert torch.equal(call(x, *leaves[1:]), call(*leaves))
+        torch.testing.assert_close(call(x, *leaves[1:]), expected, rtol=2e-3, atol=2e-3)
+        y = activation_8bit(x, "silu")
+        assert torch.equal(unpack_8bit(pack_8bit(x)), unpack_8bit(pack_8bit(leaves[0])))
+    torch.testing.assert_close(y, torch.nn.functional.silu(leaves[0]), rtol=2e-3, atol=2e-3)
+
+
+@pytest.mark.parametrize("hw", [(9, 7), (60, 57)])
+def test_the_static_workspace_serves_both_passes(hw):
+    """Launches of the kernels that must not allocate: whole images and stretches."""
+    from spio_amd.kernels import GroupNorm2dParams, group_norm_2d_bwd_kernel_factory, group_norm_2d_kernel_factory
+
+    leaves, call = _norm(c=64, hw=hw)
+    dy = torch.randn(3, 64, *hw, device="cuda").half().contiguous(memory_format=CL)
+    y, dx, dw, db = _run(leaves, call, dy)
+    x, w, b = (t.detach() for t in leaves)
+    params = GroupNorm2dParams(3, 64, *hw, 4, activation=2)
+    out, grad, sums = torch.empty_like(x), torch.empty_like(x), torch.empty(2, 64, device="cuda")
+    stats = torch.empty(3, 4, 2, device="cuda")
+    forward = group_norm_2d_kernel_factory.get_kernel(params, x.device)
+    forward.launch(out, None, None, stats, x, w, b, params.pixels, 3, static_workspace=True)
+    backward = group_norm_2d_bwd_kernel_factory.get_kernel(params, x.device)
+    backward.launch(sums, grad, x, None, dy, stats, w, b, params.pixels, 3, static_workspace=True)
+    _same([out, grad, sums[0], sums[1]], [y, dx, dw, db])
+
+
+def test_replays_of_a_captured_convolution():
+    leaves, call = _conv()
+    dy = torch.randn(3, 24, 9, 7, device="cuda").half().contiguous(memory_format=CL)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _run(leaves, call, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = _run(leaves, call, dy)
+    for seed in range(3):
+        torch.manual_seed(seed)
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(3, 24, 9, 7, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        _same(out, _run(leaves, call, dy), exact=False)
+
+
+def test_a_compiled_convolution():
+    leaves, call = _conv()
+    compiled = torch.compile(lambda x, w, b: conv2d_gw8_8bit(x, w, b, padding_y=1, padding_x=1, groups=3), backend="aot_eager")
+    _same(_run(leaves, compiled), _run(leaves, call), exact=False)
+
+
 def test_arguments_by_name_and_what_the_native_path_leaves_to_python():
     leaves, call = _norm()
     x, w, b = leaves
