@@ -6,11 +6,16 @@
 //   dweight[c] = sum dz * xhat,  dbias[c] = sum dz          float32, over images and pixels
 //
 // The group's sums are those of its channels times their weights, so one pair of sums for each image and channel
-// serves all three gradients.  HBM-bound: where an image's slice of channels fits the registers of one workgroup
-// (SPIO_GN_SPLIT 0) input and gradient are read once, and a second launch adds the images' rows of channel sums.  Otherwise
-// the first launch leaves a row of channel sums for every stretch and the pair of each group; the second one reads
-// input and gradient again, and its first workgroups add the rows meanwhile.  Nothing is atomic: every sum is
-// made in the same order always.
+// serves all three gradients.  Where an image's slice of channels fits the registers of one workgroup (SPIO_GN_SPLIT 0)
+// input and gradient are read once, and a second launch adds the images' rows of channel sums: 128n 768c 7x7 without
+// activation 7.2 us for 30 MB and 2.8, 32n 192c 28x28 float32 with silu 16.2 us for 59 MB and 3.8.
+//
+// Otherwise the first launch leaves a row of channel sums for every stretch and the pair of each group; the second one
+// reads input and gradient again, and its first workgroups add the rows meanwhile (as a launch of its own that takes 3
+// us).  128n 96c 56x56 with silu from 8 bits: 28.6 us for 121 MB and 36.2 us for 202 MB (5.6 TB/s).  Both issue vector
+// instructions for 77 to 88 % of their time: a value costs 17 or 18 of them in either launch, an exp and a rcp among them,
+// which count fourfold.  One launch whose workgroups exchange sums through memory waits more than it saves
+// (32n 48c 224x224 148 to 165 us against 125 to 144).  Nothing is atomic: every sum is made in the same order always.
 #include "spio_group_norm.h"
 
 #ifndef SPIO_GN_AFFINE
@@ -73,7 +78,8 @@ PW_DEVICE Inputs load_inputs(const Stretch& s, int u) {
     return in;
 }
 
-// How many of a stretch's units a lane has in registers: all where it works on them twice.
+// How many of a stretch's units a lane has in registers: all where it works on them twice, else DEPTH, each replaced
+// by the next as soon as it is done with: a lane needs no more registers for a longer stretch.
 constexpr int HELD = SPIO_GN_SPLIT ? DEPTH : UN;
 // ... with dz in place of grad_output: that takes more registers, but an activation's derivative takes more
 // instructions than all the rest of the second pass (silu, us: 128n 384c 14x14 16.8 -> 14.7, 64n 128c 28x28 17.3 -> 13.8).
@@ -258,7 +264,8 @@ PW_DEVICE void group_pairs(const Place& p, const float* red, float* pairs, const
     sync();
 }
 
-PW_DEVICE void apply(Inputs (&in)[HELD], const float (&held)[UN][8], const Stretch& c, const Place& p, const Lane& l, void* din, const float* pairs, long long pixels) {
+PW_DEVICE void apply(Inputs (&in)[HELD], const float (&held)[UN][8], const Stretch& c, const Place& p, const Lane& l,
+                     void* din, const float* pairs, long long pixels) {
     const pw_rsrc rs = pw::buffer(reinterpret_cast<unsigned char*>(din) + c.first * (C * pw::VALUE_BYTES),
                                   (unsigned)c.pixels * (C * pw::VALUE_BYTES));
     const float count = pw::reciprocal((float)pixels * CG);

@@ -55,7 +55,8 @@ constexpr int WAVES = THREADS / 64;
 constexpr int BLOCKS = (C + 31) / 32;           // exponents of a pixel
 static_assert(C % 8 == 0 && C % GROUPS == 0 && SLICE % 8 == 0 && SLICE % CG == 0 && SLICE <= C, "bad geometry");
 static_assert(SLICE == C || SLICE % 32 == 0, "a block lies in one slice");
-// Units that a lane has under way where it does not hold on to them
+// Units that a lane has under way where it does not hold on to them (with 4, 6 or 8 of them 32n 48c 224x224 and 128n 96c
+// 56x56 take as long or longer: what more units hide, fewer waves beside each other lose)
 #ifndef SPIO_GN_DEPTH
 #define SPIO_GN_DEPTH 3
 #endif

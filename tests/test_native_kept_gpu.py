@@ -348,3 +348,39 @@ def test_arguments_by_name_and_what_the_native_path_leaves_to_python():
         activation_8bit(x, "none")
     one = group_norm_2d(x, 4, w, b, 1)  # eps as an integer
     assert torch.equal(one, group_norm_2d(x, 4, w, b, 1.0))
+
+
+def test_a_block_of_all_of_them_and_its_tuning(monkeypatch, tmp_path):
+    """A convolution, a norm and an activation that keep their inputs in 8 bits, one behind the other: gradients within
+    what the checkpoints' half steps change, and the same results after the model's kernels were timed and recorded."""
+    from spio_amd.layers import Activation8bit, Conv2dGw8, GroupNorm2d
+    from spio_amd.tune import tune_model
+
+    monkeypatch.setenv("SPIO_TUNE_DB", str(tmp_path / "tuned.json"))
+    torch.manual_seed(8)
+    conv = Conv2dGw8(96, 96, 3, padding=1, groups=12, bias=False)
+    norm = GroupNorm2d(12, 96, activation="silu")
+    block = torch.nn.Sequential(conv, norm, torch.nn.Conv2d(96, 192, 1), Activation8bit("gelu"))
+    block = block.cuda().half().to(memory_format=CL)
+    x = torch.randn(4, 96, 20, 18, device="cuda").half().contiguous(memory_format=CL)
+
+    def gradients(kept):
+        conv.checkpoint_8bit = norm.checkpoint_8bit = kept
+        block.zero_grad()
+        y = block(x)
+        y.float().square().mean().backward()
+        return [y.detach().clone(), *(p.grad.clone() for p in block.parameters())]
+
+    plain, kept = gradients(False), gradients(True)
+    assert torch.equal(plain[0], kept[0])
+    for a, b in zip(plain[1:], kept[1:]):
+        # a checkpoint is off by 1/255 of a block's largest value (five deviations, say) at most, and an input by
+        # 1/50 of its deviation so; as a vector a gradient is off by no more than these add up to in the two kept inputs
+        assert (a - b).float().norm() <= 0.04 * a.float().norm()
+    results = tune_model(block, [x], iters=1, warmup=1)
+    names = {r["kernel"].split("__")[0] for r in results}
+    assert {"spio_group_norm_2d", "spio_group_norm_2d_bwd", "spio_activation_8bit", "spio_activation_8bit_bwd", "spio_pack_8bit",
+            "spio_unpack_8bit", "spio_conv2d_gw8_fprop"} <= names  # fmt: skip
+    assert all(r["config"] is not None for r in results)
+    for a, b in zip(kept, gradients(True)):
+        torch.testing.assert_close(a, b, rtol=2e-2, atol=2e-2 * float(a.abs().max()))
