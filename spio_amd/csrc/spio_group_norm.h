@@ -4,6 +4,7 @@
 //   SPIO_GN_SLICE               channels that a workgroup works on: whole groups and whole blocks of 32 channels,
 //                               or all of them; the last slice may have fewer
 //   SPIO_GN_THREADS, SPIO_GN_UNITS   threads of a workgroup; units of eight channels that a lane holds
+//   SPIO_GN_ROWS                pixels whose units the threads have at a time
 //   SPIO_GN_EPS, SPIO_GN_HAS_WEIGHT, SPIO_GN_HAS_BIAS
 //   SPIO_GN_KEPT                the input in the 8-bit form is written (forward) or read (backward)
 //   SPIO_GN_SPLIT               images are cut into stretches of pixels, one workgroup each
@@ -49,7 +50,7 @@ constexpr int GS = SLICE / CG;                  // groups of a slice
 constexpr int SU = SLICE / 8;                   // units of a pixel's slice
 // a block of the 8-bit form is four neighbouring lanes of one wave
 constexpr int SUP = SPIO_GN_KEPT ? (SU + 3) / 4 * 4 : SU;
-constexpr int ROWS = THREADS / SUP;
+constexpr int ROWS = SPIO_GN_ROWS;
 constexpr int SPAN = ROWS * UN;                 // pixels that a workgroup holds
 constexpr int WAVES = THREADS / 64;
 constexpr int BLOCKS = (C + 31) / 32;           // exponents of a pixel
@@ -61,7 +62,7 @@ static_assert(SLICE == C || SLICE % 32 == 0, "a block lies in one slice");
 #define SPIO_GN_DEPTH 3
 #endif
 constexpr int DEPTH = SPIO_GN_DEPTH < UN ? SPIO_GN_DEPTH : UN;
-static_assert(THREADS % 64 == 0 && ROWS >= 1, "bad geometry");
+static_assert(THREADS % 64 == 0 && ROWS >= 1 && ROWS <= THREADS / SUP, "bad geometry");
 
 // A lane's eight channels as the groups divide them: KEYS values for it, KEY_CHANNELS channels each, all of one group.
 constexpr int KEYS = CG % 8 == 0 ? 1 : 8 % CG == 0 ? 8 / CG : 8;
@@ -70,6 +71,7 @@ constexpr int GROUP_KEYS = CG / KEY_CHANNELS;   // of a group
 
 // Lanes of a wave that have the same channels add up by an exchange if their number is a power of two.
 constexpr bool kFold = SUP <= 64 && (SUP & (SUP - 1)) == 0;
+static_assert(!kFold || ROWS == THREADS / SUP, "lanes without a pixel are not folded in");
 constexpr int SUM_ROWS = kFold ? WAVES : ROWS;  // what then is left to add
 
 struct Place {

@@ -95,6 +95,15 @@ def _lane_units(params: GroupNorm2dParams, width: int) -> int:
     return divup(width // 8, 4) * 4 if params.kept else width // 8
 
 
+def _rows(params: GroupNorm2dParams, threads: int, width: int) -> int:
+    """Pixels that a workgroup's threads have one unit each of: all that there are lanes for, or, where that idles no
+    more than a sixteenth of them, as many as make whole lines."""
+    rows = threads // _lane_units(params, width)
+    pixel = params.c * (4 if params.dtype == 2 else 2)
+    lines = rows - rows % (128 // gcd(128, pixel))
+    return lines if width == params.c and 16 * (rows - lines) <= rows else rows
+
+
 def is_legal(params: GroupNorm2dParams, config: GroupNorm2dConfig) -> bool:
     return (
         config.threads in (256, 512, 1024)
@@ -108,48 +117,74 @@ def is_legal(params: GroupNorm2dParams, config: GroupNorm2dConfig) -> bool:
 
 def _span(params: GroupNorm2dParams, config: GroupNorm2dConfig) -> int:
     """Pixels that a workgroup holds."""
-    return config.threads // _lane_units(params, config.slice) * config.units
+    return _rows(params, config.threads, config.slice) * config.units
 
 
-# How a configuration is chosen.  The times of its two kinds were fitted to sweeps of 20 shapes in both directions (1 to
-# 256 images, 64 to 1280 channels, 7x7 to 224x224): a launch, and for every round of workgroups over the device what the
+# How a configuration is chosen.  The times of its two kinds were fitted to sweeps of 200 shapes in both directions (1 to
+# 256 images, 48 to 1280 channels, 5x5 to 224x224): a launch, and for every round of workgroups over the device what the
 # units of a workgroup take.  us = LAUNCH + PER_UNIT * rounds * threads * units for whole images, us = LAUNCH +
-# PER_UNIT * units of the tensor / compute units in stretches, where the input is read twice; both for 16-byte units.
+# PER_UNIT * units of the tensor / compute units + PER_JOIN * (joins - 1) in stretches, where the input is read twice; both for
+# 16-byte units.  Over 120 more random shapes the choice takes 1.02 times the best of ten others on average, at most 1.39.
 # Whole images win where there are enough of them, us whole and in stretches: forward 128n 384c 14x14 9.5 and 12, 64n
 # 128c 28x28 9.6 and 11.3, 8n 1280c 8x8 5.6 and 6.9, but 4n 256c 32x32 8.5 and 7.1, 64n 192c 20x20 with one group 9.4 and 8.9;
 # backward 128n 384c 14x14 14.7 and 19.4, 32n 192c 28x28 float32 17.9 and 21.2, 64n 128c 28x28 13.8 and 14.7, but 4n 256c
 # 32x32 15 and 7.6.
-_WHOLE = {False: (3.2, 1.1e-3), True: (5.4, 1.3e-3)}  # forward; backward, whose sums over images are a launch
-_STRETCHES = {False: (6.0, 1.8e-3), True: (6.4, 2.75e-3)}
+_WHOLE = {False: (3.3, 1.1e-3), True: (6.0, 1.65e-3)}  # forward; backward, whose sums over images are a launch
+_STRETCHES = {False: (6.2, 1.75e-3, 0.67), True: (6.6, 3.0e-3, 0.39)}
+
+
+def _shared_lines(params: GroupNorm2dParams, width: int, bwd: bool) -> float:
+    """How much longer a pass takes where slices of `width` channels share lines of 128 bytes, which every one of them
+    touches, or sectors of 32, which none can write whole.  Fitted to 450 measurements (45 shapes).  us: 128n 384c 14x14 in
+    slices of 96 channels 10.4, of 192 9.5; with a checkpoint 64n 128c 28x28 in slices of 32 channels 15.6, of 64, half as many
+    workgroups, 11.4; 103n 328c 27x27 in slices of 64 75, in stretches 32.  Less where the caches hold it all: 10n 112c 10x10
+    in slices of 32 channels 3.8, of 64 5.3."""
+    if width == params.c:
+        return 1.0
+    value = 4 if params.dtype == 2 else 2
+    pixel = params.c * value
+    lines = 0 if width * value % 128 == 0 and pixel % 128 == 0 else 112 / (width * value)  # more than its own, of each
+    code_lines = 0 if not params.kept or (width % 128 == 0 and params.c % 128 == 0) else 120 / width
+    sectors, code_sectors = pixel % 32 != 0, params.kept and params.c % 32 != 0
+    if bwd:
+        more = 0.5 * lines + 0.1 * code_lines + 0.3 * code_sectors
+    else:
+        more = 0.42 * lines + 0.34 * code_lines + 0.36 * sectors + 0.24 * code_sectors
+    return 1.0 + more * (0.3 if params.n * params.pixels * pixel < 8 << 20 else 1.0)
 
 
 def _best_whole(params: GroupNorm2dParams, cus: int, bwd: bool):
     """(cost, configuration) that holds whole images, or None; the cost is rounds * threads * units."""
     wide = params.dtype == 2
-    value = 4 if wide else 2
     # units in a lane's registers, of which 1024 threads have 128 each: 8 backward and 4 forward (16-bit types)
     most = ((8, 3) if wide else (13, 5)) if bwd else ((12, 6) if wide else (16, 12))
     granule = _granule(params)
+    gelu = 1.25 if params.activation == 3 and not bwd else 1.0
     best = None
     for width in [*range(granule, params.c, granule), params.c]:
         lanes = _lane_units(params, width)
         groups = params.n * divup(params.c, width)
-        # lines that two workgroups share cost: 128n 384c 14x14 in slices of 96 channels 10.4 us, of 192 9.5;
-        # 64n 128c 28x28 with a checkpoint in slices of 32 channels 15.6 us, of 64, half as many workgroups, 11.4.  Not
-        # where the caches hold it all: 10n 112c 10x10 in slices of 32 channels 3.8 us, of 64 5.3.
-        split_line = 1.0 if width == params.c or width * value % 128 == 0 else 1.25 if width * value > 128 else 2.2
-        if params.n * params.pixels * params.c * value < 8 << 20:
-            split_line = 1.0
+        shared = _shared_lines(params, width, bwd)
         for threads in (256, 512, 1024) if groups >= 2 * cus else (512, 256, 1024):
             if threads < lanes:
                 continue
-            units = divup(params.pixels, threads // lanes)
+            units = divup(params.pixels, _rows(params, threads, width))
             if units > most[threads == 1024]:
                 continue
-            cost = divup(groups, cus) * threads * units * split_line
+            # a workgroup is faster where others leave it more of the memory's rate, and slower by gelu's instructions
+            cost = divup(groups, cus) * threads * units * shared * (0.7 + 0.3 * min(1.0, groups / cus)) * gelu
             if best is None or cost < best[0]:
                 best = (cost, GroupNorm2dConfig(threads, units, width, 0))
     return best
+
+
+def _joins(params: GroupNorm2dParams, config: GroupNorm2dConfig) -> int:
+    """Times that a lane of the second launch waits for partial results: the lanes of a group load those of four
+    stretches each at once."""
+    lanes = 64
+    while lanes > 1 and lanes * params.groups > config.threads:
+        lanes //= 2
+    return divup(params.groups, config.threads // lanes) * divup(params.pixels, _span(params, config) * 4 * lanes)
 
 
 def _best_stretches(params: GroupNorm2dParams, cus: int, bwd: bool) -> GroupNorm2dConfig:
@@ -166,24 +201,27 @@ def _best_stretches(params: GroupNorm2dParams, cus: int, bwd: bool) -> GroupNorm
         lanes = _lane_units(params, params.c)
         if threads < lanes:
             continue
-        grid = params.n * divup(params.pixels, threads // lanes * units)
-        cost = divup(grid, cus) * (threads * units + 512)
+        grid = params.n * divup(params.pixels, _rows(params, threads, params.c) * units)
+        config = GroupNorm2dConfig(threads, units, params.c, 1)
+        cost = divup(grid, cus) * (threads * units + 512) + (125 if bwd else 400) * (_joins(params, config) - 1)
         if best is None or cost < best[0]:
-            best = (cost, GroupNorm2dConfig(threads, units, params.c, 1))
+            best = (cost, config)
     return best[1]
 
 
 def _choose(params: GroupNorm2dParams, device_attr, bwd: bool) -> List[GroupNorm2dConfig]:
+    params.validate()
     cus = getattr(device_attr, "multiprocessor_count", 256) or 256
-    whole = _best_whole(params, cus, bwd)
+    whole, split = _best_whole(params, cus, bwd), _best_stretches(params, cus, bwd)
     if whole is not None:
         size = 2 if params.dtype == 2 else 1
         total = params.n * params.pixels * params.c / 8 / cus
         launch, per_unit = _WHOLE[bwd]
-        launches, per_unit_twice = _STRETCHES[bwd]
-        if launch + per_unit * size * whole[0] <= launches + per_unit_twice * size * total:
+        launches, per_unit_twice, per_join = _STRETCHES[bwd]
+        stretches = launches + per_unit_twice * size * total + per_join * (_joins(params, split) - 1)
+        if launch + per_unit * size * whole[0] <= stretches:
             return [whole[1]]
-    return [_best_stretches(params, cus, bwd)]
+    return [split]
 
 
 def _get_configs(params: GroupNorm2dParams, device_attr=None) -> List[GroupNorm2dConfig]:
@@ -198,9 +236,9 @@ def _defines(params: GroupNorm2dParams, config: GroupNorm2dConfig):
     return {
         "SPIO_GN_C": params.c, "SPIO_GN_GROUPS": params.groups, "SPIO_GN_SLICE": config.slice,
         "SPIO_GN_THREADS": config.threads, "SPIO_GN_UNITS": config.units, "SPIO_GN_SPLIT": config.split,
-        "SPIO_GN_EPS": f"{float(params.eps)!r}f", "SPIO_GN_HAS_WEIGHT": int(params.has_weight),
-        "SPIO_GN_HAS_BIAS": int(params.has_bias), "SPIO_GN_KEPT": int(params.kept),
-        "SPIO_DTYPE": params.dtype, "SPIO_ACT": params.activation,
+        "SPIO_GN_ROWS": _rows(params, config.threads, config.slice), "SPIO_GN_EPS": f"{float(params.eps)!r}f",
+        "SPIO_GN_HAS_WEIGHT": int(params.has_weight), "SPIO_GN_HAS_BIAS": int(params.has_bias),
+        "SPIO_GN_KEPT": int(params.kept), "SPIO_DTYPE": params.dtype, "SPIO_ACT": params.activation,
     }  # fmt: skip
 
 
