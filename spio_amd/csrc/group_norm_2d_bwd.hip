@@ -268,7 +268,7 @@ PW_DEVICE void apply(Inputs (&in)[HELD], const float (&held)[UN][8], const Stret
                      void* din, const float* pairs, long long pixels) {
     const pw_rsrc rs = pw::buffer(reinterpret_cast<unsigned char*>(din) + c.first * (C * pw::VALUE_BYTES),
                                   (unsigned)c.pixels * (C * pw::VALUE_BYTES));
-    const float count = pw::reciprocal((float)pixels * CG);
+    const float count = pw::reciprocal((float)(unsigned)pixels * CG);
     // rstd * (dz * w - m1 - xhat * m2) = dz * scale + c1 + (x - mean) * c2
     float c1[KEYS], c2[KEYS];
 #pragma unroll

@@ -12,12 +12,14 @@ import torch
 
 from spio_amd.functional import group_norm_2d
 from spio_amd.functional.group_norm_2d_function import group_norm_2d_backward, group_norm_2d_forward
+from spio_amd.hip import get_device_attributes
 from spio_amd.kernels.group_norm_2d_kernel import (
     GroupNorm2dConfig,
     GroupNorm2dParams,
     group_norm_2d_bwd_kernel_factory,
     group_norm_2d_kernel_factory,
     is_legal,
+    kept_shapes,
 )
 from spio_amd.layers import GroupNorm2d
 from tests.pointwise_reference import CL, assert_within, group_norm, rounding, pack_rows
@@ -96,6 +98,30 @@ def test_forward_and_gradients(shape, groups, dtype, act, kept, affine):
     y2 = group_norm_2d(leaves[0], groups, leaves[1], leaves[2], 1e-5, act, kept)
     again = [y2.detach(), *torch.autograd.grad(y2, [t for t in leaves if t is not None], _on_gpu(dy, False))]
     assert all(torch.equal(a, b) for a, b in zip(got, again))  # sums in the same order always
+
+
+@pytest.mark.parametrize("units,kept", [(1, True), (2, True), (2, False), (3, True), (4, True)])
+def test_more_stretches_than_lanes_of_a_group(units, kept):
+    """Each lane joins several stretches' statistics, the last of which there are not everywhere."""
+    x, dy, weight, bias = _tensors(5, 768, 14, 20, FLOAT, "w")
+    params = GroupNorm2dParams(5, 768, 14, 20, 32, 2, 2, has_bias=False, kept=kept)
+    xg, wg, dyg = _on_gpu(x, False), _on_gpu(weight, False), _on_gpu(dy, False)
+    y, dx, stats, sums = torch.empty_like(xg), torch.empty_like(xg), torch.empty(5, 32, 2).cuda(), torch.empty(2, 768).cuda()
+    codes, exponents = (torch.empty(s, dtype=torch.uint8, device="cuda") if kept else None for s in kept_shapes(5, 768, 14, 20))
+    attr = get_device_attributes(0)
+    for threads in (256, 512):
+        kernels = [f.make_kernel(params, GroupNorm2dConfig(threads, units, 768, 1), attr)
+                   for f in (group_norm_2d_kernel_factory, group_norm_2d_bwd_kernel_factory)]  # fmt: skip
+        for kernel in kernels:
+            kernel.compile()
+            kernel.load(0)
+        for _ in range(3):
+            y.fill_(-42)
+            kernels[0](y, codes, exponents, stats, xg, wg, None, params.pixels, 5)
+            kernels[1](sums, dx, codes if kept else xg, exponents, dyg, stats, wg, None, params.pixels, 5)
+            _check([y, dx, sums[0]], x, dy, 32, weight, None, "silu", kept, FLOAT, f"{threads} {units}")
+        for kernel in kernels:
+            kernel.unload()
 
 
 @pytest.mark.parametrize("kept", [False, True])

@@ -1,10 +1,14 @@
 """Host side of group_norm_2d and the 8-bit operators: refusals, configurations, geometry.  CPU only."""
 
 import dataclasses
+import os
+import re
+import subprocess
 
 import pytest
 import torch
 
+from spio_amd.build import CSRC_DIR, HIPCC_DEVICE_FLAGS, ROCM_HOME
 from spio_amd.functional import activation_8bit, conv2d_gw8_8bit, group_norm_2d, pack_8bit, unpack_8bit
 from spio_amd.functional.activation_8bit_function import Packed8bit, _is_dense
 from spio_amd.functional.group_norm_2d_function import group_norm_2d_backward
@@ -187,3 +191,24 @@ def test_a_record_for_other_images_is_passed_over(monkeypatch):
     monkeypatch.setenv("SPIO_TUNE", "1")
     tuner_object.best_kernel(group_norm_2d_kernel_factory, small, 0, ATTR)
     assert used == [right]
+
+
+@pytest.mark.parametrize("factory", [group_norm_2d_kernel_factory, group_norm_2d_bwd_kernel_factory])
+@pytest.mark.parametrize("params", [
+    GroupNorm2dParams(5, 768, 14, 20, 32, 2, 2, has_bias=False, kept=True),
+    GroupNorm2dParams(32, 48, 224, 224, 8, 0, 2),
+    GroupNorm2dParams(1, 384, 50, 50, 3, 1, 3, kept=True),
+])  # fmt: skip
+def test_no_shift_of_64_bits_by_a_vector_register(factory, params, tmp_path):
+    """The hardware takes a wrong number of places where that register is the last that a wave has: a conversion
+    of a 64-bit integer, which has such a shift in it, made one of 240 values for some waves."""
+    (config,) = factory.configs(params, ATTR)
+    kernel = factory.make_kernel(params, config, ATTR)
+    assert config.split
+    out = str(tmp_path / "kernel.s")
+    subprocess.run([os.path.join(ROCM_HOME, "bin", "hipcc"), "-S", "--cuda-device-only", *HIPCC_DEVICE_FLAGS, f"-I{CSRC_DIR}",
+                    *[f"-D{k}={v}" for k, v in kernel.defines.items()], "-o", out,
+                    os.path.join(CSRC_DIR, kernel.kernel_source_file)], check=True, capture_output=True)  # fmt: skip
+    code = open(out).read()
+    assert "buffer_load_dwordx" in code
+    assert not re.findall(r"v_(?:lshl|lshr|ashr)rev_[bi]64\S* v\[\d+:\d+\], v\d+", code)
