@@ -136,7 +136,7 @@ SPIO_KERNEL_NAME(
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (SPIO_MODE == 1)
-                    y[e] = pw::activate_grad(v[u], e, pw::code(c[u], e) * step, constants);
+                    y[e] = pw::activate_grad<SPIO_DTYPE != 2>(v[u], e, pw::code(c[u], e) * step, constants);
                 else if (SPIO_MODE == 3)
                     y[e] = finite(pw::code(c[u], e) * step);
                 else

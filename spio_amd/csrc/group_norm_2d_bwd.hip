@@ -156,7 +156,7 @@ PW_DEVICE void work(float (&d)[8], float (&dz)[8], const Inputs& in, const Lane&
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float z = SPIO_GN_HAS_BIAS ? __builtin_fmaf(d[e], l.scale[e], l.b[e]) : d[e] * l.scale[e];
-        dz[e] = pw::activate_grad(in.dy, e, z, l.k);
+        dz[e] = pw::activate_grad<false>(in.dy, e, z, l.k);
     }
 }
 

@@ -171,7 +171,8 @@ PW_DEVICE float activate(float z) {
     return z;
 }
 
-// value e of dy times the activation's derivative at z
+// value e of dy times the activation's derivative at z (SHORT as in normal)
+template <bool SHORT>
 PW_DEVICE float activate_grad(const Unit& dy, int e, float z, const Constants& k) {
     if (SPIO_ACT == 1) return z > 0.f ? value(dy, e) : 0.f;
     if (SPIO_ACT == 2) {
@@ -180,7 +181,7 @@ PW_DEVICE float activate_grad(const Unit& dy, int e, float z, const Constants& k
     }
     if (SPIO_ACT == 3) {
         float density, tail;
-        normal<false>(z, density, tail);
+        normal<SHORT>(z, density, tail);
         return times(dy, e, __builtin_fmaf(z, density * 0.398942280f, z < 0.f ? tail : 1.f - tail), k);
     }
     return value(dy, e);

@@ -656,8 +656,12 @@ struct GroupNormFunction : torch::autograd::Function<GroupNormFunction> {
                                           ptr(bf), px, images});
         else if (plan->second.function)
             launch(plan->second, stream, {ptr(sums), ptr(workspace), images});
-        return {need_x ? dx : Tensor(), need_w ? sums.select(0, 0).to(weight.scalar_type()) : Tensor(),
-                need_b ? sums.select(0, 1).to(bias.scalar_type()) : Tensor(), Tensor()};
+        at::AutoDispatchBelowADInplaceOrView below;  // (nobody looks for a history or a base of these)
+        auto row = [&](int i, at::ScalarType dtype) {
+            const Tensor t = sums.select(0, i);
+            return t.scalar_type() == dtype ? t : t.to(dtype);
+        };
+        return {need_x ? dx : Tensor(), need_w ? row(0, type(9)) : Tensor(), need_b ? row(1, type(10)) : Tensor(), Tensor()};
     }
 };
 
