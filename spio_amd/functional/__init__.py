@@ -1,4 +1,4 @@
-"""Functional interface: the `spio::conv2d_gw8` custom operators."""
+"""Functional interface: the `spio::conv2d_gw8` custom operators, norms over channels_last tensors and the 8-bit form."""
 
 from .conv2d_gw8_function import (
     conv2d_gw8,
