@@ -2,7 +2,7 @@
 
 The kernels (csrc/group_norm_2d.hip, csrc/group_norm_2d_bwd.hip) are specialised by channels, groups, types and
 activation, not by the number and size of the images, which are arguments: the names of the kernels leave those out, so
-that the compiled code is one file for all of them.
+that the compiled code is one file for all that get the same configuration.
 
 Arguments, forward:  (output, codes, exponents, stats, input, weight, bias, pixels, images)
           backward:  (sums, grad_input, input or codes, exponents, grad_output, stats, weight, bias, pixels, images)
