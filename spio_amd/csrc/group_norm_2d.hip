@@ -212,15 +212,18 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
     if (SPIO_GN_HAS_BIAS) load_vector(b, bias, p);
 
     // The lanes of a wave share a group's stretches; sets of n values with means m and squares q join as
-    // n = n1 + n2, m = m1 + (m2 - m1) n2/n, q = q1 + q2 + (m2 - m1)^2 n1 n2/n.
+    // n = n1 + n2, m = m1 + (m2 - m1) n2/n, q = q1 + q2 + (m2 - m1)^2 n1 n2/n.  Where one is empty there is no difference:
+    // that to its mean of zero would be the other's mean, whose square may overflow.
     constexpr int LANES = group_lanes();
     const int part = p.tid % LANES;
     for (int g = p.tid / LANES; g < GS; g += THREADS / LANES) {
         float n = 0.f, m = 0.f, q = 0.f;
         auto join = [&](float n2, float m2, float q2) {
-            const float total = n + n2, share = total > 0.f ? n2 * pw::reciprocal(total) : 0.f, d = m2 - m;
+            const bool empty = n == 0.f;
+            const float total = n + n2, share = total > 0.f ? n2 * pw::reciprocal(total) : 0.f;
+            const float d = empty || n2 == 0.f ? 0.f : m2 - m;
             q += q2 + d * d * n * share;
-            m += d * share;
+            m = empty ? m2 : __builtin_fmaf(d, share, m);
             n = total;
         };
         if (p.slice * GS + g < GROUPS) {

@@ -1,0 +1,33 @@
+"""group_norm_2d where float32 arithmetic comes to its ends: constant groups, means far above the deviation, rows of
+sums of very many images, the smallest eps."""
+
+import pytest
+import torch
+
+from spio_amd import native
+from spio_amd.functional import group_norm_2d
+from spio_amd.hip import get_device_attributes
+from spio_amd.kernels.group_norm_2d_kernel import GroupNorm2dParams, _get_bwd_configs, _get_configs, DTYPES
+from tests.pointwise_reference import CL, assert_within, group_norm, rounding
+
+pytestmark = pytest.mark.gpu
+HALF, BF16, FLOAT = torch.float16, torch.bfloat16, torch.float32
+# (shape, groups, whether the image is cut into stretches); no group has a power of two of values
+SHAPES = [((2, 16, 7, 7), 2, 0), ((1, 72, 9, 5), 8, 0), ((1, 64, 57, 55), 32, 1), ((2, 48, 75, 61), 8, 1)]
+
+
+def _is_split(shape, groups, dtype, configs=_get_configs, **more):
+    (config,) = configs(GroupNorm2dParams(*shape, groups, DTYPES[dtype], **more), get_device_attributes(0))
+    return config.split
+
+
+@pytest.mark.parametrize("shape,groups,split", SHAPES)
+def test_a_mean_whose_square_overflows(shape, groups, split):
+    """Values around 1.2 * 2^64, 2^-9 of that apart: the squares of the differences stay finite, that of the mean does not.
+    A mean is off by 2^-19 of itself at most (chains of 128 values, then trees), which is 2^-10 of a deviation."""
+    assert _is_split(shape, groups, FLOAT, has_weight=False, has_bias=False) == split
+    g = torch.Generator().manual_seed(0)
+    x = (1.2 * 2.0**64 * (1 + 2.0**-9 * torch.randn(shape, generator=g, dtype=torch.float64))).float()
+    (exact,) = group_norm(x, groups, None, None, 1e-5, "none")
+    y = group_norm_2d(x.cuda().contiguous(memory_format=CL), groups)
+    assert_within(y, exact, 2.0**-10 + 2.0**-16 * exact.abs().max() + rounding(exact, FLOAT))
