@@ -62,7 +62,13 @@ PW_DEVICE void keep_packed(pw::Unit (&v)[UN]) {
     for (int u = 0; u < UN; ++u) pw::keep_packed(v[u]);
 }
 
-// mean[] and squares[] (sum of squared differences to it) of the groups of a chunk.
+// The mean of a group from its sum over that many pixels
+PW_DEVICE float mean_of(float sum, int pixels) {
+    const float count = (float)pixels * CG;
+    return pw::quotient(sum, count, pw::reciprocal(count));
+}
+
+// mean[] = sums and squares[] = sums of squared differences to the means of the groups of a stretch.
 PW_DEVICE void moments(pw::Unit (&v)[UN], const Stretch& c, const Place& p, const pw::Constants& k, float* red,
                        float* mean, float* squares) {
     float s[KEYS] = {};
@@ -75,11 +81,10 @@ PW_DEVICE void moments(pw::Unit (&v)[UN], const Stretch& c, const Place& p, cons
     }
     group_sums(s, p, red, mean);
     keep_packed(v);
-    const float count = pw::reciprocal((float)c.pixels * CG);
     float m[KEYS];
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
-        m[i] = mean[group_of(p, i) < GS ? group_of(p, i) : 0] * count;
+        m[i] = mean_of(mean[group_of(p, i) < GS ? group_of(p, i) : 0], c.pixels);
         s[i] = 0.f;
     }
 #pragma unroll
@@ -158,18 +163,17 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(void* __restrict__ out, unsigned char* __restric
     if (SPIO_GN_HAS_WEIGHT) load_vector(w, weight, p);
     if (SPIO_GN_HAS_BIAS) load_vector(b, bias, p);
     moments(v, c, p, k, red, sum, squares);
-    const float count = pw::reciprocal((float)(unsigned)pixels * CG);
     float mean[KEYS], rstd[KEYS];
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
         const int g = group_of(p, i) < GS ? group_of(p, i) : 0;
-        mean[i] = sum[g] * count;
+        mean[i] = mean_of(sum[g], c.pixels);
         rstd[i] = inverse_deviation(squares[g], pixels);
     }
     if (stats)
         for (int g = p.tid; g < GS && p.slice * GS + g < GROUPS; g += THREADS) {
             float* s = stats + ((long long)p.image * GROUPS + p.slice * GS + g) * 2;
-            s[0] = sum[g] * count;
+            s[0] = mean_of(sum[g], c.pixels);
             s[1] = inverse_deviation(squares[g], pixels);
         }
     apply(v, c, p, k, out, codes, exponents, mean, rstd, w, b);
@@ -188,10 +192,9 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(void*, unsigned char*, unsigned char*, float* __
     pw::Unit v[UN];
     load_units<UN, 0>(v, c);
     moments(v, c, p, k, red, sum, squares);
-    const float count = pw::reciprocal((float)c.pixels * CG);
     for (int g = p.tid; g < GS && p.slice * GS + g < GROUPS; g += THREADS) {
         float* s = partials + (((long long)p.image * GROUPS + p.slice * GS + g) * stretches + p.stretch) * 2;
-        s[0] = sum[g] * count;
+        s[0] = mean_of(sum[g], c.pixels);
         s[1] = squares[g];
     }
 }

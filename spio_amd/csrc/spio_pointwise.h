@@ -123,6 +123,13 @@ PW_DEVICE float reciprocal(float v) {
     return __builtin_fmaf(__builtin_fmaf(-v, r, 1.f), r, r);
 }
 
+// s / n for a count n with r = reciprocal(n), exact where s is a multiple of n: the mean of n equal values is that value, and
+// they have no difference to it (s * r may be a step off, which is a whole deviation where there is no other).
+PW_DEVICE float quotient(float s, float n, float r) {
+    const float q = s * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, n, s), r, q);
+}
+
 // ---- activations ----
 
 // 1 / (1 + exp(-z)); the hardware's exponential and reciprocal are within a unit in the last place.

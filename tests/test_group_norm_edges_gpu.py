@@ -21,6 +21,20 @@ def _is_split(shape, groups, dtype, configs=_get_configs, **more):
     return config.split
 
 
+@pytest.mark.parametrize("value,dtype", [(3.0, HALF), (1000.0, HALF), (0.203125, BF16), (1.0e5, FLOAT), (2.0**65, BF16),
+                                         (-1.625 * 2.0**70, BF16), (1.25 * 2.0**66, FLOAT)])  # fmt: skip
+@pytest.mark.parametrize("shape,groups,split", SHAPES)
+def test_a_constant_group_is_its_bias(shape, groups, split, value, dtype):
+    """The values have at most ten bits and a stretch less than 2^14 of them: every sum is exact in 24 bits, the mean is
+    the value, and no difference is left, whatever the size of the value."""
+    assert _is_split(shape, groups, dtype, has_weight=False) == split
+    c = shape[1]
+    x = torch.full(shape, value, dtype=dtype, device="cuda").contiguous(memory_format=CL)
+    bias = torch.arange(c, dtype=torch.float32) / 8
+    y = group_norm_2d(x, groups, None, bias.cuda()).cpu().float()
+    assert torch.equal(y, bias[:, None, None].expand(shape))
+
+
 @pytest.mark.parametrize("shape,groups,split", SHAPES)
 def test_a_mean_whose_square_overflows(shape, groups, split):
     """Values around 1.2 * 2^64, 2^-9 of that apart: the squares of the differences stay finite, that of the mean does not.
