@@ -191,6 +191,7 @@ def group_norm_2d(
     Args:
         inputs: (N, C, H, W) float16, bfloat16 or float32; C a multiple of 8 (up to 4096) and of num_groups.
         weight, bias: optional (C,), any float type.
+        eps: positive and finite; below 2^-126 it counts as that.
         activation: "none", "relu", "silu" or "gelu".
         checkpoint_8bit: keep the input for the backward pass in 8 bits.
 

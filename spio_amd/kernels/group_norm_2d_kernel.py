@@ -68,6 +68,13 @@ class GroupNorm2dParams:
         return self.h * self.w
 
     @property
+    def kernel_eps(self) -> float:
+        """eps as the kernels add it: the nearest to it that float32 has a normal number for.  As less (or nothing) it would
+        leave a group without a deviation an infinite rstd, and NaN."""
+        info = torch.finfo(torch.float32)
+        return min(max(float(self.eps), info.tiny), info.max)
+
+    @property
     def shape(self):
         return (self.n, self.c, self.h, self.w)
 
@@ -243,7 +250,7 @@ def _defines(params: GroupNorm2dParams, config: GroupNorm2dConfig):
     return {
         "SPIO_GN_C": params.c, "SPIO_GN_GROUPS": params.groups, "SPIO_GN_SLICE": config.slice,
         "SPIO_GN_THREADS": config.threads, "SPIO_GN_UNITS": config.units, "SPIO_GN_SPLIT": config.split,
-        "SPIO_GN_ROWS": _rows(params, config.threads, config.slice), "SPIO_GN_EPS": f"{float(params.eps)!r}f",
+        "SPIO_GN_ROWS": _rows(params, config.threads, config.slice), "SPIO_GN_EPS": f"{params.kernel_eps!r}f",
         "SPIO_GN_HAS_WEIGHT": int(params.has_weight), "SPIO_GN_HAS_BIAS": int(params.has_bias),
         "SPIO_GN_KEPT": int(params.kept), "SPIO_DTYPE": params.dtype, "SPIO_ACT": params.activation,
     }  # fmt: skip

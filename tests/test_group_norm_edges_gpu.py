@@ -45,3 +45,22 @@ def test_a_mean_whose_square_overflows(shape, groups, split):
     (exact,) = group_norm(x, groups, None, None, 1e-5, "none")
     y = group_norm_2d(x.cuda().contiguous(memory_format=CL), groups)
     assert_within(y, exact, 2.0**-10 + 2.0**-16 * exact.abs().max() + rounding(exact, FLOAT))
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("eps", [1e-37, 1e-40, 1e-60, 1e-300, 1e40])
+def test_eps_beyond_the_normal_numbers(eps, python):
+    """One that float32 has no normal number for counts as the nearest that it has one for: a constant group still is its
+    bias, and a group with a deviation what it is without eps (or, with the largest, its bias)."""
+    held = native.Bypass() if python else None
+    bias = torch.arange(16.0) / 8
+    for hw in ((8, 8), (64, 64)):
+        x = torch.full((1, 16, *hw), 3.0)
+        y = group_norm_2d(x.cuda().contiguous(memory_format=CL), 2, None, bias.cuda(), eps).cpu()
+        assert torch.equal(y, bias[:, None, None].expand(y.shape))
+        x = torch.randn(1, 16, *hw, generator=torch.Generator().manual_seed(2))
+        (exact,) = group_norm(x, 2, None, bias, eps, "none")
+        y = group_norm_2d(x.cuda().contiguous(memory_format=CL), 2, None, bias.cuda(), eps)
+        assert_within(y, exact, 2.0**-16 * exact.abs().max())
+    if held:
+        held.release()
