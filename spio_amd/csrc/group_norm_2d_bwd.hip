@@ -298,12 +298,13 @@ PW_DEVICE void apply(Inputs (&in)[HELD], const float (&held)[UN][8], const Stret
 }
 
 // sums[i] = sum over `rows` rows of rows[row][i], i < 2 * C: workgroup `block` has 32 columns, THREADS / 32 slices of
-// rows, which meet in LDS.
-PW_DEVICE void add_rows(float* sums, const float* table, long long rows, int block, float* red) {
+// rows, which meet in LDS.  There may be as many rows as images and stretches: sixteen at a time are added in a tree of
+// 32 bits, and these sums in 64.  (In 32 bits a chain of 8192 equal terms was off by 2^-13.7.)
+PW_DEVICE void add_rows(float* sums, const float* table, long long rows, int block, double* red) {
     constexpr int PARTS_OF_ROWS = THREADS / 32;
     const int tid = (int)__builtin_amdgcn_workitem_id_x();
     const int col = block * 32 + tid % 32, part = tid / 32;
-    float s = 0.f;
+    double s = 0.;
     if (col < 2 * C) {
         for (long long r = part; r < rows; r += PARTS_OF_ROWS * 16) {
             float v[16];
@@ -313,14 +314,17 @@ PW_DEVICE void add_rows(float* sums, const float* table, long long rows, int blo
                 v[i] = row < rows ? table[row * (2 * C) + col] : 0.f;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s += v[i];
+            for (int step = 8; step; step /= 2)
+#pragma unroll
+                for (int i = 0; i < step; ++i) v[i] += v[i + step];
+            s += (double)v[0];
         }
     }
     red[tid] = s;
     sync();
     if (part == 0 && col < 2 * C) {
         for (int i = 1; i < PARTS_OF_ROWS; ++i) s += red[i * 32 + tid];
-        sums[col] = s;
+        sums[col] = (float)s;
     }
 }
 constexpr int ADDING = SPIO_GN_AFFINE ? (2 * C + 31) / 32 : 0;  // workgroups that add the rows
@@ -354,7 +358,7 @@ SPIO_GN_KERNEL SPIO_KERNEL_NAME(float* __restrict__ rows, void* __restrict__ din
 #if SPIO_GN_AFFINE
 SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _reduce)(float* __restrict__ sums, const float* __restrict__ rows,
                                                          long long images) {
-    __shared__ float red[THREADS];
+    __shared__ double red[THREADS];
     add_rows(sums, rows, images, (int)__builtin_amdgcn_workgroup_id_x(), red);
 }
 #endif
@@ -388,11 +392,15 @@ SPIO_GN_KERNEL SPIO_GN_CONCAT(SPIO_KERNEL_NAME, _apply)(
     float* __restrict__ sums, const float* __restrict__ rows, void* __restrict__ din, const void* __restrict__ in,
     const unsigned char* __restrict__ exponents, const void* __restrict__ dout, const float* __restrict__ stats,
     const float* __restrict__ weight, const float* __restrict__ bias, long long pixels, long long images) {
-    __shared__ float pairs[2 * GS > THREADS ? 2 * GS : THREADS];
+    __shared__ union {
+        float pairs[2 * GS];
+        double rows[THREADS];
+    } lds;
+    float* const pairs = lds.pairs;
     const unsigned stretches = (unsigned)((pixels + SPAN - 1) / SPAN);
     const unsigned block = __builtin_amdgcn_workgroup_id_x();
     if (block < ADDING) {
-        add_rows(sums, rows, images * stretches, (int)block, pairs);
+        add_rows(sums, rows, images * stretches, (int)block, lds.rows);
         return;
     }
     const Place p = place(block - ADDING, stretches);

@@ -47,6 +47,25 @@ def test_a_mean_whose_square_overflows(shape, groups, split):
     assert_within(y, exact, 2.0**-10 + 2.0**-16 * exact.abs().max() + rounding(exact, FLOAT))
 
 
+@pytest.mark.parametrize("shape,split", [((65536, 8, 1, 1), 1), ((33000, 16, 2, 1), 1), ((16384, 64, 8, 8), 0)])
+def test_sums_over_very_many_images(shape, split):
+    """Rows of sums are added in trees and in 64 bits: grad_bias is within 2^-19 of the sum of the terms' magnitudes (the
+    workgroups' own chains and trees 2^-20), also where all terms are equal and roundings of a long chain all go one
+    way.  One image's share is 2^-16 or more."""
+    n, c, h, w = shape
+    assert _is_split(shape, 2, FLOAT, _get_bwd_configs, has_weight=False) == split
+    bias = torch.zeros(c, device="cuda", requires_grad=True)
+    x = torch.randn(n, h, w, c, device="cuda", dtype=FLOAT).permute(0, 3, 1, 2)
+    y = group_norm_2d(x, 2, None, bias)
+    same = torch.full((n, h, w, c), 0.1, device="cuda", dtype=FLOAT).permute(0, 3, 1, 2)
+    g = torch.Generator("cuda").manual_seed(1)
+    mixed = torch.empty(n, h, w, c, device="cuda", dtype=FLOAT).normal_(generator=g).permute(0, 3, 1, 2)
+    for dy in (same, mixed):
+        (db,) = torch.autograd.grad(y, bias, dy, retain_graph=True)
+        terms = dy.permute(0, 2, 3, 1).reshape(-1, c).double()
+        assert_within(db, terms.sum(0).cpu(), 2.0**-19 * terms.abs().sum(0).cpu())
+
+
 @pytest.mark.parametrize("python", [False, True])
 @pytest.mark.parametrize("eps", [1e-37, 1e-40, 1e-60, 1e-300, 1e40])
 def test_eps_beyond_the_normal_numbers(eps, python):
