@@ -2,6 +2,8 @@
 //
 //   SPIO_MODE 0  forward    y = act(x), and x in the 8-bit form (SPIO_KEEP)      (y, codes, exponents, x, n)
 //   SPIO_MODE 1  backward   dx = dy * act'(x as it was kept)                     (dx, codes, exponents, dy, n)
+//                (relu keeps a bit a value in place of the codes, whether its gradient passes: its derivative jumps at
+//                zero, where half a step of the 8-bit form would lose it whole; there are no exponents)
 //   SPIO_MODE 2  pack       x in the 8-bit form                                  (codes, exponents, x, n)
 //   SPIO_MODE 3  unpack     the values that codes and exponents stand for        (x, codes, exponents, n)
 //
@@ -28,8 +30,10 @@ namespace {
 constexpr int THREADS = SPIO_THREADS;
 constexpr int UN = SPIO_UNROLL;
 constexpr bool kReadsValues = SPIO_MODE != 3;
-constexpr bool kReadsCodes = SPIO_MODE == 1 || SPIO_MODE == 3;
-constexpr bool kWritesCodes = SPIO_MODE == 2 || (SPIO_MODE == 0 && SPIO_KEEP);
+constexpr bool kBits = SPIO_ACT == 1 && SPIO_MODE < 2;  // a byte a unit, bit e that of its value e
+constexpr bool kReadsCodes = (SPIO_MODE == 1 && !kBits) || SPIO_MODE == 3;
+constexpr bool kWritesCodes = SPIO_MODE == 2 || (SPIO_MODE == 0 && SPIO_KEEP && !kBits);
+constexpr bool kReadsBits = SPIO_MODE == 1 && kBits, kWritesBits = SPIO_MODE == 0 && SPIO_KEEP && kBits;
 constexpr bool kWritesValues = SPIO_MODE != 2;
 
 #if SPIO_DTYPE == 2
@@ -93,11 +97,12 @@ SPIO_KERNEL_NAME(
     const pw_rsrc rs_out = pw::buffer(out + first * 8, kWritesValues ? whole * pw::UNIT_BYTES : 0);
     const pw_rsrc rs_codes = pw::buffer(codes + first * 8, kReadsCodes || kWritesCodes ? whole * 8 : 0);
     const pw_rsrc rs_exp = pw::buffer(exponents + first / 4, kReadsCodes || kWritesCodes ? (values + 31) / 32 : 0);
+    const pw_rsrc rs_bits = pw::buffer(codes + first, kReadsBits || kWritesBits ? (values + 7) / 8 : 0);
 
     const pw::Constants constants;
     pw::Unit v[UN];
     pw_uint2 c[UN];
-    unsigned ex[UN];
+    unsigned ex[UN], bits[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
         const int unit = u * THREADS + tid;
@@ -106,6 +111,7 @@ SPIO_KERNEL_NAME(
             c[u] = __builtin_amdgcn_raw_buffer_load_b64(rs_codes, unit * 8, 0, pw::STREAM);
             ex[u] = __builtin_amdgcn_raw_buffer_load_b8(rs_exp, unit / 4, 0, 0);
         }
+        if (kReadsBits) bits[u] = __builtin_amdgcn_raw_buffer_load_b8(rs_bits, unit, 0, 0);
     }
     if (part) {  // the last unit of the tensor
 #pragma unroll
@@ -130,12 +136,20 @@ SPIO_KERNEL_NAME(
             __builtin_amdgcn_raw_buffer_store_b64(c[u], rs_codes, unit * 8, 0, pw::STREAM);
             __builtin_amdgcn_raw_buffer_store_b8((unsigned char)ex[u], rs_exp, tid % 4 == 0 ? unit / 4 : (int)pw::OOB, 0, 0);
         }
+        if (kWritesBits) {
+            bits[u] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bits[u] |= pw::passes(pw::value(v[u], e)) ? 1u << e : 0u;
+            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)bits[u], rs_bits, unit, 0, 0);
+        }
         if (kWritesValues) {
             float y[8];
             const float step = kReadsCodes ? pw::block_step(ex[u]) : 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if (SPIO_MODE == 1)
+                if (kReadsBits)
+                    y[e] = bits[u] >> e & 1 ? pw::value(v[u], e) : 0.f;
+                else if (SPIO_MODE == 1)
                     y[e] = pw::activate_grad<SPIO_DTYPE != 2>(v[u], e, pw::code(c[u], e) * step, constants);
                 else if (SPIO_MODE == 3)
                     y[e] = finite(pw::code(c[u], e) * step);

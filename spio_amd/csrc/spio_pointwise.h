@@ -178,10 +178,13 @@ PW_DEVICE float activate(float z) {
     return z;
 }
 
+// Whether relu's gradient at z is the output's (as torch has it: at NaN it is)
+PW_DEVICE bool passes(float z) { return !(z <= 0.f); }
+
 // value e of dy times the activation's derivative at z (SHORT as in normal)
 template <bool SHORT>
 PW_DEVICE float activate_grad(const Unit& dy, int e, float z, const Constants& k) {
-    if (SPIO_ACT == 1) return z > 0.f ? value(dy, e) : 0.f;
+    if (SPIO_ACT == 1) return passes(z) ? value(dy, e) : 0.f;
     if (SPIO_ACT == 2) {
         const float s = sigmoid(z);
         return times(dy, e, __builtin_fmaf(s, __builtin_fmaf(-z, s, z), s), k);  // s + s z (1 - s)

@@ -684,15 +684,19 @@ Tensor dense(const Tensor& t) { return aligned(t.is_non_overlapping_and_dense() 
 struct Kept {
     Tensor codes, exponents;
 };
-Kept empty_kept(const Tensor& x) {
-    return {empty_1d(x.numel(), at::kChar, x), empty_1d(blocks(x.numel()), at::kByte, x)};
+// Bytes of codes and of exponents of n values: one a value and one a block, or, for relu, a bit a value and none.
+constexpr int64_t RELU = 1;
+int64_t code_bytes(int64_t n, int64_t act = 0) { return act == RELU ? (n + 7) / 8 : n; }
+int64_t exponent_bytes(int64_t n, int64_t act = 0) { return act == RELU ? 0 : blocks(n); }
+Kept empty_kept(const Tensor& x, int64_t act = 0) {
+    return {empty_1d(code_bytes(x.numel(), act), at::kChar, x), empty_1d(exponent_bytes(x.numel(), act), at::kByte, x)};
 }
 
 // y of x, a tensor without gaps, and x in the 8-bit form where `kept` is given.
 Tensor activation_forward(const Tensor& x, int64_t act, Kept* kept) {
     const auto plan = find_plan(values_key(ACTIVATION, x, dtype_number(x), act, kept != nullptr));
     const Tensor y = empty_as(x, x.scalar_type());
-    if (kept) *kept = empty_kept(x);
+    if (kept) *kept = empty_kept(x, act);
     launch_values(*plan, x.numel(), c10::hip::getCurrentHIPStream(x.get_device()),
                   {ptr(y), kept ? ptr(kept->codes) : nullptr, kept ? ptr(kept->exponents) : nullptr, ptr(x), number(x.numel())});
     return y;
@@ -715,7 +719,8 @@ struct ActivationFunction : torch::autograd::Function<ActivationFunction> {
         const Tensor &codes = saved[0], &exponents = saved[1], &grad = grads[0];
         const int64_t n = grad.numel();
         const bool native = !stands_aside(grad) && grad.scalar_type() == static_cast<at::ScalarType>(v[1]) &&
-                            is_again(codes, grad, {n}, at::kChar) && is_again(exponents, grad, {blocks(n)}, at::kByte);
+                            is_again(codes, grad, {code_bytes(n, v[0])}, at::kChar) &&
+                            is_again(exponents, grad, {exponent_bytes(n, v[0])}, at::kByte);
         if (!native) {
             py::gil_scoped_acquire gil;
             return {py::reinterpret_borrow<py::object>(g_activation_gradient)(grad, codes, exponents, ACTIVATIONS[v[0]], strides)

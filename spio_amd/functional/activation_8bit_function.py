@@ -60,18 +60,20 @@ def _require_gpu(t, what):
         raise ValueError(f"spio::{what} runs on the GPU only")
 
 
-def _exponents(n):
-    return divup(n, BLOCK)
+def _kept_sizes(n, activation=None):
+    """Bytes of codes and of exponents: one a value and one a block, or, for relu, a bit a value and none."""
+    return (divup(n, 8), 0) if activation == "relu" else (n, divup(n, BLOCK))
 
 
-def _empty_kept(t, kept=True):
-    n = t.numel() if kept else 0
-    return t.new_empty((n,), dtype=torch.int8), t.new_empty((_exponents(n),), dtype=torch.uint8)
+def _empty_kept(t, kept=True, activation=None):
+    sizes = _kept_sizes(t.numel() if kept else 0, activation)
+    return t.new_empty((sizes[0],), dtype=torch.int8), t.new_empty((sizes[1],), dtype=torch.uint8)
 
 
-def _check_kept(codes, exponents, n, device):
-    assert codes.dtype == torch.int8 and tuple(codes.shape) == (n,), "codes of another tensor"
-    assert exponents.dtype == torch.uint8 and tuple(exponents.shape) == (_exponents(n),), "exponents of another tensor"
+def _check_kept(codes, exponents, n, device, activation=None):
+    sizes = _kept_sizes(n, activation)
+    assert codes.dtype == torch.int8 and tuple(codes.shape) == (sizes[0],), "codes of another tensor"
+    assert exponents.dtype == torch.uint8 and tuple(exponents.shape) == (sizes[1],), "exponents of another tensor"
     assert codes.device == exponents.device == device, "codes and exponents must be on one device"
 
 
@@ -149,13 +151,14 @@ def _check_activation(inputs, activation):
 @torch.library.custom_op("spio::activation_8bit_forward", mutates_args=())
 def activation_8bit_forward(inputs: torch.Tensor, activation: str,
                             keep: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
-    """(act(inputs), codes, exponents) of a tensor without gaps; the last two are empty unless `keep`."""
+    """(act(inputs), codes, exponents) of a tensor without gaps; the last two are empty unless `keep`.  relu's codes are
+    a bit a value, whether its gradient passes there (bit e of byte u is value 8u + e's), and it has no exponents."""
     _check_activation(inputs, activation)
     assert inputs.numel() == 0 or _is_dense(inputs.shape, inputs.stride()), "activation_8bit takes a tensor without gaps"
     _require_gpu(inputs, "activation_8bit")
     x = aligned(inputs)
     out = torch.empty_like(x)
-    codes, exponents = _empty_kept(x, keep)
+    codes, exponents = _empty_kept(x, keep, activation)
     n = x.numel()
     if n:
         params = Activation8bitParams(DTYPES[x.dtype], ACTIVATIONS[activation], keep)
@@ -167,17 +170,17 @@ def activation_8bit_forward(inputs: torch.Tensor, activation: str,
 @activation_8bit_forward.register_fake
 def _activation_fake(inputs, activation, keep):
     _check_activation(inputs, activation)
-    return (torch.empty_like(inputs), *_empty_kept(inputs, keep))
+    return (torch.empty_like(inputs), *_empty_kept(inputs, keep, activation))
 
 
 @torch.library.custom_op("spio::activation_8bit_backward", mutates_args=())
 def activation_8bit_backward(grad_output: torch.Tensor, codes: torch.Tensor, exponents: torch.Tensor,
                              activation: str) -> torch.Tensor:  # fmt: skip
-    """grad_output * act'(the kept input); grad_output lies in memory as the input did."""
+    """grad_output * act'(the kept input), for relu act'(the input); grad_output lies in memory as the input did."""
     _check_activation(grad_output, activation)
     n = grad_output.numel()
     assert n == 0 or _is_dense(grad_output.shape, grad_output.stride())
-    _check_kept(codes, exponents, n, grad_output.device)
+    _check_kept(codes, exponents, n, grad_output.device, activation)
     _require_gpu(grad_output, "activation_8bit")
     dy = aligned(grad_output)
     grad_input = torch.empty_like(dy)
@@ -227,7 +230,8 @@ activation_8bit_forward.register_autograd(_backward, setup_context=_setup_contex
 
 def activation_8bit(inputs: torch.Tensor, activation: str = "gelu") -> torch.Tensor:
     """relu, silu or gelu (of the normal distribution) of a GPU tensor of any shape, in its type; what the backward
-    pass needs of the input is kept in 8 bits."""
+    pass needs of the input is kept in 8 bits.  relu needs its sign only and keeps that, in one bit: its gradient is the
+    input's own."""
     y = native.call("activation_8bit", inputs, activation)
     if y is not NotImplemented:
         return y

@@ -10,7 +10,8 @@ from .group_norm_2d import TORCH_ACTIVATIONS
 
 class Activation8bit(nn.Module):
     """`nn.ReLU`, `nn.SiLU` or `nn.GELU` (activation "relu", "silu", "gelu") on GPU tensors of float16, bfloat16 or
-    float32; tensors elsewhere and of other types take torch's function, which is the same and keeps its input as it is."""
+    float32; what the backward pass needs of these is kept in 8 bits a value, of relu's in one.  Tensors elsewhere and of
+    other types take torch's function, which is the same and keeps its input as it is."""
 
     def __init__(self, activation="gelu"):
         super().__init__()
