@@ -110,13 +110,14 @@ PW_DEVICE void apply(pw::Unit (&v)[COUNT], const Stretch& c, const Place& p, con
     const unsigned bytes = (unsigned)c.pixels * (C * pw::VALUE_BYTES);
     const pw_rsrc rs_out = pw::buffer(reinterpret_cast<unsigned char*>(out) + c.first * (C * pw::VALUE_BYTES), bytes);
     const pw_rsrc rs_codes = pw::buffer(codes + c.first * C, SPIO_GN_KEPT ? (unsigned)c.pixels * C : 0);
-    const pw_rsrc rs_exp = pw::buffer(exponents + c.first * BLOCKS, SPIO_GN_KEPT ? (unsigned)c.pixels * BLOCKS : 0);
+    const pw_rsrc rs_exp = pw::buffer(exponents + c.first * EXP_ROW, SPIO_GN_KEPT ? (unsigned)c.pixels * EXP_ROW : 0);
     float scale[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) scale[e] = rstd[e / KEY_CHANNELS] * (SPIO_GN_HAS_WEIGHT ? w[e] : 1.f);
     // (the codes and exponents of lanes without any are stored behind the end of theirs)
     const unsigned off_codes = p.live ? (unsigned)(p.row * C + p.channel) : pw::OOB;
-    const unsigned off_exp = p.live && p.tid % 4 == 0 ? (unsigned)(p.row * BLOCKS + p.channel / 32) : pw::OOB;
+    const unsigned off_exp = p.live && p.tid % 4 == 0 ? (unsigned)(p.row * EXP_ROW + p.channel / 32) : pw::OOB;
+    const unsigned off_bits = p.live ? (unsigned)(p.row * EXP_ROW + BLOCKS + p.channel / 8) : pw::OOB;
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
         const pw::Unit x = v[u % COUNT];
@@ -130,7 +131,13 @@ PW_DEVICE void apply(pw::Unit (&v)[COUNT], const Stretch& c, const Place& p, con
         if (SPIO_GN_KEPT) {
             const unsigned ex = pw::block_exponent(x);
             __builtin_amdgcn_raw_buffer_store_b64(pw::encode(x, ex), rs_codes, (int)(off_codes + u * (ROWS * C)), 0, pw::STREAM);
-            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)ex, rs_exp, (int)(off_exp + u * (ROWS * BLOCKS)), 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)ex, rs_exp, (int)(off_exp + u * (ROWS * EXP_ROW)), 0, 0);
+        }
+        if (kBits) {
+            unsigned bits = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bits |= pw::passes(y[e]) ? 1u << e : 0u;  // (relu of z passes where z does)
+            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)bits, rs_exp, (int)(off_bits + u * (ROWS * EXP_ROW)), 0, 0);
         }
         if (u + COUNT < UN) v[u % COUNT] = pw::load_unit<pw::STREAM>(c.in, c.off + (u + COUNT) * STEP);
         __builtin_amdgcn_sched_barrier(0);

@@ -29,7 +29,7 @@ using namespace gn;
 struct Inputs {  // a unit of the norm's input, as the backward pass has it, and of grad_output
 #if SPIO_GN_KEPT
     pw_uint2 code;
-    unsigned exponent;
+    unsigned exponent, bits;
 #else
     pw::Unit x;
 #endif
@@ -42,7 +42,7 @@ constexpr unsigned STEP = (unsigned)(ROWS * C) * pw::VALUE_BYTES;
 struct Stretch {
     int pixels;         // from its first on
     unsigned off;       // of the lane's first unit; the others follow STEP apart
-    unsigned off_codes, off_exp;
+    unsigned off_codes, off_exp, off_bits;
     long long first;    // pixel of the tensors that the offsets start from
     pw_rsrc in, exponents, dout;
 };
@@ -57,9 +57,10 @@ PW_DEVICE Stretch stretch_of(const void* in, const unsigned char* exponents, con
     s.first = p.image * pixels + begin;
     s.off = p.live ? (unsigned)(p.row * C + p.channel) * pw::VALUE_BYTES : pw::OOB;
     s.off_codes = p.live ? (unsigned)(p.row * C + p.channel) : pw::OOB;
-    s.off_exp = p.live ? (unsigned)(p.row * BLOCKS + p.channel / 32) : pw::OOB;
+    s.off_exp = p.live ? (unsigned)(p.row * EXP_ROW + p.channel / 32) : pw::OOB;
+    s.off_bits = p.live ? (unsigned)(p.row * EXP_ROW + BLOCKS + p.channel / 8) : pw::OOB;
     s.in = pw::buffer(reinterpret_cast<const unsigned char*>(in) + s.first * (C * IN_BYTES), (unsigned)s.pixels * (C * IN_BYTES));
-    s.exponents = pw::buffer(exponents + s.first * BLOCKS, SPIO_GN_KEPT ? (unsigned)s.pixels * BLOCKS : 0);
+    s.exponents = pw::buffer(exponents + s.first * EXP_ROW, SPIO_GN_KEPT ? (unsigned)s.pixels * EXP_ROW : 0);
     s.dout = pw::buffer(reinterpret_cast<const unsigned char*>(dout) + s.first * (C * pw::VALUE_BYTES),
                         (unsigned)s.pixels * (C * pw::VALUE_BYTES));
     return s;
@@ -70,7 +71,8 @@ PW_DEVICE Inputs load_inputs(const Stretch& s, int u) {
     Inputs in;
 #if SPIO_GN_KEPT
     in.code = __builtin_amdgcn_raw_buffer_load_b64(s.in, (int)(s.off_codes + u * (ROWS * C)), 0, POLICY);
-    in.exponent = __builtin_amdgcn_raw_buffer_load_b8(s.exponents, (int)(s.off_exp + u * (ROWS * BLOCKS)), 0, 0);
+    in.exponent = __builtin_amdgcn_raw_buffer_load_b8(s.exponents, (int)(s.off_exp + u * (ROWS * EXP_ROW)), 0, 0);
+    if (kBits) in.bits = __builtin_amdgcn_raw_buffer_load_b8(s.exponents, (int)(s.off_bits + u * (ROWS * EXP_ROW)), 0, 0);
 #else
     in.x = pw::load_unit<POLICY>(s.in, s.off + u * STEP);
 #endif
@@ -155,6 +157,12 @@ PW_DEVICE void work(float (&d)[8], float (&dz)[8], const Inputs& in, const Lane&
     centre(d, in, l);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
+#if SPIO_GN_KEPT
+        if (kBits) {
+            dz[e] = in.bits >> e & 1 ? pw::value(in.dy, e) : 0.f;
+            continue;
+        }
+#endif
         const float z = SPIO_GN_HAS_BIAS ? __builtin_fmaf(d[e], l.scale[e], l.b[e]) : d[e] * l.scale[e];
         dz[e] = pw::activate_grad<false>(in.dy, e, z, l.k);
     }

@@ -12,7 +12,9 @@
 // A workgroup's pixels form rows of ROWS: lane t has unit t % SUP of the pixels t / SUP + k * ROWS, the same eight channels
 // of all of them, and loads of neighbouring lanes are neighbours in memory.
 //
-// The 8-bit form's blocks are up to 32 channels of one pixel; its exponents lie in rows of ceil(C / 32) bytes.
+// The 8-bit form's blocks are up to 32 channels of one pixel; its exponents lie in rows of ceil(C / 32) bytes.  With
+// relu a byte for every eight channels follows them in the row: bit e, whether the gradient of that output passes.  (Its
+// derivative jumps at zero: the kept input is on the other side of it where the output is less than half a step.)
 #ifndef SPIO_GROUP_NORM_H
 #define SPIO_GROUP_NORM_H
 
@@ -54,6 +56,8 @@ constexpr int ROWS = SPIO_GN_ROWS;
 constexpr int SPAN = ROWS * UN;                 // pixels that a workgroup holds
 constexpr int WAVES = THREADS / 64;
 constexpr int BLOCKS = (C + 31) / 32;           // exponents of a pixel
+constexpr bool kBits = SPIO_GN_KEPT && SPIO_ACT == 1;
+constexpr int EXP_ROW = BLOCKS + (kBits ? C / 8 : 0);
 static_assert(C % 8 == 0 && C % GROUPS == 0 && SLICE % 8 == 0 && SLICE % CG == 0 && SLICE <= C, "bad geometry");
 static_assert(SLICE == C || SLICE % 32 == 0, "a block lies in one slice");
 // Units that a lane has under way where it does not hold on to them (with 4, 6 or 8 of them 32n 48c 224x224 and 128n 96c

@@ -531,6 +531,7 @@ int64_t dtype_number(const Tensor& t) {
     }
 }
 constexpr const char* ACTIVATIONS[4] = {"none", "relu", "silu", "gelu"};
+constexpr int64_t RELU = 1;
 int64_t activation_number(PyObject* o) {
     if (!PyUnicode_CheckExact(o)) return -1;
     for (int i = 0; i < 4; ++i)
@@ -561,7 +562,7 @@ struct GroupNorm {
     }
     int64_t pixels() const { return h * w; }
     std::vector<int64_t> codes() const { return {n, h, w, c}; }
-    std::vector<int64_t> exponents() const { return {n, h, w, blocks(c)}; }
+    std::vector<int64_t> exponents() const { return {n, h, w, blocks(c) + (act == RELU ? c / 8 : 0)}; }  // (and relu's bits)
 };
 
 struct GroupNormOutput {
@@ -685,7 +686,6 @@ struct Kept {
     Tensor codes, exponents;
 };
 // Bytes of codes and of exponents of n values: one a value and one a block, or, for relu, a bit a value and none.
-constexpr int64_t RELU = 1;
 int64_t code_bytes(int64_t n, int64_t act = 0) { return act == RELU ? (n + 7) / 8 : n; }
 int64_t exponent_bytes(int64_t n, int64_t act = 0) { return act == RELU ? 0 : blocks(n); }
 Kept empty_kept(const Tensor& x, int64_t act = 0) {

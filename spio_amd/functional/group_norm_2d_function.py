@@ -5,8 +5,9 @@
 
 With `checkpoint_8bit` the forward pass writes its input in the 8-bit form of csrc/spio_pointwise.h (blocks of up to
 32 channels of a pixel, a power-of-two step each) and the backward pass reads that in the input's place: half of what
-a float16 input keeps, a quarter of a float32 one's.  Mean and rstd are those of the input itself.  The gradients are then those of the formula
-at the values the checkpoint stands for, each off by half a step at most.
+a float16 input keeps, a quarter of a float32 one's.  Mean and rstd are those of the input itself.  The gradients are
+then those of the formula at the values the checkpoint stands for, each off by half a step at most; but where relu's passes,
+which half a step would decide, is that of the input itself and kept in a bit a value more.
 
 The reference has no such operator; its sibling here is `layernorm_2d`.
 """
@@ -57,10 +58,9 @@ def _check(inputs, num_groups, weight, bias, eps, activation):
         assert t is None or t.device == inputs.device, "weight and bias must be on the inputs' device"
 
 
-def _empty_like_kept(inputs, kept):
-    """Codes and exponents of an input: [n, h, w, c] and [n, h, w, ceil(c / 32)], empty where it is not kept."""
-    n, c, h, w = inputs.shape
-    shapes = kept_shapes(n, c, h, w) if kept else ((0,), (0,))
+def _empty_like_kept(inputs, kept, activation):
+    """Codes and exponents of an input, empty where it is not kept."""
+    shapes = kept_shapes(*inputs.shape, ACTIVATIONS[activation]) if kept else ((0,), (0,))
     return inputs.new_empty(shapes[0], dtype=torch.int8), inputs.new_empty(shapes[1], dtype=torch.uint8)
 
 
@@ -70,7 +70,8 @@ def group_norm_2d_forward(
     activation: str, checkpoint_8bit: bool,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:  # fmt: skip
     """(output, statistics [n, groups, 2] = mean and rstd in float32, codes, exponents); the last two are empty
-    without `checkpoint_8bit`."""
+    without `checkpoint_8bit`.  Codes are [n, h, w, c], exponents [n, h, w, ceil(c / 32)], with relu followed by c / 8
+    bytes of bits, whether the gradient of an output passes."""
     _check(inputs, num_groups, weight, bias, eps, activation)
     if inputs.device.type != "cuda":
         raise ValueError("spio::group_norm_2d runs on the GPU only")
@@ -78,7 +79,7 @@ def group_norm_2d_forward(
     x = aligned(inputs.contiguous(memory_format=CL))
     out = torch.empty_like(x, memory_format=CL)
     stats = torch.empty((params.n, params.groups, 2), dtype=torch.float32, device=x.device)
-    codes, exponents = _empty_like_kept(x, params.kept)
+    codes, exponents = _empty_like_kept(x, params.kept, activation)
     if x.numel() == 0:
         return out, stats.zero_(), codes, exponents
     kernel = group_norm_2d_kernel_factory.get_kernel(params, x.device)
@@ -92,7 +93,7 @@ def _forward_fake(inputs, num_groups, weight, bias, eps, activation, checkpoint_
     _check(inputs, num_groups, weight, bias, eps, activation)
     return (torch.empty_like(inputs, memory_format=CL),
             inputs.new_empty((inputs.shape[0], num_groups, 2), dtype=torch.float32),
-            *_empty_like_kept(inputs, checkpoint_8bit))  # fmt: skip
+            *_empty_like_kept(inputs, checkpoint_8bit, activation))  # fmt: skip
 
 
 @torch.library.custom_op("spio::group_norm_2d_backward", mutates_args=())
@@ -111,7 +112,7 @@ def group_norm_2d_backward(
     assert inputs.device == stats.device == grad_output.device
     assert stats.dtype == torch.float32 and tuple(stats.shape) == (n, num_groups, 2), "statistics of another norm"
     if kept:
-        shapes = kept_shapes(n, c, h, w)
+        shapes = kept_shapes(n, c, h, w, ACTIVATIONS[activation])
         assert inputs.dtype == torch.int8 and tuple(inputs.shape) == shapes[0], "codes of another input"
         assert exponents.dtype == torch.uint8 and tuple(exponents.shape) == shapes[1], "exponents of another input"
         assert exponents.device == grad_output.device

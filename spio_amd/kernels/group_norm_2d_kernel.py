@@ -7,7 +7,8 @@ that the compiled code is one file for all that get the same configuration.
 Arguments, forward:  (output, codes, exponents, stats, input, weight, bias, pixels, images)
           backward:  (sums, grad_input, input or codes, exponents, grad_output, stats, weight, bias, pixels, images)
 `stats` is float32 [n][groups][2] (mean, rstd), `sums` float32 [2][c] (0 = grad_weight, 1 = grad_bias), absent where
-there are neither.  Codes and exponents are the input in the 8-bit form of csrc/spio_pointwise.h.
+there are neither.  Codes and exponents are the input in the 8-bit form of csrc/spio_pointwise.h (relu's exponents with a
+bit a value more: kept_shapes).
 """
 
 from dataclasses import dataclass
@@ -313,14 +314,15 @@ def _images(params, device):
     return x.contiguous(memory_format=torch.channels_last)
 
 
-def kept_shapes(n, c, h, w):
-    """Shapes of the codes and exponents of an input that is kept in 8 bits (channels innermost)."""
-    return (n, h, w, c), (n, h, w, divup(c, 32))
+def kept_shapes(n, c, h, w, activation=0):
+    """Shapes of the codes and exponents of an input that is kept in 8 bits (channels innermost); relu's exponents are
+    followed by a byte for every eight channels, whether the gradient of each output passes."""
+    return (n, h, w, c), (n, h, w, divup(c, 32) + (c // 8 if activation == ACTIVATIONS["relu"] else 0))
 
 
 def _make_test_args(params: GroupNorm2dParams, device):
     codes, exponents = (torch.empty(s, device=device, dtype=torch.uint8) if params.kept else None
-                        for s in kept_shapes(*params.shape))  # fmt: skip
+                        for s in kept_shapes(*params.shape, params.activation))  # fmt: skip
     x = _images(params, device)
     stats = torch.empty((params.n, params.groups, 2), device=device)
     return (torch.empty_like(x), codes, exponents, stats, x, *_vectors(params, device), params.pixels, params.n)
@@ -329,7 +331,7 @@ def _make_test_args(params: GroupNorm2dParams, device):
 def _make_bwd_test_args(params: GroupNorm2dParams, device):
     dy = _images(params, device)
     if params.kept:
-        codes, exponents = kept_shapes(*params.shape)
+        codes, exponents = kept_shapes(*params.shape, params.activation)
         x = torch.randint(0, 256, codes, device=device, dtype=torch.uint8)
         exponents = torch.full(exponents, 126, device=device, dtype=torch.uint8)
     else:

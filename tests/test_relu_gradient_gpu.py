@@ -105,8 +105,72 @@ def _norm_exact(x, dy, groups, weight, bias):
     return z, out[1:], w_terms, b_terms
 
 
-# whole images and stretches, a last block of 24 and of 8 channels, units that make no whole block
+# images that the backward pass holds whole (all channels and slices of 32) and in stretches, a last block of 24 and of 8 channels
 NORM_CASES = [
-    ((3, 24, 9, 7), 4, HALF, "wb", 0), ((2, 64, 14, 13), 8, BF16, "wb", 0), ((2, 320, 13, 11), 32, FLOAT, "w", 0),
+    ((3, 24, 9, 7), 4, HALF, "wb", 0), ((2, 64, 14, 13), 8, BF16, "wb", 1), ((24, 320, 13, 11), 10, FLOAT, "w", 0),
     ((1, 72, 60, 57), 9, HALF, "wb", 1), ((2, 96, 56, 56), 32, BF16, "", 1), ((1, 40, 75, 61), 10, FLOAT, "b", 1),
 ]  # fmt: skip
+
+
+@pytest.mark.parametrize("shape,groups,dtype,affine,split", NORM_CASES)
+def test_norm_with_relu_and_a_checkpoint(shape, groups, dtype, affine, split, path):
+    """Tolerances as in the tests of the norm: 2^-16 of a tensor's largest value, 2^-17 of a sum's terms."""
+    x, dy, weight, bias = _norm_tensors(shape, dtype, affine)
+    params = GroupNorm2dParams(*shape, groups, NUMBERS[dtype], 1, 1e-5, weight is not None, bias is not None, True)
+    assert _get_bwd_configs(params, get_device_attributes(0))[0].split == split
+    z, *_ = _norm_exact(x, dy, groups, weight, bias)
+    dy = torch.where(z.abs() < 2.0**-12 * z.abs().max(), 0, dy)  # where the arithmetic decides the sign
+    z, exact, w_terms, b_terms = _norm_exact(x, dy, groups, weight, bias)
+    rounded = values(*pack_rows(x.permute(0, 2, 3, 1))).permute(0, 3, 1, 2)
+    assert ((rounded > 0) != (x > 0)).any()
+    leaves = [None if t is None else t.cuda().requires_grad_() for t in (x.cuda().contiguous(memory_format=CL), weight, bias)]
+    y = group_norm_2d(leaves[0], groups, leaves[1], leaves[2], 1e-5, "relu", True)
+    wanted = z.clamp_min(0)
+    assert_within(y.detach(), wanted, 2.0**-16 * wanted.max() + rounding(wanted, dtype), "y")
+    dx, *rest = torch.autograd.grad(y, [t for t in leaves if t is not None], dy.cuda())
+    assert_within(dx, exact[0], 2.0**-16 * exact[0].abs().max() + rounding(exact[0], dtype), "dx")
+    sums = [(exact[1], w_terms), (exact[2], b_terms)]
+    for got, (e, terms) in zip(rest, [s for s, v in zip(sums, (weight, bias)) if v is not None]):
+        assert_within(got, e, 2.0**-17 * terms + 2.0**-40, "sums")
+
+
+def test_the_norms_operator():
+    """A pixel's row of exponents ends with a byte for every eight channels."""
+    x, dy, weight, bias = _norm_tensors((2, 72, 5, 6), HALF, "wb")
+    xg, wg, bg = (t.cuda().requires_grad_() for t in (x.cuda().contiguous(memory_format=CL), weight, bias))
+    y, _, codes, exponents = group_norm_2d_forward(xg, 9, wg, bg, 1e-5, "relu", True)
+    assert codes.shape == (2, 5, 6, 72) and exponents.shape == (2, 5, 6, 3 + 9)
+    expected_codes, expected_exponents = pack_rows(x.permute(0, 2, 3, 1))
+    assert torch.equal(codes.cpu(), expected_codes) and torch.equal(exponents[..., :3].cpu(), expected_exponents)
+    bits = (exponents[..., 3:, None].to(torch.int32) >> torch.arange(8, device="cuda") & 1).flatten(-2).bool()
+    assert torch.equal(bits, (y > 0).permute(0, 2, 3, 1))
+    torch.library.opcheck(group_norm_2d_forward, (xg, 9, wg, bg, 1e-5, "relu", True))
+    compiled = torch.compile(lambda x, w, b: group_norm_2d(x, 9, w, b, 1e-5, "relu", True), backend="aot_eager")
+    got = torch.autograd.grad(compiled(xg, wg, bg), [xg, wg, bg], dy.cuda())
+    expected = torch.autograd.grad(group_norm_2d(xg, 9, wg, bg, 1e-5, "relu", True), [xg, wg, bg], dy.cuda())
+    assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+def test_replays_of_a_captured_pass():
+    x = _with_outliers(3 * 24 * 9 * 7, HALF).reshape(3, 24, 9, 7).cuda().contiguous(memory_format=CL).requires_grad_()
+    dy = torch.randn_like(x)
+
+    def step():
+        y = activation_8bit(group_norm_2d(x, 3, activation="relu", checkpoint_8bit=True) - 0.5, "relu")
+        return [y.detach(), torch.autograd.grad(y, x, dy)[0]]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step()
+    for seed in range(3):
+        torch.manual_seed(seed)
+        with torch.no_grad():
+            x.copy_(torch.randn(3, 24, 9, 7, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
