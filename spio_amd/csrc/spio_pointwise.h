@@ -81,10 +81,6 @@ PW_DEVICE float value(const Unit& u, int e) {
     if (SPIO_DTYPE == 1) return as_float(e % 2 ? u.q[0][e / 2] & 0xffff0000u : u.q[0][e / 2] << 16);
     return (float)__builtin_bit_cast(pw_half8, u.q[0])[e];
 }
-PW_DEVICE void unpack(float (&v)[8], const Unit& u) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = value(u, e);
-}
 // The vector units are what most of these kernels wait for, so instructions count: a float16 value enters a
 // mixed-precision multiply-add instead of being converted, in products with a 1 and sums with a -0 that the compiler
 // does not know for such.
