@@ -13,9 +13,10 @@
 // values, so that loads are 16 bytes and four neighbouring lanes hold a block: its largest magnitude is two
 // steps through the data-parallel-primitive operand path, nothing meets in LDS.  A workgroup has one stretch of
 // THREADS * UNROLL units, all requested before the first is worked on: 256 * 2, which beats larger ones by up to a tenth.
-// 128n 384c 56x56 with gelu, 776 MB each way, forward 140 us (5.5 TB/s) and backward 139 by themselves, 245 one after the
-// other, where the checkpoint comes from the memory-side cache; vector instructions take as long (23 and 24 a value)
-// and run beside the loads.  128n 64c 56x56, 78 MB each way: pack 13.7-15 us (5.2-5.7 TB/s), unpack 13.2-13.8.
+// 128n 384c 56x56 with gelu, 776 MB each way, forward 140-148 us (5.2-5.5 TB/s) and backward 138 by themselves, 246 one after
+// the other, where the checkpoint comes from the memory-side cache; vector instructions take as long (23 and 22 a value)
+// and run beside the loads.  With relu, 636 MB each way, 98 and 97 us (6.5 TB/s), 194 one after the other.  128n 64c 56x56,
+// 78 MB each way: pack 13.1-15.0 us (5.2-5.9 TB/s), unpack 13.2-15.8.
 #include "spio_pointwise.h"
 
 #ifndef SPIO_MODE

@@ -10,16 +10,16 @@
 //
 // A value is read and written once where an image's slice of channels fits the registers of one workgroup (SPIO_GN_SPLIT 0:
 // one launch).  128n 768c 7x7 without activation takes 6.1 us for 19 MB, 3 of which any launch and its first load take;
-// 32n 192c 28x28 float32 with silu 11.7 us for 39 MB: 192 workgroups hold an image's slice each, all load at once, and none
+// 32n 192c 28x28 float32 with silu 11.6 us for 39 MB: 192 workgroups hold an image's slice each, all load at once, and none
 // stores before its last value has come.
 //
 // Otherwise (SPIO_GN_SPLIT 1) images are cut into stretches: one launch leaves mean and sum of squared differences of
 // every stretch and group, the second one combines them, in the same order always, while its own first loads are on
-// their way, and reads the input again.  32n 48c 224x224 with silu: 27.3 us for 155 MB (5.7 TB/s) and 44.1 us for 309 MB (7.0
+// their way, and reads the input again.  32n 48c 224x224 with silu: 27.8 us for 155 MB (5.6 TB/s) and 44.4 us for 309 MB (7.0
 // TB/s, part of it from the memory-side cache), where one pass would be 52 us at the rate of a copy.  Workgroups of
 // an image that hold their stretches and exchange sums through memory need no second read, but wait for each other: 79.5
-// us against 71.  The second launch issues vector instructions for 69 % of that time (78 % where it writes 8 bits too: 128n 96c
-// 56x56 16.2 and 28.6 us): rounding, packing and the activation are what it has besides its loads.
+// us where the pair took 73 to 78.  The second launch issues vector instructions for 75 % of that time (86 % where it writes 8
+// bits too: 128n 96c 56x56 16.3 and 28.6 us): rounding, packing and the activation are what it has besides its loads.
 //
 // Loads: the first launch's leave lines in the caches for the second, whose own and whose stores are streamed (plain
 // stores take the pair 10 to 25 % longer); the second launch has DEPTH units a lane under way, the first all of them.

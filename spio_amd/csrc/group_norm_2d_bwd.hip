@@ -8,12 +8,13 @@
 // The group's sums are those of its channels times their weights, so one pair of sums for each image and channel
 // serves all three gradients.  Where an image's slice of channels fits the registers of one workgroup (SPIO_GN_SPLIT 0)
 // input and gradient are read once, and a second launch adds the images' rows of channel sums: 128n 768c 7x7 without
-// activation 7.1 us for 30 MB and 2.8, 32n 192c 28x28 float32 with silu 16.3 us for 59 MB and 3.9.
+// activation 7.4 us for 30 MB and 2.9, 32n 192c 28x28 float32 with silu 16.3 us for 59 MB and 3.9.  (Its few workgroups walk all
+// rows: 4096n 64c 8x8 takes 20.6 us and 28.0.)
 //
 // Otherwise the first launch leaves a row of channel sums for every stretch and the pair of each group; the second one
 // reads input and gradient again, and its first workgroups add the rows meanwhile (as a launch of its own that takes 3
-// us).  128n 96c 56x56 with silu from 8 bits: 28.7 us for 121 MB and 33.0 us for 198 MB (6.0 TB/s).  Both issue vector
-// instructions for 83 to 88 % of their time: a value costs 17 or 18 of them in either launch, an exp and a rcp among them,
+// us).  128n 96c 56x56 with silu from 8 bits: 27.7 us for 121 MB and 32.8 us for 198 MB (6.0 TB/s).  Both issue vector
+// instructions for 81 to 86 % of their time: a value costs 15 or 16 of them in either launch, an exp and a rcp among them,
 // which count fourfold.  One launch whose workgroups exchange sums through memory waits more than it saves
 // (32n 48c 224x224 148 to 165 us against 125 to 144).  Nothing is atomic: every sum is made in the same order always.
 #include "spio_group_norm.h"

@@ -95,8 +95,9 @@ PW_DEVICE void sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
-// Workgroup `block` of `stretches` stretches an image: neighbours are slices of the same pixels (they share lines
-// where a slice is not whole lines), then stretches, then images.
+// Workgroup `block` of `stretches` stretches an image: neighbours are slices of the same pixels, then stretches, then images.
+// (Slices that are not whole lines share some.  Workgroups are dealt to the XCDs in turn, so neighbours have different
+// L2s and meet in the memory-side cache; what that costs is in the rule that chooses the slices.)
 PW_DEVICE Place place(unsigned block, unsigned stretches) {
     Place p;
     p.tid = (int)__builtin_amdgcn_workitem_id_x();

@@ -9,6 +9,9 @@ a float16 input keeps, a quarter of a float32 one's.  Mean and rstd are those of
 then those of the formula at the values the checkpoint stands for, each off by half a step at most; but where relu's passes,
 which half a step would decide, is that of the input itself and kept in a bit a value more.
 
+All sums are float32: those of a group's values and of the squares of their differences to the mean have to stay below
+its largest number (3.4e38), which bfloat16 and float32 values beyond 10^16 may pass.
+
 The reference has no such operator; its sibling here is `layernorm_2d`.
 """
 
@@ -194,7 +197,7 @@ def group_norm_2d(
         weight, bias: optional (C,), any float type.
         eps: positive and finite; below 2^-126 it counts as that.
         activation: "none", "relu", "silu" or "gelu".
-        checkpoint_8bit: keep the input for the backward pass in 8 bits.
+        checkpoint_8bit: keep the input for the backward pass in 8 bits (and a bit more for relu).
 
     Returns:
         (N, C, H, W) in the inputs' type, channels_last.

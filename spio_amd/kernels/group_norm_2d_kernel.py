@@ -132,7 +132,8 @@ def _span(params: GroupNorm2dParams, config: GroupNorm2dConfig) -> int:
 # 256 images, 48 to 1280 channels, 5x5 to 224x224): a launch, and for every round of workgroups over the device what the
 # units of a workgroup take.  us = LAUNCH + PER_UNIT * rounds * threads * units for whole images, us = LAUNCH +
 # PER_UNIT * units of the tensor / compute units + PER_JOIN * (joins - 1) in stretches, where the input is read twice; both for
-# 16-byte units.  Over 120 more random shapes the choice takes 1.02 times the best of ten others on average, at most 1.39.
+# 16-byte units.  Over 120 more random shapes the choice took 1.02 times the best of ten others on average, at most 1.39 (with
+# stretches of four or five lengths; any number of units since, which _best_stretches measures).
 # Whole images win where there are enough of them, us whole and in stretches: forward 128n 384c 14x14 9.5 and 12, 64n
 # 128c 28x28 9.6 and 11.3, 8n 1280c 8x8 5.6 and 6.9, but 4n 256c 32x32 8.5 and 7.1, 64n 192c 20x20 with one group 9.4 and 8.9;
 # backward 128n 384c 14x14 14.7 and 19.4, 32n 192c 28x28 float32 17.9 and 21.2, 64n 128c 28x28 13.8 and 14.7, but 4n 256c
@@ -143,10 +144,11 @@ _STRETCHES = {False: (6.2, 1.75e-3, 0.67), True: (6.6, 3.0e-3, 0.39)}
 
 def _shared_lines(params: GroupNorm2dParams, width: int, bwd: bool) -> float:
     """How much longer a pass takes where slices of `width` channels share lines of 128 bytes, which every one of them
-    touches, or sectors of 32, which none can write whole.  Fitted to 450 measurements (45 shapes).  us: 128n 384c 14x14 in
-    slices of 96 channels 10.4, of 192 9.5; with a checkpoint 64n 128c 28x28 in slices of 32 channels 15.6, of 64, half as many
-    workgroups, 11.4; 103n 328c 27x27 in slices of 64 75, in stretches 32.  Less where the caches hold it all: 10n 112c 10x10
-    in slices of 32 channels 3.8, of 64 5.3."""
+    touches, or sectors of 32, which none can write whole.  Fitted to 450 measurements (45 shapes), all with workgroups in
+    the order of gn::place, whose neighbours are on different XCDs.  us: 128n 384c 14x14 in slices of 96 channels 10.4, of
+    192 9.5; with a checkpoint 64n 128c 28x28 in slices of 32 channels 15.6, of 64, half as many workgroups, 11.4; 103n 328c
+    27x27 in slices of 64 75, in stretches 32.  Less where the caches hold it all: 10n 112c 10x10 in slices of 32 channels
+    3.8, of 64 5.3."""
     if width == params.c:
         return 1.0
     value = 4 if params.dtype == 2 else 2
