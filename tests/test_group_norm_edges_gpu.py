@@ -8,6 +8,7 @@ from spio_amd import native
 from spio_amd.functional import group_norm_2d
 from spio_amd.hip import get_device_attributes
 from spio_amd.kernels.group_norm_2d_kernel import GroupNorm2dParams, _get_bwd_configs, _get_configs, DTYPES
+from spio_amd.layers import GroupNorm2d
 from tests.pointwise_reference import CL, assert_within, group_norm, rounding
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +84,31 @@ def test_eps_beyond_the_normal_numbers(eps, python):
         assert_within(y, exact, 2.0**-16 * exact.abs().max())
     if held:
         held.release()
+
+
+@pytest.mark.parametrize("shape", [(128, 9, 5, 4), (200, 9, 5, 4), (129, 15, 7), (1000, 12), (300, 20, 1, 1)])
+@pytest.mark.parametrize("dtype", [HALF, FLOAT, torch.float64])
+def test_the_layer_on_more_images_than_torch_sums_right(shape, dtype):
+    """Tensors that the kernels do not take, against the same layer in 64 bits on the CPU.  Of the largest value: four steps of the
+    type for the roundings of norm, activation, their gradients and the result, and 2^-12 for float32 arithmetic on groups of
+    as few as three values, whose deviation may be a hundredth of them."""
+    g = torch.Generator().manual_seed(3)
+    n, c = shape[:2]
+    layer = GroupNorm2d(c // 3 if c % 3 == 0 else 4, c, activation="silu")
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.copy_((torch.rand(c, generator=g) + 0.5).to(dtype))
+    x, dy = (torch.randn(shape, generator=g).to(dtype) for _ in range(2))
+    exact = GroupNorm2d(layer.num_groups, c, activation="silu").double()
+    exact.load_state_dict(layer.state_dict())
+    xe, xg = x.double().requires_grad_(), x.cuda().requires_grad_()
+    expected = [exact(xe), *torch.autograd.grad(exact(xe), [xe, *exact.parameters()], dy.double())]
+    layer = layer.to(dtype).cuda()
+    y = layer(xg)
+    got = [y, *torch.autograd.grad(y, [xg, *layer.parameters()], dy.cuda())]
+    for a, e, name in zip(got, expected, ("y", "dx", "dw", "db")):
+        assert a.dtype == dtype and a.shape == e.shape
+        assert_within(a.detach(), e.detach(), (2.0**-12 + 4 * torch.finfo(dtype).eps) * e.detach().abs().max(), name)
+    with torch.autocast("cuda", dtype=HALF):
+        y = layer(xg)
+    assert y.dtype == (FLOAT if dtype == HALF else dtype)
