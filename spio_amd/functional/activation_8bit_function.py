@@ -24,7 +24,7 @@ from ..kernels.activation_8bit_kernel import (
 )
 from ..kernels.group_norm_2d_kernel import ACTIVATIONS, DTYPES
 from ..util.math import divup
-from .group_norm_2d_function import aligned, refuse_second_derivatives
+from .group_norm_2d_function import aligned, refuse_forward_derivatives, refuse_second_derivatives
 
 POINTWISE = tuple(name for name in ACTIVATIONS if name != "none")
 
@@ -235,5 +235,6 @@ def activation_8bit(inputs: torch.Tensor, activation: str = "gelu") -> torch.Ten
     y = native.call("activation_8bit", inputs, activation)
     if y is not NotImplemented:
         return y
+    refuse_forward_derivatives(inputs)
     keep = torch.is_grad_enabled() and inputs.requires_grad
     return activation_8bit_forward(dense(inputs), activation, keep)[0]

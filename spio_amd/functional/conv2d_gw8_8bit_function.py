@@ -11,7 +11,7 @@ import torch
 from .. import native
 from .activation_8bit_function import pack_8bit_op, unpack_8bit_op
 from .conv2d_gw8_function import conv2d_gw8, conv2d_gw8_backward_op
-from .group_norm_2d_function import refuse_second_derivatives
+from .group_norm_2d_function import refuse_forward_derivatives, refuse_second_derivatives
 
 CL = torch.channels_last
 
@@ -82,10 +82,12 @@ def conv2d_gw8_8bit(
     """conv2d_gw8 (the same arguments, checks and autocast rules) that keeps its input for grad_weight in 8 bits.
     Where no grad_weight is wanted it is conv2d_gw8."""
     if not (torch.is_grad_enabled() and weight.requires_grad):
+        refuse_forward_derivatives(inputs, weight, bias)
         return conv2d_gw8(inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)
     y = native.call("conv2d_gw8_8bit", inputs, weight, bias, stride, padding_y, padding_x, dilation, groups)
     if y is not NotImplemented:
         return y
+    refuse_forward_derivatives(inputs, weight, bias)
     if not torch.is_autocast_enabled("cuda"):
         assert inputs.dtype == torch.float16 and weight.dtype == torch.float16
         assert bias is None or bias.dtype == torch.float32

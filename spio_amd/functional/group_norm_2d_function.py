@@ -18,6 +18,7 @@ The reference has no such operator; its sibling here is `layernorm_2d`.
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import native
 from ..kernels.group_norm_2d_kernel import (
@@ -149,6 +150,12 @@ def refuse_second_derivatives():
         raise RuntimeError("an input that was kept in 8 bits has no second derivatives (create_graph=True)")
 
 
+def refuse_forward_derivatives(*tensors):
+    """The operators have no formula for forward mode; a tangent would vanish on the way, as if it were zero."""
+    if not torch.compiler.is_compiling() and any(t is not None and unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("no forward-mode derivatives of this operator")
+
+
 def group_norm_2d_gradients(grad_output, inputs, exponents, stats, num_groups, weight, bias, eps, activation, needs_input,
                             needs_weight, needs_bias):  # fmt: skip
     """Gradients of group_norm_2d in the types of the tensors they belong to, None where not needed."""
@@ -205,6 +212,7 @@ def group_norm_2d(
     y = native.call("group_norm_2d", inputs, num_groups, weight, bias, eps, activation, checkpoint_8bit)
     if y is not NotImplemented:
         return y
+    refuse_forward_derivatives(inputs, weight, bias)
     kept = bool(checkpoint_8bit) and torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (inputs, weight, bias))  # fmt: skip
     return group_norm_2d_forward(inputs, num_groups, weight, bias, eps, activation, kept)[0]
