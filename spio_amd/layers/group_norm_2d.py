@@ -15,8 +15,8 @@ class GroupNorm2d(nn.GroupNorm):
 
     GPU tensors [N, C, H, W] in float16, bfloat16 or float32 whose channel count is a multiple of 8 go through the
     `group_norm_2d` kernels (channels_last in memory, float32 arithmetic, the input's type out, under autocast too);
-    everything else takes torch's group_norm and activation, which are the same function.  `checkpoint_8bit`
-    keeps the kernels' input for the backward pass in 8 bits.
+    everything else takes torch's group_norm (with weight and bias outside it where its gradients of them would be wrong)
+    and activation, which are the same function.  `checkpoint_8bit` keeps the kernels' input for the backward pass in 8 bits.
     """
 
     def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, device=None, dtype=None, activation="none",
