@@ -101,11 +101,12 @@ def build_native(force: bool = True, verbose: bool = False) -> str:
 
 
 def extension_digest() -> str:
-    """What a _native.so is built from: its source, the header of the library it calls and torch's version."""
+    """What a _native.so is built from: its source, the headers it includes and torch's version."""
     import torch  # pylint: disable=import-outside-toplevel
 
     digest = hashlib.sha256(torch.__version__.encode())
-    for path in (os.path.join(CSRC_DIR, "spio_torch.cpp"), os.path.join(_include_dir(), "spio_hip.h")):
+    for path in (os.path.join(CSRC_DIR, "spio_torch.cpp"), os.path.join(CSRC_DIR, "spio_token_args.h"),
+                 os.path.join(_include_dir(), "spio_hip.h")):  # fmt: skip
         with open(path, "rb") as f:
             digest.update(f.read())
     return digest.hexdigest()[:32]
@@ -133,7 +134,7 @@ def build_extension(verbose: bool = False) -> str:
     if cxx is None:
         raise RuntimeError("no host C++ compiler found to build _native.so")
     root = os.path.dirname(torch.__file__)
-    includes = [_include_dir(), os.path.join(root, "include"),
+    includes = [_include_dir(), CSRC_DIR, os.path.join(root, "include"),
                 os.path.join(root, "include", "torch", "csrc", "api", "include"),
                 os.path.join(ROCM_HOME, "include"), sysconfig.get_paths()["include"]]  # fmt: skip
     tmp = f"{EXTENSION_PATH}.tmp{os.getpid()}"

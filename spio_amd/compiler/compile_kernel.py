@@ -13,7 +13,7 @@ from ..hip.driver import Function, Module, set_device
 from .compile import compile_hip, GFX_ARCH
 
 # Headers that kernel sources may include; handed to hipRTC as in-memory files.
-_HEADER_NAMES = ("spio_conv_common.h", "spio_pointwise.h", "spio_group_norm.h")
+_HEADER_NAMES = ("spio_conv_common.h", "spio_pointwise.h", "spio_group_norm.h", "spio_tokens.h", "spio_token_args.h")
 
 
 @functools.lru_cache(maxsize=None)

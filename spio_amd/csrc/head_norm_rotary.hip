@@ -1,0 +1,250 @@
+// Rotation of the heads of queries and keys by their positions, with or without a norm of every head before it (gfx950):
+//
+//   xhat = x rsqrt(mean(x^2) + eps),  n = xhat weight                       (SPIO_NORM; else n = x)
+//   angle = position frequency[i];  a pair (n1, n2) of channels becomes
+//   (n1 cos - n2 sin, n2 cos + n1 sin) scale,                               channels behind the pairs stay as they are
+//
+// Pair i is channels (2i, 2i + 1) (SPIO_INTERLEAVED) or (i, pairs + i).  Backward, the gradients are turned by the
+// negative angle, then
+//
+//   g = dn weight,  dx = rstd (g - xhat mean(g xhat)),  dweight = sum dn xhat
+//
+//   SPIO_MODE 0  forward
+//   SPIO_MODE 1  backward   sums over tokens and heads as partial sums, a row for every workgroup
+//   SPIO_MODE 2  sums       the partial sums added up
+//
+// A lane has two units of eight channels of a head, those of eight pairs where these are rotated; LANES neighbouring lanes
+// are a head, and a group of them has the same head numbers modulo `parts` of a token.  So cosines and sines are computed
+// once for all of these, and the sums of a norm cross lanes of a row only.  Angles are taken in turns in float64 (a
+// position of six digits leaves float32 no digits behind the turns), of which the fraction is exact in float32.
+// HBM-bound: 2 + 2 bytes a value forward, 2 + 2 + 2 backward for 16-bit types.
+#include "spio_tokens.h"
+
+#ifndef SPIO_MODE
+#error "SPIO_MODE, SPIO_HEAD, SPIO_NORM, SPIO_INTERLEAVED, SPIO_HEADS are required"
+#endif
+
+namespace {
+
+using tk::value_t;
+constexpr int D = SPIO_HEAD, UNITS = D / 8;
+constexpr int PAIRED = (UNITS + 1) / 2;  // lanes of a head that have channels
+constexpr int LANES = PAIRED <= 1 ? 1 : PAIRED <= 2 ? 2 : PAIRED <= 4 ? 4 : PAIRED <= 8 ? 8 : 16;
+constexpr int GROUPS = 256 / LANES;      // of a workgroup
+constexpr int U = SPIO_HEADS;            // heads requested at once
+constexpr bool BACK = SPIO_MODE == 1;
+static_assert(D % 8 == 0 && D <= 256, "heads of up to 256 channels, whole units");
+
+// cos and sin of a fraction of a turn in [-1/2, 1/2]: the nearest quarter turn, and the Taylor series of what is left, at
+// most pi / 4 (next terms 2e-10 and 2e-9)
+__device__ inline void cos_sin(float turn, float& c, float& s) {
+    const float quarter = __builtin_rintf(turn * 4.f);
+    const float x = __builtin_fmaf(quarter, -0.25f, turn) * 6.28318531f, q = x * x;
+    float sine = 2.75573192e-6f, cosine = -2.75573192e-7f;
+    sine = __builtin_fmaf(sine, q, -1.98412698e-4f);
+    sine = __builtin_fmaf(sine, q, 8.33333333e-3f);
+    sine = __builtin_fmaf(sine, q, -0.166666667f);
+    sine = __builtin_fmaf(sine * q, x, x);
+    cosine = __builtin_fmaf(cosine, q, 2.48015873e-5f);
+    cosine = __builtin_fmaf(cosine, q, -1.38888889e-3f);
+    cosine = __builtin_fmaf(cosine, q, 4.16666667e-2f);
+    cosine = __builtin_fmaf(cosine, q, -0.5f);
+    cosine = __builtin_fmaf(cosine, q, 1.f);
+    const int k = (int)quarter;
+    const float even = k & 1 ? sine : cosine, odd = k & 1 ? cosine : sine;
+    c = (k + 1) & 2 ? -even : even;
+    s = k & 2 ? -odd : odd;
+}
+
+// The two units of a lane, and the pairs in them
+struct Place {
+    int unit[2];   // -1: none
+    int pair;      // of the first one: eight pairs from there on, or none (>= pairs)
+    bool rotated;  // (SPIO_INTERLEAVED: the pairs before `pairs` are)
+};
+__device__ inline Place place(int lane, int pairs) {
+    Place p;
+    if (SPIO_INTERLEAVED) {
+        p.unit[0] = 2 * lane;
+        p.pair = 8 * lane;
+        p.unit[1] = p.unit[0] + 1;
+        p.rotated = true;
+    } else {
+        const int half = pairs / 8;
+        p.rotated = lane < half;
+        p.unit[0] = p.rotated ? lane : 2 * half + 2 * (lane - half);
+        p.unit[1] = p.rotated ? lane + half : p.unit[0] + 1;
+        p.pair = 8 * lane;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (p.unit[i] >= UNITS) p.unit[i] = -1;
+    return p;
+}
+
+// (v[0], v[1]) turned by the angles, or, `back`, by their negatives
+__device__ inline void rotate(float (&v)[2][8], const float (&c)[8], const float (&s)[8], bool rotated) {
+    if (!rotated) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float& a = SPIO_INTERLEAVED ? v[i / 4][i % 4 * 2] : v[0][i];
+        float& b = SPIO_INTERLEAVED ? v[i / 4][i % 4 * 2 + 1] : v[1][i];
+        const float turned = a * c[i] - b * s[i];
+        b = __builtin_fmaf(a, s[i], b * c[i]);
+        a = turned;
+    }
+}
+
+struct Rows {
+    const value_t *x, *dy;
+    value_t* out;
+    long long row, head;  // of x
+    int heads;
+};
+
+// The heads `part`, `part + parts`, ... of a token.
+__device__ inline void heads_of(const Rows& r, const Place& p, long long token, int part, int parts, const float (&c)[8],
+                                const float (&s)[8], const float (&w)[2][8], float eps, float (&dw)[2][8]) {
+    const value_t* x = r.x + token * r.row;
+    for (int first = part; first < r.heads; first += parts * U) {
+        pw::Unit in[U][2], grad[U][2];
+#pragma unroll
+        for (int h = 0; h < U; ++h) {
+            const int head = first + h * parts < r.heads ? first + h * parts : first;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                in[h][i] = grad[h][i] = pw::Unit{};
+                if (p.unit[i] < 0) continue;
+                if (SPIO_NORM || !BACK) in[h][i] = tk::load(x + head * r.head + p.unit[i] * 8);
+                if (BACK) grad[h][i] = tk::load(r.dy + (token * r.heads + head) * D + p.unit[i] * 8);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < U; ++h) {
+            const int head = first + h * parts;
+            const bool there = head < r.heads;
+            float v[2][8], g[2][8];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                tk::values(in[h][i], v[i]);
+                tk::values(grad[h][i], g[i]);
+            }
+            if (SPIO_NORM) {
+                float squares = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) squares = __builtin_fmaf(v[i][e], v[i][e], squares);
+                squares = tk::sum_of<LANES>(squares);
+                const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, 1.f / D, eps));
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] *= rstd;
+                if (BACK) {
+                    rotate(g, c, s, p.rotated);
+                    float dot = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (there) dw[i][e] = __builtin_fmaf(g[i][e], v[i][e], dw[i][e]);
+                            g[i][e] *= w[i][e];
+                            dot = __builtin_fmaf(g[i][e], v[i][e], dot);
+                        }
+                    dot = tk::sum_of<LANES>(dot) * (1.f / D);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) g[i][e] = rstd * __builtin_fmaf(-dot, v[i][e], g[i][e]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[i][e] *= w[i][e];
+                    rotate(v, c, s, p.rotated);
+                }
+            } else if (BACK) {
+                rotate(g, c, s, p.rotated);
+            } else {
+                rotate(v, c, s, p.rotated);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (there && p.unit[i] >= 0)
+                    tk::store(r.out + (token * r.heads + head) * D + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
+        }
+    }
+}
+
+__device__ inline void weights(const float* from, const Place& p, float (&w)[2][8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[i][e] = from && p.unit[i] >= 0 ? from[p.unit[i] * 8 + e] : 0.f;
+}
+
+}  // namespace
+
+#if SPIO_MODE < 2
+
+extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))) SPIO_KERNEL_NAME(const SpioRotaryArgs a) {
+    const int tid = (int)__builtin_amdgcn_workitem_id_x(), lane = tid % LANES;
+    const int pairs = (int)a.pairs, parts = (int)a.parts;
+    const Place p = place(lane, pairs);
+    const Rows q = {(const value_t*)a.q, (const value_t*)a.dq, (value_t*)a.q_out, a.q_row, a.q_head, (int)a.q_heads};
+    const Rows k = {(const value_t*)a.k, (const value_t*)a.dk, (value_t*)a.k_out, a.k_row, a.k_head, (int)a.k_heads};
+    float wq[2][8], wk[2][8], dwq[2][8] = {}, dwk[2][8] = {};
+    weights(SPIO_NORM ? a.q_weight : nullptr, p, wq);
+    weights(SPIO_NORM ? a.k_weight : nullptr, p, wk);
+    double frequency[8];  // turns a position
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        frequency[i] = p.rotated && p.pair + i < pairs ? a.frequencies[p.pair + i] * 0.15915494309189535 : 0.;
+    const long long groups = (long long)__builtin_amdgcn_grid_size_x() / LANES;
+    // (a group's lanes stay together: they cross lanes for the norm)
+    for (long long item = ((long long)__builtin_amdgcn_workgroup_id_x() * 256 + tid) / LANES; item < a.tokens * parts; item += groups) {
+        const long long token = item / parts;
+        const int part = (int)(item % parts);
+        const long long at = token % a.position_tokens;
+        const long long position = a.wide_positions ? ((const long long*)a.positions)[at] : ((const int*)a.positions)[at];
+        float c[8], s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double turns = (double)position * frequency[i];
+            cos_sin((float)(turns - __builtin_rint(turns)), c[i], s[i]);
+            if (p.rotated && p.pair + i < pairs) c[i] *= (float)a.scale, s[i] *= BACK ? -(float)a.scale : (float)a.scale;
+        }
+        heads_of(q, p, token, part, parts, c, s, wq, (float)a.eps, dwq);
+        heads_of(k, p, token, part, parts, c, s, wk, (float)a.eps, dwk);
+    }
+#if SPIO_MODE == 1 && SPIO_NORM
+    // the groups of a workgroup, one after the other
+    __shared__ float sums[GROUPS][D];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        tk::barrier();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (p.unit[i] >= 0) sums[tid / LANES][p.unit[i] * 8 + e] = which ? dwk[i][e] : dwq[i][e];
+        tk::barrier();
+        for (int d = tid; d < D; d += 256) {
+            float sum = 0.f;
+#pragma unroll 8
+            for (int g = 0; g < GROUPS; ++g) sum += sums[g][d];
+            a.partials[((long long)__builtin_amdgcn_workgroup_id_x() * 2 + which) * D + d] = sum;
+        }
+    }
+#endif
+}
+
+#else
+
+extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))) SPIO_KERNEL_NAME(const SpioRotaryArgs a) {
+    // (`parts` has the rows)
+    tk::column_sums({a.partials, a.sums, a.parts, D, 0, 2}, __builtin_amdgcn_workgroup_id_x());
+}
+
+#endif

@@ -30,6 +30,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <limits>
@@ -39,6 +40,7 @@
 #include <unordered_map>
 
 #include "spio_hip.h"
+#include "spio_token_args.h"
 
 namespace {
 
@@ -52,7 +54,9 @@ constexpr auto CL = at::MemoryFormat::ChannelsLast;
 
 enum Kind : int64_t {
     FPROP = 0, DGRAD = 1, WGRAD = 2, BGRAD = 3, NORM = 4, NORM_BWD = 5,
-    GROUP_NORM = 6, GROUP_NORM_BWD = 7, ACTIVATION = 8, ACTIVATION_BWD = 9, PACK = 10, UNPACK = 11
+    GROUP_NORM = 6, GROUP_NORM_BWD = 7, ACTIVATION = 8, ACTIVATION_BWD = 9, PACK = 10, UNPACK = 11,
+    CONV1D = 12, CONV1D_BWD = 13, CONV1D_SUMS = 14, CONV1D_STEP = 15, SCAN_ENDS = 16, SCAN = 17, SCAN_ENDS_BWD = 18, SCAN_BWD = 19,
+    SCAN_SUMS = 20, SCAN_STEP = 21, ROTARY = 22, ROTARY_BWD = 23, ROTARY_SUMS = 24
 };
 
 // What selects a plan: the kind, the device and the numbers of the problem.
@@ -805,6 +809,416 @@ struct ConvKeptFunction : torch::autograd::Function<ConvKeptFunction> {
     }
 };
 
+// ---- operators over sequences of tokens -----------------------------------------------------------------
+
+int64_t divup(int64_t n, int64_t d) { return (n + d - 1) / d; }
+
+// The launch of a kernel that takes one structure of arguments.
+void launch_structure(const Plan& plan, int64_t grid, hipStream_t stream, const void* args) {
+    TORCH_CHECK_VALUE(grid * plan.main.block[0] < (int64_t(1) << 32), "more workgroups than a launch can have");
+    void* params[1] = {const_cast<void*>(args)};
+    const Stage& s = plan.main;
+    const int rc = spio_hip_launch(s.function, static_cast<unsigned>(grid), 1, 1, s.block[0], 1, 1, s.lds, stream, params, 1);
+    TORCH_CHECK_VALUE(rc == 0, "kernel launch failed: ", spio_hip_last_error());
+}
+Key token_key(Kind kind, int64_t device, int64_t a, int64_t b, int64_t c = 0, int64_t d = 0) {
+    return {{kind, device, a, b, c, d, 0, 0, 0, 0, 0, 0}};
+}
+Tensor empty_of(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+constexpr int64_t SUM_COLUMNS = 16;  // of a workgroup that adds up partial sums
+
+// [.., values] as rows of values that are equally far apart, or a copy without gaps (functional/token_rows.py: rows_of)
+struct Rows {
+    Tensor t;
+    int64_t row = 0;
+};
+Rows rows_of(const Tensor& t, int64_t step = 1) {
+    if (!t.defined()) return {};
+    const int64_t last = t.size(-1);
+    int64_t row = last, outer = -1;  // outer: the distance that the next dimension outwards must have
+    bool even = true, seen = false;
+    for (int64_t i = t.dim() - 2; i >= 0; --i) {
+        if (t.size(i) == 1) continue;
+        if (!seen) row = t.stride(i);
+        even = even && (!seen || t.stride(i) == outer);
+        outer = t.size(i) * t.stride(i);
+        seen = true;
+    }
+    const bool fits = step == 1 || (row * t.element_size() % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+    if (even && fits && (last == 1 || t.stride(-1) == 1)) return {t, row};
+    return {t.clone(at::MemoryFormat::Contiguous), last};
+}
+Tensor whole(const Tensor& t) { return t.defined() ? aligned(t.contiguous()) : t; }  // without gaps, on 16 bytes
+
+// Whether the bytes from a tensor's first to its last value meet another's
+bool overlap(const Tensor& a, const Tensor& b) {
+    auto end = [](const Tensor& t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return reinterpret_cast<uintptr_t>(t.data_ptr()) + (last + 1) * t.element_size();
+    };
+    return a.numel() && b.numel() && reinterpret_cast<uintptr_t>(a.data_ptr()) < end(b) &&
+           reinterpret_cast<uintptr_t>(b.data_ptr()) < end(a);
+}
+bool on_16_bytes(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// Whether a state may be written to `out`: the same tensor, or one like it that shares nothing with it; nor with the inputs
+bool writable_state(const Tensor& state, const Tensor& out, std::initializer_list<Tensor> inputs) {
+    if (!is_plain(out) || out.sizes() != state.sizes() || out.scalar_type() != state.scalar_type() ||
+        out.device() != state.device() || !state.is_contiguous() || !out.is_contiguous() || !on_16_bytes(state) ||
+        !on_16_bytes(out) || (state.data_ptr() != out.data_ptr() && overlap(state, out)) || wants_grad(out) || out.is_inference())
+        return false;
+    return std::none_of(inputs.begin(), inputs.end(), [&](const Tensor& t) { return t.defined() && overlap(t, out); });
+}
+void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+float* floats(const Tensor& t) { return static_cast<float*>(mut(t)); }
+
+PyObject *g_conv1d_gradients = nullptr, *g_scan_gradients = nullptr, *g_rotary_gradients = nullptr;
+py::object to_py(const Tensor& t) { return t.defined() ? py::cast(t) : py::object(py::none()); }
+Tensor from_py(const py::tuple& r, int i) { return r[i].is_none() ? Tensor() : r[i].cast<Tensor>(); }
+int64_t type_of(const Tensor& t) { return static_cast<int64_t>(t.defined() ? t.scalar_type() : at::kFloat); }
+Tensor typed(const Tensor& t, int64_t type) {
+    return t.scalar_type() == static_cast<at::ScalarType>(type) ? t : t.to(static_cast<at::ScalarType>(type));
+}
+
+// ---- causal convolution ----
+
+struct Conv1d {
+    int64_t n, l, c, width, act;
+    bool keep_state = false;
+    Tensor before, after;  // states, which have no history
+};
+int64_t conv1d_slice(int64_t tokens, int64_t channels, int64_t sequences, bool backward) {
+    const int64_t lanes = channels / 8 * sequences, even = divup(tokens * lanes, 1 << 17);
+    if (backward) return std::max({int64_t(16), std::min(int64_t(256), even), divup(tokens * sequences, 4096)});
+    return std::max(int64_t(4), std::min(int64_t(32), even));
+}
+PlanPtr conv1d_plan(Kind kind, const Conv1d& cv, const Tensor& x, const Tensor& weight) {
+    return find_plan(token_key(kind, x.get_device(), cv.width, dtype_number(x), dtype_number(weight), cv.act));
+}
+Tensor conv1d_forward(Conv1d& cv, const Tensor& x, const Tensor& weight, const Tensor& bias) {
+    const auto plan = conv1d_plan(CONV1D, cv, x, weight);
+    const Rows rows = rows_of(x, 8);
+    const Tensor w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias, before = whole(cv.before);
+    const Tensor y = empty_of({cv.n, cv.l, cv.c}, x.scalar_type(), x);
+    if (cv.keep_state) cv.after = empty_of({cv.n, cv.width - 1, cv.c}, x.scalar_type(), x);
+    SpioConv1dArgs a = {};
+    a.x = ptr(rows.t), a.weight = ptr(w), a.bias = ptr(b), a.before = ptr(before), a.out = mut(y), a.after = mut(cv.after);
+    a.tokens = cv.l, a.channels = cv.c, a.sequences = cv.n, a.x_row = rows.row;
+    a.slice = conv1d_slice(cv.l, cv.c, cv.n, false);
+    launch_structure(*plan, divup(cv.n * divup(cv.l, a.slice) * (cv.c / 8), 256), c10::hip::getCurrentHIPStream(x.get_device()), &a);
+    return y;
+}
+
+struct Conv1dFunction : torch::autograd::Function<Conv1dFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_arg,
+                          Conv1d* cv) {
+        const Tensor bias = bias_arg.value_or(Tensor());
+        const Tensor y = conv1d_forward(*cv, x, weight, bias);
+        ctx->save_for_backward({x, weight, bias, cv->before});
+        ctx->saved_data["v"] = std::vector<int64_t>{cv->n, cv->l, cv->c, cv->width, cv->act, type_of(x), type_of(weight), type_of(bias)};
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->saved_data["v"].toIntVector();
+        const Conv1d cv{v[0], v[1], v[2], v[3], v[4]};
+        auto type = [&](int i) { return static_cast<at::ScalarType>(v[i]); };
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &before = saved[3], &dy = grads[0];
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+                   need_b = bias.defined() && ctx->needs_input_grad(2);
+        const bool native = !stands_aside(dy) && is_again(dy, dy, {cv.n, cv.l, cv.c}, type(5)) &&
+                            is_again(x, dy, {cv.n, cv.l, cv.c}, type(5)) && is_again(weight, dy, {cv.c, cv.width}, type(6)) &&
+                            (!bias.defined() || is_again(bias, dy, {cv.c}, type(7))) &&
+                            (!before.defined() || is_again(before, dy, {cv.n, cv.width - 1, cv.c}, type(5)));
+        if (!native) {
+            py::gil_scoped_acquire gil;
+            py::tuple r = py::reinterpret_borrow<py::object>(g_conv1d_gradients)(
+                dy, x, weight, to_py(bias), cv.act ? "silu" : "none", to_py(before), need_x, need_w, need_b);
+            return {from_py(r, 0), from_py(r, 1), from_py(r, 2), Tensor()};
+        }
+        RECORD_FUNCTION("spio::causal_conv1d_backward", tensors({dy, x, weight, bias}));
+        const Rows rows = rows_of(x, 8);
+        const Tensor g = whole(dy), w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias, first = whole(before);
+        const auto main = conv1d_plan(CONV1D_BWD, cv, x, weight), second = conv1d_plan(CONV1D_SUMS, cv, x, weight);
+        const Tensor dx = empty_of(x.sizes(), x.scalar_type(), x);
+        SpioConv1dArgs a = {};
+        a.slice = conv1d_slice(cv.l, cv.c, cv.n, true);
+        const int64_t slices = divup(cv.l, a.slice);
+        const Tensor partials = empty_1d(cv.n * slices * (cv.width + 1) * cv.c, at::kFloat, x);
+        const Tensor sums = empty_1d(cv.c * (cv.width + 1), at::kFloat, x);
+        a.x = ptr(rows.t), a.weight = ptr(w), a.bias = ptr(b), a.dy = ptr(g), a.before = ptr(first), a.dx = mut(dx);
+        a.partials = floats(partials), a.sums = floats(sums);
+        a.tokens = cv.l, a.channels = cv.c, a.sequences = cv.n, a.x_row = rows.row;
+        hipStream_t stream = c10::hip::getCurrentHIPStream(x.get_device());
+        launch_structure(*main, divup(cv.n * slices * (cv.c / 8), 256), stream, &a);
+        if (need_w || need_b) launch_structure(*second, divup((cv.width + 1) * cv.c, SUM_COLUMNS), stream, &a);
+        at::AutoDispatchBelowADInplaceOrView below;
+        return {need_x ? dx : Tensor(), need_w ? typed(sums.narrow(0, 0, cv.c * cv.width).view({cv.c, cv.width}), v[6]) : Tensor(),
+                need_b ? typed(sums.narrow(0, cv.c * cv.width, cv.c), v[7]) : Tensor(), Tensor()};
+    }
+};
+
+// ---- selective scan ----
+
+constexpr int64_t SCAN_MAX_STATES = 32, SCAN_LANES = 64;
+int64_t scan_tile(int64_t states) { return states <= 8 ? 8 : states <= 16 ? 6 : 4; }
+int64_t scan_chunk(int64_t tokens, int64_t channels, int64_t sequences, int64_t states) {
+    const int64_t waves = divup(channels, SCAN_LANES) * sequences, tile = scan_tile(states);
+    const int64_t chunks = std::max(int64_t(1), std::min(1024 / waves, tokens / 32));
+    return divup(divup(tokens, chunks), tile) * tile;
+}
+
+struct Scan {
+    int64_t n, l, c, s;
+    bool softplus;
+    bool keep_state = false;
+    Tensor before, after;  // states, which have no history
+};
+// What a scan's launches share: u, delta, A, B, C, D, gate, bias in this order, as the kernels read them
+struct ScanInputs {
+    SpioScanArgs a = {};
+    std::vector<Tensor> held;
+    ScanInputs(const Scan& sc, const variable_list& t) {
+        auto rows = [&](int i, const void*& p, long long& row) {
+            const Rows r = rows_of(t[i]);
+            held.push_back(r.t);
+            p = ptr(r.t), row = r.row;
+        };
+        auto parameter = [&](int i, const float*& p, bool to_16_bytes = false) {
+            held.push_back(to_float_1d(t[i]));
+            if (to_16_bytes) held.back() = aligned(held.back());
+            p = floats(held.back());
+        };
+        rows(0, a.u, a.u_row), rows(1, a.delta, a.delta_row), rows(3, a.B, a.b_row), rows(4, a.C, a.c_row), rows(6, a.gate, a.gate_row);
+        parameter(2, a.A, true), parameter(5, a.D), parameter(7, a.bias);
+        a.tokens = sc.l, a.channels = sc.c, a.sequences = sc.n, a.softplus = sc.softplus;
+        a.chunk = scan_chunk(sc.l, sc.c, sc.n, sc.s);
+    }
+};
+PlanPtr scan_plan(Kind kind, const Scan& sc, const Tensor& u) {
+    return find_plan(token_key(kind, u.get_device(), sc.s, dtype_number(u)));
+}
+Tensor scan_forward(Scan& sc, const variable_list& t, Tensor* kept) {
+    const Tensor& u = t[0];
+    ScanInputs in(sc, t);
+    const int64_t chunks = divup(sc.l, in.a.chunk), grid = sc.n * chunks * divup(sc.c, SCAN_LANES);
+    hipStream_t stream = c10::hip::getCurrentHIPStream(u.get_device());
+    const Tensor y = empty_of({sc.n, sc.l, sc.c}, u.scalar_type(), u);
+    const Tensor before = sc.before.defined() ? sc.before.contiguous() : sc.before;
+    if (sc.keep_state) sc.after = empty_of({sc.n, sc.c, sc.s}, at::kFloat, u);
+    if (kept) *kept = empty_of({sc.n, divup(sc.l, scan_tile(sc.s)), sc.s, sc.c}, at::kFloat, u);
+    Tensor ends;
+    if (chunks > 1) ends = empty_1d(sc.n * chunks * (sc.s + 1) * sc.c, at::kFloat, u);
+    in.a.before = floats(before), in.a.out = mut(y), in.a.after = floats(sc.after), in.a.ends = floats(ends);
+    in.a.kept = kept ? floats(*kept) : nullptr;
+    if (chunks > 1) launch_structure(*scan_plan(SCAN_ENDS, sc, u), grid, stream, &in.a);
+    launch_structure(*scan_plan(SCAN, sc, u), grid, stream, &in.a);
+    return y;
+}
+
+struct ScanFunction : torch::autograd::Function<ScanFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& u, const Tensor& delta, const Tensor& A, const Tensor& B,
+                          const Tensor& C, const std::optional<Tensor>& D, const std::optional<Tensor>& gate,
+                          const std::optional<Tensor>& bias, Scan* sc) {
+        const variable_list t = {u, delta, A, B, C, D.value_or(Tensor()), gate.value_or(Tensor()), bias.value_or(Tensor())};
+        Tensor kept;
+        const Tensor y = scan_forward(*sc, t, &kept);
+        variable_list saved = t;
+        saved.push_back(kept);
+        ctx->save_for_backward(saved);
+        std::vector<int64_t> v = {sc->n, sc->l, sc->c, sc->s, sc->softplus};
+        for (const Tensor& one : t) v.push_back(type_of(one));
+        ctx->saved_data["v"] = v;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->saved_data["v"].toIntVector();
+        const Scan sc{v[0], v[1], v[2], v[3], v[4] != 0};
+        const auto saved = ctx->get_saved_variables();
+        const variable_list t(saved.begin(), saved.begin() + 8);
+        const Tensor &kept = saved[8], &dy = grads[0], &u = t[0];
+        const std::vector<int64_t> tensor = {sc.n, sc.l, sc.c}, row = {sc.n, sc.l, sc.s}, rate = {sc.c, sc.s}, channel = {sc.c};
+        const std::vector<int64_t>* shapes[8] = {&tensor, &tensor, &rate, &row, &row, &channel, &tensor, &channel};
+        bool native = !stands_aside(dy) && is_again(dy, dy, tensor, static_cast<at::ScalarType>(v[5])) &&
+                      is_again(kept, dy, {sc.n, divup(sc.l, scan_tile(sc.s)), sc.s, sc.c}, at::kFloat);
+        std::vector<bool> needs(8);
+        int edge = 0;  // absent tensors have none
+        for (int i = 0; i < 8; ++i) {
+            if (!t[i].defined()) continue;
+            needs[i] = ctx->needs_input_grad(edge++);
+            native = native && is_again(t[i], dy, *shapes[i], static_cast<at::ScalarType>(v[5 + i]));
+        }
+        if (!native) {
+            py::gil_scoped_acquire gil;
+            py::tuple r = py::reinterpret_borrow<py::object>(g_scan_gradients)(
+                dy, u, t[1], t[2], t[3], t[4], to_py(t[5]), to_py(t[6]), to_py(t[7]), sc.softplus, kept, needs);
+            variable_list out;
+            for (int i = 0; i < 8; ++i) out.push_back(from_py(r, i));
+            out.emplace_back();
+            return out;
+        }
+        RECORD_FUNCTION("spio::selective_scan_backward", tensors({dy, u, t[1], t[2], t[3], t[4], t[5], t[6], t[7]}));
+        ScanInputs in(sc, t);
+        const int64_t chunks = divup(sc.l, in.a.chunk), blocks = divup(sc.c, SCAN_LANES), grid = sc.n * chunks * blocks;
+        hipStream_t stream = c10::hip::getCurrentHIPStream(u.get_device());
+        const Tensor g = dy.contiguous(), k = kept.contiguous();
+        const Tensor du = empty_of(tensor, u.scalar_type(), u), ddelta = empty_of(tensor, u.scalar_type(), u);
+        const Tensor dgate = t[6].defined() ? empty_of(tensor, u.scalar_type(), u) : Tensor();
+        const Tensor dB = empty_of(row, u.scalar_type(), u), dC = empty_of(row, u.scalar_type(), u);
+        const Tensor sums = empty_1d(sc.c * (sc.s + 2), at::kFloat, u);
+        const Tensor token_sums = empty_1d(sc.n * sc.l * blocks * 2 * sc.s, at::kFloat, u);
+        const Tensor channel_sums = empty_1d(sc.n * chunks * (sc.s + 2) * sc.c, at::kFloat, u);
+        Tensor ends;
+        if (chunks > 1) ends = empty_1d(sc.n * chunks * (sc.s + 1) * sc.c, at::kFloat, u);
+        in.a.dout = ptr(g), in.a.kept = floats(k), in.a.ends = floats(ends), in.a.du = mut(du), in.a.ddelta = mut(ddelta);
+        in.a.dgate = mut(dgate), in.a.dB = mut(dB), in.a.dC = mut(dC), in.a.sums = floats(sums);
+        in.a.token_sums = floats(token_sums), in.a.channel_sums = floats(channel_sums);
+        if (chunks > 1) launch_structure(*scan_plan(SCAN_ENDS_BWD, sc, u), grid, stream, &in.a);
+        launch_structure(*scan_plan(SCAN_BWD, sc, u), grid, stream, &in.a);
+        launch_structure(*scan_plan(SCAN_SUMS, sc, u), divup(sc.n * sc.l * 2 * sc.s, 256) + divup((sc.s + 2) * sc.c, SUM_COLUMNS),
+                         stream, &in.a);
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto sum = [&](int i, int64_t from, int64_t count) { return typed(sums.narrow(0, from, count), v[5 + i]); };
+        return {needs[0] ? du : Tensor(), needs[1] ? ddelta : Tensor(), needs[2] ? sum(2, 0, sc.c * sc.s).view(rate) : Tensor(),
+                needs[3] ? dB : Tensor(), needs[4] ? dC : Tensor(), needs[5] ? sum(5, sc.c * sc.s, sc.c) : Tensor(),
+                needs[6] ? dgate : Tensor(), needs[7] ? sum(7, sc.c * (sc.s + 1), sc.c) : Tensor(), Tensor()};
+    }
+};
+
+// ---- rotary positions and norms of heads ----
+
+constexpr int64_t ROTARY_MAX_HEAD = 256, ROTARY_THREADS = 256, ROTARY_SUMMED = 512;
+int64_t rotary_lanes(int64_t head) {
+    int64_t lanes = 1;
+    while (lanes * 16 < head) lanes *= 2;
+    return lanes;
+}
+int64_t rotary_parts(int64_t tokens, int64_t heads, int64_t head) {
+    const int64_t waves = divup(tokens * rotary_lanes(head), 64);
+    return std::max(int64_t(1), std::min(divup(heads, 2), divup(2048, waves)));
+}
+int64_t rotary_grid(int64_t tokens, int64_t parts, int64_t head, bool summed) {
+    const int64_t grid = divup(tokens * parts * rotary_lanes(head), ROTARY_THREADS);
+    return summed ? std::min(grid, ROTARY_SUMMED) : grid;
+}
+
+struct Rotary {
+    int64_t n, l, q_heads, k_heads, d;
+    bool interleaved;
+    double eps, scale;
+    Tensor positions, frequencies;  // have no gradients
+    int64_t tokens() const { return n * l; }
+    int64_t parts() const { return rotary_parts(tokens(), std::max(q_heads, k_heads), d); }
+    std::vector<int64_t> shape(int64_t heads) const { return {n, l, heads, d}; }
+    SpioRotaryArgs args() const {
+        SpioRotaryArgs a = {};
+        a.positions = ptr(positions), a.frequencies = static_cast<const double*>(ptr(frequencies));
+        a.tokens = tokens(), a.q_heads = q_heads, a.k_heads = k_heads, a.parts = parts(), a.pairs = frequencies.numel();
+        a.position_tokens = positions.numel(), a.wide_positions = positions.scalar_type() == at::kLong;
+        a.eps = eps, a.scale = scale;
+        return a;
+    }
+};
+PlanPtr rotary_plan(Kind kind, const Rotary& r, const Tensor& q, bool norm) {
+    return find_plan(token_key(kind, q.get_device(), r.d, dtype_number(q), norm, r.interleaved));
+}
+// Rows (tokens) and heads that are equally far apart and start on 16 bytes, or a copy without gaps
+struct Heads {
+    Tensor t;
+    int64_t row, head;
+};
+Heads heads_of(const Tensor& t) {
+    const int64_t n = t.size(0), l = t.size(1), h = t.size(2), d = t.size(3), size = t.element_size();
+    const int64_t row = l != 1 ? t.stride(1) : n != 1 ? t.stride(0) : h * d, head = h != 1 ? t.stride(2) : d;
+    const bool even = n == 1 || l == 1 || t.stride(0) == l * t.stride(1);
+    if (even && t.stride(3) == 1 && on_16_bytes(t) && row * size % 16 == 0 && head * size % 16 == 0) return {t, row, head};
+    return {t.clone(at::MemoryFormat::Contiguous), h * d, d};
+}
+variable_list rotary_forward(const Rotary& r, const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight) {
+    const Heads qh = heads_of(q), kh = heads_of(k);
+    const Tensor wq = to_float_1d(q_weight), wk = to_float_1d(k_weight);
+    const Tensor qo = empty_of(r.shape(r.q_heads), q.scalar_type(), q), ko = empty_of(r.shape(r.k_heads), k.scalar_type(), k);
+    SpioRotaryArgs a = r.args();
+    a.q = ptr(qh.t), a.q_row = qh.row, a.q_head = qh.head, a.k = ptr(kh.t), a.k_row = kh.row, a.k_head = kh.head;
+    a.q_weight = floats(wq), a.k_weight = floats(wk), a.q_out = mut(qo), a.k_out = mut(ko);
+    launch_structure(*rotary_plan(ROTARY, r, q, wq.defined()), rotary_grid(r.tokens(), a.parts, r.d, false),
+                     c10::hip::getCurrentHIPStream(q.get_device()), &a);
+    return {qo, ko};
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const std::optional<Tensor>& q_weight,
+                                 const std::optional<Tensor>& k_weight, const Rotary& r) {
+        const Tensor wq = q_weight.value_or(Tensor()), wk = k_weight.value_or(Tensor());
+        const bool norm = wq.defined();
+        variable_list out = rotary_forward(r, q, k, wq, wk);
+        ctx->set_materialize_grads(false);
+        // without a norm the gradients need no inputs
+        ctx->save_for_backward({norm ? q : Tensor(), norm ? k : Tensor(), wq, wk, r.positions, r.frequencies});
+        ctx->saved_data["v"] = std::vector<int64_t>{r.n, r.l, r.q_heads, r.k_heads, r.d, r.interleaved, type_of(q), type_of(wq),
+                                                    type_of(wk), type_of(r.positions), q.get_device()};
+        ctx->saved_data["eps"] = r.eps;
+        ctx->saved_data["scale"] = r.scale;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        if (!grads[0].defined() && !grads[1].defined()) return variable_list(5);
+        const auto v = ctx->saved_data["v"].toIntVector();
+        const auto saved = ctx->get_saved_variables();
+        const Rotary r{v[0], v[1], v[2], v[3], v[4], v[5] != 0, ctx->saved_data["eps"].toDouble(), ctx->saved_data["scale"].toDouble(),
+                       saved[4], saved[5]};
+        auto type = [&](int i) { return static_cast<at::ScalarType>(v[i]); };
+        const Tensor &q = saved[0], &k = saved[1], &wq = saved[2], &wk = saved[3];
+        const bool norm = wq.defined();
+        const auto options = at::TensorOptions().dtype(type(6)).device(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(v[10])));
+        const Tensor gq = grads[0].defined() ? grads[0] : at::zeros(r.shape(r.q_heads), options);
+        const Tensor gk = grads[1].defined() ? grads[1] : at::zeros(r.shape(r.k_heads), options);
+        const bool native =
+            !stands_aside(gq) && !stands_aside(gk) && is_again(gq, gq, r.shape(r.q_heads), type(6)) &&
+            is_again(gk, gq, r.shape(r.k_heads), type(6)) &&
+            (!norm || (is_again(q, gq, r.shape(r.q_heads), type(6)) && is_again(k, gq, r.shape(r.k_heads), type(6)) &&
+                       is_again(wq, gq, {r.d}, type(7)) && is_again(wk, gq, {r.d}, type(8)))) &&
+            is_again(r.positions, gq, r.positions.sizes(), type(9)) && r.positions.is_contiguous() &&
+            (r.positions.numel() == r.l || r.positions.numel() == r.tokens()) &&
+            is_again(r.frequencies, gq, r.frequencies.sizes(), at::kDouble) && r.frequencies.is_contiguous();
+        const bool needs[4] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), norm && ctx->needs_input_grad(2),
+                               norm && ctx->needs_input_grad(3)};
+        if (!native) {
+            py::gil_scoped_acquire gil;
+            py::tuple out = py::reinterpret_borrow<py::object>(g_rotary_gradients)(
+                gq, gk, to_py(q), to_py(k), to_py(wq), to_py(wk), r.positions, r.frequencies, r.eps, r.interleaved, r.scale,
+                std::vector<bool>(needs, needs + 4));
+            return {from_py(out, 0), from_py(out, 1), from_py(out, 2), from_py(out, 3), Tensor()};
+        }
+        RECORD_FUNCTION("spio::head_norm_rotary_backward", tensors({gq, gk, q, k, wq, wk}));
+        const Tensor gqc = whole(gq), gkc = whole(gk), wqf = to_float_1d(wq), wkf = to_float_1d(wk);
+        const Tensor dq = empty_of(gq.sizes(), type(6), gq), dk = empty_of(gk.sizes(), type(6), gk);
+        SpioRotaryArgs a = r.args();
+        const int64_t grid = rotary_grid(r.tokens(), a.parts, r.d, norm);
+        Heads qh, kh;
+        Tensor partials, sums;
+        if (norm) {
+            qh = heads_of(q), kh = heads_of(k);
+            a.q = ptr(qh.t), a.q_row = qh.row, a.q_head = qh.head, a.k = ptr(kh.t), a.k_row = kh.row, a.k_head = kh.head;
+            partials = empty_1d(grid * 2 * r.d, at::kFloat, gq);
+            sums = empty_of({2, r.d}, at::kFloat, gq);
+        }
+        a.dq = ptr(gqc), a.dk = ptr(gkc), a.q_weight = floats(wqf), a.k_weight = floats(wkf), a.q_out = mut(dq), a.k_out = mut(dk);
+        a.partials = floats(partials), a.sums = floats(sums);
+        hipStream_t stream = c10::hip::getCurrentHIPStream(gq.get_device());
+        launch_structure(*rotary_plan(ROTARY_BWD, r, gq, norm), grid, stream, &a);
+        if (needs[2] || needs[3]) {
+            a.parts = grid;
+            launch_structure(*rotary_plan(ROTARY_SUMS, r, gq, norm), divup(2 * r.d, SUM_COLUMNS), stream, &a);
+        }
+        at::AutoDispatchBelowADInplaceOrView below;
+        return {needs[0] ? dq : Tensor(), needs[1] ? dk : Tensor(), needs[2] ? typed(sums.select(0, 0), v[7]) : Tensor(),
+                needs[3] ? typed(sums.select(0, 1), v[8]) : Tensor(), Tensor()};
+    }
+};
+
 // ---- Python boundary ------------------------------------------------------------------------
 
 // Arguments of a Python call by position or keyword; false if they do not fit the names.
@@ -1091,7 +1505,248 @@ PyObject* unpack_8bit(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObje
     END_HANDLE_TH_ERRORS
 }
 
+// What the functions below are called with: positional arguments, by the functions of spio_amd/functional, in their order.
+bool optional_tensor(PyObject* o, Tensor* t) { return o == Py_None || tensor_arg(o, t); }
+bool number_arg(PyObject* o, double* v) {
+    if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+    *v = PyFloat_AsDouble(o);
+    if (*v == -1.0 && PyErr_Occurred()) {  // an integer that no float64 is near
+        PyErr_Clear();
+        return false;
+    }
+    return true;
+}
+bool bool_arg(PyObject* o, bool* v) {
+    *v = o == Py_True;
+    return PyBool_Check(o);
+}
+bool ready(Py_ssize_t nargs, Py_ssize_t expected, PyObject* kwnames) {
+    return g_bypass.load(std::memory_order_relaxed) == 0 && eager_mode() && nargs == expected && !kwnames;
+}
+// A plain tensor of that shape, on the device of `like`; with `typed` of its type, too, else of one of the three
+bool fits(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, bool typed) {
+    return is_plain(t) && t.sizes() == sizes && t.device() == like.device() &&
+           (typed ? t.scalar_type() == like.scalar_type() : dtype_number(t) >= 0);
+}
+bool absent_or_fits(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, bool typed) {
+    return !t.defined() || fits(t, like, sizes, typed);
+}
+bool state_fits(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, at::ScalarType dtype) {
+    return !t.defined() || (is_plain(t) && t.sizes() == sizes && t.device() == like.device() && t.scalar_type() == dtype);
+}
+PyObject* with_state(const Tensor& y, const Tensor& state) {
+    return state.defined() ? py::make_tuple(y, state).release().ptr() : THPVariable_Wrap(y);
+}
+constexpr int64_t CONV1D_MIN_WIDTH = 2, CONV1D_MAX_WIDTH = 8;
+
+// Whether weight and bias are what the convolution's kernels read; `act`: its number
+bool conv1d_fits(PyObject* activation, const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t* act) {
+    *act = activation_number(activation);
+    const int64_t c = x.size(-1);
+    return (*act == 0 || *act == 2) && dtype_number(x) >= 0 && c > 0 && c % 8 == 0 && is_plain(weight) && weight.dim() == 2 &&
+           weight.size(1) >= CONV1D_MIN_WIDTH && weight.size(1) <= CONV1D_MAX_WIDTH &&
+           fits(weight, x, {c, weight.size(1)}, false) && absent_or_fits(bias, x, {c}, false) &&
+           (!bias.defined() || bias.scalar_type() == weight.scalar_type());
+}
+
+// causal_conv1d(inputs, weight, bias, activation, initial_state, return_state)
+PyObject* causal_conv1d(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    if (!ready(nargs, 6, kwnames)) return not_implemented();
+    Tensor x, weight, bias;
+    Conv1d cv{};
+    if (!tensor_arg(args[0], &x) || !tensor_arg(args[1], &weight) || !optional_tensor(args[2], &bias) ||
+        !optional_tensor(args[4], &cv.before) || !bool_arg(args[5], &cv.keep_state))
+        return not_implemented();
+    if (!is_plain(x) || x.dim() != 3 || x.numel() == 0 || !conv1d_fits(args[3], x, weight, bias, &cv.act)) return not_implemented();
+    cv.n = x.size(0), cv.l = x.size(1), cv.c = x.size(2), cv.width = weight.size(1);
+    if (!state_fits(cv.before, x, {cv.n, cv.width - 1, cv.c}, x.scalar_type())) return not_implemented();
+    const bool grad = at::GradMode::is_enabled();
+    if (grad && wants_grad(cv.before)) return not_implemented();
+    Tensor y;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(x.device());
+        RECORD_FUNCTION("spio::causal_conv1d_forward", tensors({x, weight, bias, cv.before}));
+        c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
+        if (grad && (wants_grad(x) || wants_grad(weight) || wants_grad(bias))) {
+            y = Conv1dFunction::apply(x, weight, optional(bias), &cv);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            y = conv1d_forward(cv, x, weight, bias);
+        }
+    }
+    return with_state(y, cv.after);
+    END_HANDLE_TH_ERRORS
+}
+
+// causal_conv1d_step(inputs, state, weight, bias, activation, out_state)
+PyObject* causal_conv1d_step(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    if (!ready(nargs, 6, kwnames)) return not_implemented();
+    Tensor x, weight, bias, after;
+    Conv1d cv{};
+    if (!tensor_arg(args[0], &x) || !tensor_arg(args[1], &cv.before) || !tensor_arg(args[2], &weight) ||
+        !optional_tensor(args[3], &bias) || !tensor_arg(args[5], &after))
+        return not_implemented();
+    if (!is_plain(x) || x.dim() != 2 || x.numel() == 0 || !conv1d_fits(args[4], x, weight, bias, &cv.act)) return not_implemented();
+    cv.n = x.size(0), cv.l = 1, cv.c = x.size(1), cv.width = weight.size(1);
+    if (!state_fits(cv.before, x, {cv.n, cv.width - 1, cv.c}, x.scalar_type()) || !writable_state(cv.before, after, {x}))
+        return not_implemented();
+    Tensor y;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(x.device());
+        RECORD_FUNCTION("spio::causal_conv1d_step", tensors({x, cv.before, weight, bias}));
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Rows rows = rows_of(x, 8);
+        const Tensor w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
+        const auto plan = conv1d_plan(CONV1D_STEP, cv, x, weight);
+        y = empty_of({cv.n, cv.c}, x.scalar_type(), x);
+        SpioConv1dArgs a = {};
+        a.x = ptr(rows.t), a.weight = ptr(w), a.bias = ptr(b), a.before = ptr(cv.before), a.out = mut(y), a.after = mut(after);
+        a.tokens = a.slice = 1, a.channels = cv.c, a.sequences = cv.n, a.x_row = rows.row;
+        launch_structure(*plan, divup(cv.n * (cv.c / 8), 64), c10::hip::getCurrentHIPStream(x.get_device()), &a);
+        after.unsafeGetTensorImpl()->bump_version();
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// Shapes and types of a scan's tensors: u, delta, A, B, C, D, gate, bias
+bool scan_fits(const variable_list& t) {
+    const Tensor &u = t[0], &A = t[2];
+    if (dtype_number(u) < 0 || u.numel() == 0 || !is_plain(A) || A.dim() != 2 || A.size(1) < 1 || A.size(1) > SCAN_MAX_STATES)
+        return false;
+    std::vector<int64_t> row = u.sizes().vec();
+    const int64_t c = row.back();
+    row.back() = A.size(1);
+    return fits(t[1], u, u.sizes(), true) && fits(A, u, {c, A.size(1)}, false) && fits(t[3], u, row, true) &&
+           fits(t[4], u, row, true) && absent_or_fits(t[5], u, {c}, false) && absent_or_fits(t[6], u, u.sizes(), true) &&
+           absent_or_fits(t[7], u, {c}, false);
+}
+bool scan_tensors(PyObject* const* args, const int (&at)[8], variable_list* t) {
+    t->resize(8);
+    for (int i = 0; i < 8; ++i)
+        if (!(i < 5 ? tensor_arg(args[at[i]], &(*t)[i]) : optional_tensor(args[at[i]], &(*t)[i]))) return false;
+    return is_plain((*t)[0]);
+}
+
+// selective_scan(inputs, delta, A, B, C, D, gate, delta_bias, delta_softplus, initial_state, return_state)
+PyObject* selective_scan(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    if (!ready(nargs, 11, kwnames)) return not_implemented();
+    variable_list t;
+    Scan sc{};
+    if (!scan_tensors(args, {0, 1, 2, 3, 4, 5, 6, 7}, &t) || !bool_arg(args[8], &sc.softplus) ||
+        !optional_tensor(args[9], &sc.before) || !bool_arg(args[10], &sc.keep_state))
+        return not_implemented();
+    const Tensor& u = t[0];
+    if (u.dim() != 3 || u.size(1) >= int64_t(1) << 30 || !scan_fits(t)) return not_implemented();
+    sc.n = u.size(0), sc.l = u.size(1), sc.c = u.size(2), sc.s = t[2].size(1);
+    if (!state_fits(sc.before, u, {sc.n, sc.c, sc.s}, at::kFloat)) return not_implemented();
+    const bool grad = at::GradMode::is_enabled();
+    if (grad && wants_grad(sc.before)) return not_implemented();
+    Tensor y;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(u.device());
+        RECORD_FUNCTION("spio::selective_scan_forward", tensors({u, t[1], t[2], t[3], t[4], t[5], t[6], t[7], sc.before}));
+        c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
+        if (grad && std::any_of(t.begin(), t.end(), wants_grad)) {
+            y = ScanFunction::apply(u, t[1], t[2], t[3], t[4], optional(t[5]), optional(t[6]), optional(t[7]), &sc);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            y = scan_forward(sc, t, nullptr);
+        }
+    }
+    return with_state(y, sc.after);
+    END_HANDLE_TH_ERRORS
+}
+
+// selective_scan_step(inputs, state, delta, A, B, C, D, gate, delta_bias, delta_softplus, out_state)
+PyObject* selective_scan_step(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    if (!ready(nargs, 11, kwnames)) return not_implemented();
+    variable_list t;
+    Tensor after;
+    Scan sc{};
+    if (!scan_tensors(args, {0, 2, 3, 4, 5, 6, 7, 8}, &t) || !tensor_arg(args[1], &sc.before) || !bool_arg(args[9], &sc.softplus) ||
+        !tensor_arg(args[10], &after))
+        return not_implemented();
+    const Tensor& u = t[0];
+    if (u.dim() != 2 || !scan_fits(t)) return not_implemented();
+    sc.n = u.size(0), sc.l = 1, sc.c = u.size(1), sc.s = t[2].size(1);
+    if (!state_fits(sc.before, u, {sc.n, sc.c, sc.s}, at::kFloat) || !writable_state(sc.before, after, {u, t[1], t[3], t[4], t[6]}))
+        return not_implemented();
+    Tensor y;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(u.device());
+        RECORD_FUNCTION("spio::selective_scan_step", tensors({u, sc.before, t[1], t[2], t[3], t[4], t[5], t[6], t[7]}));
+        at::AutoDispatchBelowADInplaceOrView below;
+        ScanInputs in(sc, t);
+        const auto plan = scan_plan(SCAN_STEP, sc, u);
+        y = empty_of({sc.n, sc.c}, u.scalar_type(), u);
+        in.a.before = floats(sc.before), in.a.out = mut(y), in.a.after = floats(after);
+        const int64_t lanes = sc.s <= 4 ? 1 : sc.s <= 8 ? 2 : sc.s <= 16 ? 4 : 8;
+        launch_structure(*plan, divup(sc.n * sc.c * lanes, 256), c10::hip::getCurrentHIPStream(u.get_device()), &in.a);
+        after.unsafeGetTensorImpl()->bump_version();
+    }
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// head_norm_rotary(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, scale); without weights no norm
+PyObject* head_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+    HANDLE_TH_ERRORS
+    if (!ready(nargs, 9, kwnames)) return not_implemented();
+    Tensor q, k, wq, wk;
+    Rotary r{};
+    if (!tensor_arg(args[0], &q) || !tensor_arg(args[1], &k) || !optional_tensor(args[2], &wq) || !optional_tensor(args[3], &wk) ||
+        !tensor_arg(args[4], &r.positions) || !tensor_arg(args[5], &r.frequencies) || !number_arg(args[6], &r.eps) ||
+        !bool_arg(args[7], &r.interleaved) || !number_arg(args[8], &r.scale))
+        return not_implemented();
+    if (!is_plain(q) || q.dim() != 4 || dtype_number(q) < 0 || !is_plain(k) || k.dim() != 4) return not_implemented();
+    r.n = q.size(0), r.l = q.size(1), r.q_heads = q.size(2), r.k_heads = k.size(2), r.d = q.size(3);
+    const int64_t pairs = is_plain(r.frequencies) && r.frequencies.dim() == 1 ? r.frequencies.size(0) : 0;
+    if (q.numel() == 0 || k.numel() == 0 || !fits(k, q, r.shape(r.k_heads), true) || r.d % 8 || r.d > ROTARY_MAX_HEAD ||
+        wq.defined() != wk.defined() || !absent_or_fits(wq, q, {r.d}, false) || !absent_or_fits(wk, q, {r.d}, false) ||
+        !(r.eps > 0) || r.eps > std::numeric_limits<double>::max() || !std::isfinite(r.scale) || pairs < 1 || 2 * pairs > r.d ||
+        (!r.interleaved && pairs % 8) || r.frequencies.scalar_type() != at::kDouble || r.frequencies.device() != q.device() ||
+        !is_plain(r.positions) || (r.positions.scalar_type() != at::kLong && r.positions.scalar_type() != at::kInt) ||
+        r.positions.device() != q.device() ||
+        !(r.positions.sizes() == at::IntArrayRef({r.l}) || r.positions.sizes() == at::IntArrayRef({r.n, r.l})))
+        return not_implemented();
+    variable_list out;
+    {
+        py::gil_scoped_release no_gil;
+        c10::DeviceGuard device(q.device());
+        RECORD_FUNCTION("spio::head_norm_rotary_forward", tensors({q, k, wq, wk, r.positions, r.frequencies}));
+        c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);
+        r.positions = r.positions.contiguous(), r.frequencies = r.frequencies.contiguous();
+        if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(wq) || wants_grad(wk))) {
+            out = RotaryFunction::apply(q, k, optional(wq), optional(wk), r);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            out = rotary_forward(r, q, k, wq, wk);
+        }
+    }
+    return py::make_tuple(out[0], out[1]).release().ptr();
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef g_methods[] = {
+    {"causal_conv1d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(causal_conv1d)),
+     METH_FASTCALL | METH_KEYWORDS, "causal_conv1d on plain GPU tensors, else NotImplemented"},
+    {"causal_conv1d_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(causal_conv1d_step)),
+     METH_FASTCALL | METH_KEYWORDS, "causal_conv1d_step on plain GPU tensors, else NotImplemented"},
+    {"selective_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(selective_scan)),
+     METH_FASTCALL | METH_KEYWORDS, "selective_scan on plain GPU tensors, else NotImplemented"},
+    {"selective_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(selective_scan_step)),
+     METH_FASTCALL | METH_KEYWORDS, "selective_scan_step on plain GPU tensors, else NotImplemented"},
+    {"head_norm_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(head_norm_rotary)),
+     METH_FASTCALL | METH_KEYWORDS, "head_norm_rotary on plain GPU tensors, else NotImplemented"},
     {"group_norm_2d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_norm_2d)),
      METH_FASTCALL | METH_KEYWORDS, "group_norm_2d on plain GPU tensors, else NotImplemented"},
     {"activation_8bit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(activation_8bit)),
@@ -1131,6 +1786,17 @@ PYBIND11_MODULE(_native, m) {
         g_activation_gradient = activation_gradient.release().ptr();
         g_conv_kept_gradients = conv_gradients.release().ptr();
     });
+    m.def("configure_tokens", [](py::object conv1d_gradients, py::object scan_gradients, py::object rotary_gradients) {
+        g_conv1d_gradients = conv1d_gradients.release().ptr();
+        g_scan_gradients = scan_gradients.release().ptr();
+        g_rotary_gradients = rotary_gradients.release().ptr();
+    });
+    // how work over sequences of tokens is cut, which kernels/*_kernel.py compute as well
+    m.def("conv1d_slice", &conv1d_slice);
+    m.def("scan_chunk", &scan_chunk);
+    m.def("scan_tile", &scan_tile);
+    m.def("rotary_parts", &rotary_parts);
+    m.def("rotary_grid", &rotary_grid);
     m.def("bypass", [](int64_t change) { g_bypass.fetch_add(change); });
     m.def("forget", [] {
         g_generation.fetch_add(1);

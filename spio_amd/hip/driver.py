@@ -333,6 +333,16 @@ class Function:
         if rc:
             _check(rc)
 
+    def launch_structure(self, grid, block, array, shared_mem_bytes: int = 0, stream: int = 0):
+        """Asynchronous launch of a kernel whose one parameter is a structure, the ctypes array `array`."""
+        params = (_vp * 1)(ctypes.addressof(array))
+        rc = _lib.spio_hip_launch(
+            self._handle, grid[0], grid[1], grid[2], block[0], block[1], block[2],
+            shared_mem_bytes, stream or None, params, 1,
+        )  # fmt: skip
+        if rc:
+            _check(rc)
+
     def launch_scratch(self, grid, block, args, scratch_param: int, scratch_bytes: int,
                        shared_mem_bytes: int = 0, stream: int = 0):  # fmt: skip
         """Launch with the library's static device workspace as argument `scratch_param`.

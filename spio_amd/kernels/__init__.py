@@ -41,3 +41,28 @@ from .activation_8bit_kernel import (
     Activation8bitParams,
     Activation8bitConfig,
 )
+from .selective_scan_kernel import (
+    selective_scan_ends_kernel_factory,
+    selective_scan_kernel_factory,
+    selective_scan_ends_bwd_kernel_factory,
+    selective_scan_bwd_kernel_factory,
+    selective_scan_sums_kernel_factory,
+    selective_scan_step_kernel_factory,
+    SelectiveScanParams,
+    SelectiveScanConfig,
+)
+from .causal_conv1d_kernel import (
+    causal_conv1d_kernel_factory,
+    causal_conv1d_bwd_kernel_factory,
+    causal_conv1d_sums_kernel_factory,
+    causal_conv1d_step_kernel_factory,
+    CausalConv1dParams,
+    CausalConv1dConfig,
+)
+from .head_norm_rotary_kernel import (
+    head_norm_rotary_kernel_factory,
+    head_norm_rotary_bwd_kernel_factory,
+    head_norm_rotary_sums_kernel_factory,
+    HeadNormRotaryParams,
+    HeadNormRotaryConfig,
+)

@@ -54,6 +54,8 @@ class KernelSpec:
     overwrites_output: bool = False
     # Element-wise kernels: the values a workgroup takes; their number is the last argument, and the grid follows from it
     values_per_workgroup: int = 0
+    # Kernels over sequences of tokens: one structure of arguments (token_args.py), launched on a grid that comes with it
+    takes_structure: bool = False
 
     def grid(self, args):
         """Workgroups of a launch with these arguments."""
@@ -227,6 +229,26 @@ class Kernel:
                 self.function.launch(lp.grid, lp.block, main_args, lp.shared_mem_bytes, stream)
                 ep = spec.epilogue_launch_params
                 self.epilogue_function.launch(ep.grid, ep.block, epilogue_args, ep.shared_mem_bytes, stream)
+            if timer is not None:
+                stop.record()
+        except Exception as e:
+            raise ValueError(f"Error in kernel {self}") from e
+
+    def launch_structure(self, grid: int, arguments):
+        """Asynchronous launch of a kernel that takes a structure (token_args.Arguments), in `grid` workgroups on torch's
+        current stream of its tensors' device."""
+        try:
+            device = self._prepare(arguments.tensors)
+            lp = self.kernel_spec.launch_params
+            assert 0 < grid and grid * lp.block[0] < 1 << 32, "more workgroups than a launch can have"
+            stream = torch.cuda.current_stream(device).cuda_stream
+            timer = LaunchTimer.active
+            if timer is not None:
+                start = torch.cuda.Event(enable_timing=True)
+                stop = torch.cuda.Event(enable_timing=True)
+                timer.events.setdefault(self, []).append((start, stop))
+                start.record()
+            self.function.launch_structure((grid, 1, 1), lp.block, arguments.array, lp.shared_mem_bytes, stream)
             if timer is not None:
                 stop.record()
         except Exception as e:

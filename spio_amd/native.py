@@ -134,6 +134,9 @@ def _make_plan(values):
                                            has_bias=bool(vectors & 1), kept=bool(kept))  # fmt: skip
         factory = kernels.group_norm_2d_kernel_factory if kind == 6 else kernels.group_norm_2d_bwd_kernel_factory
         kernel = factory.get_kernel(params, device)
+    elif kind >= 12:
+        factory, params = _token_kernel(kind, values[2:6])
+        kernel = factory.get_kernel(params, device)
     else:
         dtype, activation, kept = values[2:5]
         factory = (kernels.activation_8bit_kernel_factory, kernels.activation_8bit_bwd_kernel_factory,
@@ -151,6 +154,26 @@ def _make_plan(values):
     if kernel.epilogue_half_function is not None:
         stages.append(_stage(kernel.epilogue_half_function, spec.epilogue_half_launch_params))
     return stages, spec.workspace_bytes, spec.overwrites_output, kernel
+
+
+def _token_kernel(kind, numbers):
+    """Factory and parameters of a kernel over sequences of tokens."""
+    from . import kernels
+
+    if kind < 16:
+        width, dtype, weight_dtype, activation = numbers
+        factories = (kernels.causal_conv1d_kernel_factory, kernels.causal_conv1d_bwd_kernel_factory,
+                     kernels.causal_conv1d_sums_kernel_factory, kernels.causal_conv1d_step_kernel_factory)  # fmt: skip
+        return factories[kind - 12], kernels.CausalConv1dParams(width, dtype, weight_dtype, activation)
+    if kind < 22:
+        factories = (kernels.selective_scan_ends_kernel_factory, kernels.selective_scan_kernel_factory,
+                     kernels.selective_scan_ends_bwd_kernel_factory, kernels.selective_scan_bwd_kernel_factory,
+                     kernels.selective_scan_sums_kernel_factory, kernels.selective_scan_step_kernel_factory)  # fmt: skip
+        return factories[kind - 16], kernels.SelectiveScanParams(*numbers[:2])
+    factories = (kernels.head_norm_rotary_kernel_factory, kernels.head_norm_rotary_bwd_kernel_factory,
+                 kernels.head_norm_rotary_sums_kernel_factory)  # fmt: skip
+    head, dtype, norm, interleaved = numbers
+    return factories[kind - 22], kernels.HeadNormRotaryParams(head, dtype, bool(norm), bool(interleaved))
 
 
 class NativeOp(CustomOpDef):
@@ -183,6 +206,12 @@ def configure_kept(group_norm_gradients, activation_gradient, conv_gradients):
     aside."""
     if _native is not None:
         _native.configure_kept(group_norm_gradients, activation_gradient, conv_gradients)
+
+
+def configure_tokens(conv1d_gradients, scan_gradients, rotary_gradients):
+    """What the backward passes of causal_conv1d, selective_scan and head_norm_rotary hand over to where they stand aside."""
+    if _native is not None:
+        _native.configure_tokens(conv1d_gradients, scan_gradients, rotary_gradients)
 
 
 def configure(backward_op, norm_gradients):
