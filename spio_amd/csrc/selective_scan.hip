@@ -12,11 +12,12 @@
 //   dB = sum_channels g dl u,   dC = sum_channels dy h,   dD = sum dy u,   ddelta = ddl softplus' = dbias's terms
 //
 //   SPIO_MODE 0  ends      what a chunk of tokens adds to the states, and the sum of its dl
-//   SPIO_MODE 1  out       outputs, from the states before a chunk: those of the ends before it joined
+//   SPIO_MODE 1  out       outputs, from the states before a chunk
 //   SPIO_MODE 2  ends back what a chunk adds to exp(dl A) g at its first token
 //   SPIO_MODE 3  back      gradients; sums over channels and over tokens as partial sums
 //   SPIO_MODE 4  sums      the partial sums added up
 //   SPIO_MODE 5  step      one token of every sequence: states read and written once
+//   SPIO_MODE 6  join      the ends of chunks made the states before them; 7: the same from the last chunk to the first
 //
 // Modes 0 to 3: a lane is a channel and holds its N states, a wave is 64 channels and a chunk of a sequence.  So nothing
 // crosses lanes but the sums over channels of dB and dC, and B and C are the same for a wave: it converts tiles of T
@@ -29,16 +30,20 @@
 #include "spio_tokens.h"
 
 #ifndef SPIO_MODE
-#error "SPIO_MODE, SPIO_STATES are required"
+#error "SPIO_MODE, SPIO_STATES, SPIO_T, SPIO_HELD, SPIO_WAVES, SPIO_GATE, SPIO_SOFTPLUS, SPIO_KEEP are required"
 #endif
 
 namespace {
 
 constexpr int N = SPIO_STATES;
 constexpr int T = SPIO_T;                       // tokens of a tile, and between kept states
-constexpr int NP = (N + 3) / 4 * 4;        // states of a row in LDS
+constexpr int NP = (N + 3) / 4 * 4;        // states of a row in LDS, zeros behind the last one
 constexpr int M = 2 * N;                   // a token's B and C
-constexpr int STAGED = (T * M + 63) / 64;  // of those of a tile, a lane's
+constexpr int STAGED = (T * N + 63) / 64;  // of a tile's B, a lane's, and of its C
+constexpr bool GATE = SPIO_GATE, SOFTPLUS = SPIO_SOFTPLUS, KEEP = SPIO_KEEP;
+constexpr int STATES_AT = T > 2 ? T - 3 : 0;  // token behind which there are registers for the states of the next tile
+constexpr int HELD = SPIO_HELD;            // last tokens of a tile whose decays the backward pass holds, the others are taken again
+
 typedef SpioScanArgs Args;
 using tk::LN2;
 using tk::LOG2E;
@@ -89,44 +94,80 @@ __device__ inline Place place(const Args& a) {
     return p;
 }
 
+// The value that many bytes behind an address that all lanes have
+__device__ inline float at(const float* base, unsigned bytes) { return *(const float*)((const char*)base + bytes); }
+
+// Memory from an address on that all lanes have.  Stores of lanes behind `bytes` are dropped; loads stay before the end by
+// themselves (WHOLE).
+constexpr unsigned WHOLE = 0x7ffffff0u;
+constexpr unsigned SIZE = sizeof(value_t);
+__device__ inline value_t load(pw_rsrc rs, unsigned lane_bytes, unsigned bytes) {
+#if SPIO_DTYPE == 2
+    return pw::as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, (int)lane_bytes, (int)bytes, 0));
+#else
+    return __builtin_bit_cast(value_t, __builtin_amdgcn_raw_buffer_load_b16(rs, (int)lane_bytes, (int)bytes, 0));
+#endif
+}
+// (The offset within the range is the lane's alone: it is what is compared with the end.)
+__device__ inline void store(pw_rsrc rs, unsigned lane_bytes, value_t v) {
+#if SPIO_DTYPE == 2
+    __builtin_amdgcn_raw_buffer_store_b32(pw::as_bits(v), rs, (int)lane_bytes, 0, 0);
+#else
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rs, (int)lane_bytes, 0, 0);
+#endif
+}
+__device__ inline void store_float(pw_rsrc rs, unsigned lane_bytes, float v) {
+    __builtin_amdgcn_raw_buffer_store_b32(pw::as_bits(v), rs, (int)lane_bytes, 0, 0);
+}
+// The rows of a tile of an array [tokens][channels] to be stored to, as far as there are tokens
+__device__ inline pw_rsrc rows_to(void* to, const Args& a, const Place& p, int token) {
+    const int count = p.last - token < T ? p.last - token : T;
+    return pw::buffer((value_t*)to + (p.sequence * a.tokens + token) * a.channels, (unsigned)count * (unsigned)a.channels * SIZE);
+}
+
 // The tile of tokens [token, token + T), those from `last` on in the place of which the last one is read.
 struct Tile {
-    value_t u[T], delta[T], gate[T], dout[T], bc[STAGED];
+    value_t u[T], delta[T], gate[T], dout[T], B[STAGED], C[STAGED];
 };
+__device__ inline void request_channels(value_t (&v)[T], const void* from, long long stride, long long row0, const Place& p, int token) {
+    const pw_rsrc rs = pw::buffer((const value_t*)from + (row0 + token) * stride, WHOLE);
+    const int left = p.last - 1 - token;
+#pragma unroll
+    for (int t = 0; t < T; ++t) v[t] = load(rs, (unsigned)p.loaded * SIZE, (unsigned)(t < left ? t : left) * (unsigned)stride * SIZE);
+}
+__device__ inline void request_rows(value_t (&v)[STAGED], const void* from, long long stride, long long row0, const Place& p, int token) {
+    const int lane = (int)__builtin_amdgcn_workitem_id_x();
+    const pw_rsrc rs = pw::buffer((const value_t*)from + (row0 + token) * stride, WHOLE);
+    const int left = p.last - 1 - token;
+#pragma unroll
+    for (int i = 0; i < STAGED; ++i) {
+        const int e = i * 64 + lane, t = e / N < left ? e / N : left;
+        v[i] = load(rs, (unsigned)(t * (int)stride + e % N) * SIZE, 0);
+    }
+}
 template <bool U, bool DOUT, bool B, bool C>
 __device__ inline void request(Tile& tile, const Args& a, const Place& p, int token) {
     const long long row0 = p.sequence * a.tokens;
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-        const int at = token + t < p.last ? token + t : p.last - 1;
-        const long long row = row0 + at;
-        if (U) tile.u[t] = ((const value_t*)a.u + row * a.u_row)[p.loaded];
-        tile.delta[t] = ((const value_t*)a.delta + row * a.delta_row)[p.loaded];
-        if (C && a.gate) tile.gate[t] = ((const value_t*)a.gate + row * a.gate_row)[p.loaded];
-        if (DOUT) tile.dout[t] = ((const value_t*)a.dout + row * a.channels)[p.loaded];
-    }
-    const int lane = (int)__builtin_amdgcn_workitem_id_x();
-#pragma unroll
-    for (int i = 0; i < STAGED; ++i) {
-        int e = i * 64 + lane;
-        e = e < T * M ? e : T * M - 1;
-        const int t = e / M, s = e % M;
-        const int at = token + t < p.last ? token + t : p.last - 1;
-        const bool is_c = s >= N;
-        if (is_c ? !C : !B) continue;
-        const value_t* from = is_c ? (const value_t*)a.C + (row0 + at) * a.c_row + (s - N) : (const value_t*)a.B + (row0 + at) * a.b_row + s;
-        tile.bc[i] = *from;
-    }
+    if (U) request_channels(tile.u, a.u, a.u_row, row0, p, token);
+    request_channels(tile.delta, a.delta, a.delta_row, row0, p, token);
+    if (C && GATE) request_channels(tile.gate, a.gate, a.gate_row, row0, p, token);
+    if (DOUT) request_channels(tile.dout, a.dout, a.channels, row0, p, token);
+    if (B) request_rows(tile.B, a.B, a.b_row, row0, p, token);
+    if (C) request_rows(tile.C, a.C, a.c_row, row0, p, token);
 }
 // B and C of the tile in LDS, [T][2][NP]
+template <bool B, bool C>
 __device__ inline void stage(const Tile& tile, float* lds) {
     const int lane = (int)__builtin_amdgcn_workitem_id_x();
     barrier();
 #pragma unroll
     for (int i = 0; i < STAGED; ++i) {
-        const int e = i * 64 + lane, t = e / M, s = e % M;
-        if (e < T * M) lds[(t * 2 + (s >= N)) * NP + (s >= N ? s - N : s)] = (float)tile.bc[i];
+        const int e = i * 64 + lane, t = e / N, s = e % N;
+        if (e >= T * N) break;
+        if (B) lds[t * 2 * NP + s] = (float)tile.B[i];
+        if (C) lds[(t * 2 + 1) * NP + s] = (float)tile.C[i];
     }
+    if (N % 2 && lane < 2 * T) lds[lane * NP + N] = 0.f;  // (read where the states are halved)
     barrier();
 }
 __device__ inline void row_of(const float* lds, int t, int which, float (&v)[NP]) {
@@ -139,28 +180,20 @@ __device__ inline void row_of(const float* lds, int t, int which, float (&v)[NP]
     }
 }
 
+// The states of a half of the wave only, (N + 1) / 2 each; zeros behind the last one
+template <int H>
+__device__ inline void half_row(const float* lds, int t, int which, int half, float (&v)[H]) {
+    const float* row = lds + (t * 2 + which) * NP + half * H;
+#pragma unroll
+    for (int i = 0; i < H; ++i) v[i] = row[i];
+}
+
 // A of a channel as the exponents of 2 that its rates are
 __device__ inline void rates(const Args& a, const Place& p, float (&A2)[N]) {
 #pragma unroll
     for (int s = 0; s < N; ++s) A2[s] = a.A[(long long)p.loaded * N + s] * LOG2E;
 }
-__device__ inline float time_step(const Args& a, float delta, float bias) {
-    const float raw = delta + bias;
-    return a.softplus ? softplus(raw) : raw;
-}
-
-// What precedes the chunk in the order of the scan, joined: chunk by chunk from the far end, v = exp(A sum dl) v + end
-__device__ inline void join(const Args& a, const Place& p, const float (&A2)[N], float (&v)[N], bool back) {
-    const long long row = a.channels;
-    const float* ends = a.ends + p.sequence * p.chunks * (N + 1) * row + p.loaded;
-    const int count = back ? p.chunks - 1 - p.chunk : p.chunk;
-    for (int i = 0; i < count; ++i) {
-        const float* e = ends + (long long)(back ? p.chunks - 1 - i : i) * (N + 1) * row;
-        const float sum = e[N * row];
-#pragma unroll
-        for (int s = 0; s < N; ++s) v[s] = __builtin_fmaf(exp2_(sum * A2[s]), v[s], e[s * row]);
-    }
-}
+__device__ inline float time_step(float raw) { return SOFTPLUS ? softplus(raw) : raw; }
 
 }  // namespace
 
@@ -178,27 +211,39 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
     const float bias = a.bias ? a.bias[p.loaded] : 0.f;
     const float D = OUT && a.D ? a.D[p.loaded] : 0.f;
 #pragma unroll
-    for (int s = 0; s < N; ++s) h[s] = OUT && a.before ? a.before[(p.sequence * a.channels + p.loaded) * N + s] : 0.f;
-    if (OUT && p.chunk) join(a, p, A2, h, false);
+    for (int s = 0; s < N; ++s) h[s] = 0.f;
+    if (OUT && p.chunks > 1) {
+        const float* start = a.ends + (p.sequence * p.chunks + p.chunk) * (N + 1) * a.channels;
+#pragma unroll
+        for (int s = 0; s < N; ++s) h[s] = at(start + s * a.channels, (unsigned)p.loaded * 4u);
+    } else if (OUT && a.before) {
+#pragma unroll
+        for (int s = 0; s < N; ++s) h[s] = a.before[(p.sequence * a.channels + p.loaded) * N + s];
+    }
     float sum = 0.f;
     const long long tiles = (a.tokens + T - 1) / T;
+    const unsigned lane_bytes = p.live ? (unsigned)p.channel * SIZE : pw::OOB;
     for (int token = p.first; token < p.last; token += T) {
-        stage(tile, lds);
+        stage<true, OUT>(tile, lds);
         float u[T], dl[T], gate[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             u[t] = (float)tile.u[t];
-            dl[t] = time_step(a, (float)tile.delta[t], bias);
+            dl[t] = time_step((float)tile.delta[t] + bias);
             if (token + t >= p.last) u[t] = dl[t] = 0.f;  // (decays by 1, adds nothing)
-            gate[t] = OUT && a.gate ? (float)tile.gate[t] : 0.f;
+            gate[t] = OUT && GATE ? (float)tile.gate[t] : 0.f;
             if (!OUT) sum += dl[t];
         }
         if (token + T < p.last) request<true, false, true, OUT>(tile, a, p, token + T);
-        if (OUT && a.kept && p.live) {
-            float* kept = a.kept + ((p.sequence * tiles + token / T) * N) * a.channels + p.channel;
+        if (OUT && KEEP) {
+            const pw_rsrc kept = pw::buffer(a.kept + (p.sequence * tiles + token / T) * N * a.channels, N * (unsigned)a.channels * 4);
 #pragma unroll
-            for (int s = 0; s < N; ++s) kept[s * a.channels] = h[s];
+            for (int s = 0; s < N; ++s) {
+                const int row = s * (int)a.channels * 4;
+                __builtin_amdgcn_raw_buffer_store_b32(pw::as_bits(h[s]), kept, (int)(p.live ? (unsigned)p.channel * 4 : pw::OOB), row, 0);
+            }
         }
+        const pw_rsrc out = rows_to(a.out, a, p, token);
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             float B[NP], C[NP];
@@ -211,9 +256,9 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
                 h[s] = __builtin_fmaf(exp2_(dl[t] * A2[s]), h[s], x * B[s]);
                 if (OUT) y = __builtin_fmaf(C[s], h[s], y);
             }
-            if (OUT && token + t < p.last && p.live) {
-                if (a.gate) y *= gate[t] * pw::sigmoid(gate[t]);
-                ((value_t*)a.out + (p.sequence * a.tokens + token + t) * a.channels)[p.channel] = (value_t)y;
+            if (OUT) {
+                if (GATE) y *= gate[t] * pw::sigmoid(gate[t]);
+                store(out, lane_bytes + (unsigned)t * (unsigned)a.channels * SIZE, (value_t)y);
             }
         }
     }
@@ -244,13 +289,13 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
 #pragma unroll
     for (int s = 0; s < N; ++s) r[s] = 0.f;
     for (; token >= p.first; token -= T) {
-        stage(tile, lds);
+        stage<false, true>(tile, lds);
         float dy[T], dl[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const float gate = a.gate ? (float)tile.gate[t] : 0.f;
-            dy[t] = (float)tile.dout[t] * (a.gate ? gate * pw::sigmoid(gate) : 1.f);
-            dl[t] = time_step(a, (float)tile.delta[t], bias);
+            const float gate = GATE ? (float)tile.gate[t] : 0.f;
+            dy[t] = (float)tile.dout[t] * (GATE ? gate * pw::sigmoid(gate) : 1.f);
+            dl[t] = time_step((float)tile.delta[t] + bias);
             if (token + t >= p.last) dy[t] = dl[t] = 0.f;
             sum += dl[t];
         }
@@ -317,41 +362,87 @@ struct Sum<6, m> {
 
 }  // namespace
 
-extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64), amdgpu_waves_per_eu(SPIO_WAVES))) SPIO_KERNEL_NAME(const Args a) {
+// A lane has two channels, 32 apart, and half of their states: the sums over channels of dB and dC so begin within a lane and
+// cross 32 others, half as many steps as with a channel a lane, and a lane needs half of B and C.  What goes by channel (time
+// steps, gradients of the inputs) is done with a channel a lane, and passes through LDS one way, through an exchange of
+// halves of the wave with which the sums over states end the other way.
+extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64), amdgpu_waves_per_eu(SPIO_WAVES)))
+SPIO_KERNEL_NAME(const Args a) {
     __shared__ __attribute__((aligned(16))) float lds[T * 2 * NP];
-    enum { U, DL, SLOPE, DY, DGATE, OWN };
-    __shared__ float own[T][OWN][64];  // what a lane has of every token of the tile, out of the registers' way
-    const int lane = (int)__builtin_amdgcn_workitem_id_x();
+    enum { DL, X, DY, U, SLOPE, DGATE, OWN };
+    __shared__ float own[T][OWN][64];  // of every token of the tile, by channel
+    constexpr int H = (N + 1) / 2;     // states of a lane
+    const int lane = (int)__builtin_amdgcn_workitem_id_x(), half = lane / 32, j = lane % 32;
     const Place p = place(a);
     const int blocks = (int)((a.channels + 63) / 64);
     const long long tiles = (a.tokens + T - 1) / T;
     Tile tile;
     int token = p.first + (p.last - p.first - 1) / T * T;
     request<true, true, true, true>(tile, a, p, token);
-    float A2[N], r[N], dA[N];
-    rates(a, p, A2);
+    int channel[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        channel[c] = p.block * 64 + c * 32 + j;
+        channel[c] = channel[c] < (int)a.channels ? channel[c] : (int)a.channels - 1;
+    }
+    // (a state behind the last one, where they are odd: rate, B and C of zero)
+    auto state = [&](int i) { return half * H + i < N ? half * H + i : N - 1; };
+    auto there = [&](int i) { return half * H + i < N; };
+    // bytes from a row of channels [i] of a [N][channels] array to the lane's state i
+    auto offset = [&](int c, int i) {
+        const int skipped = N % 2 && i == H - 1 ? half * (N - H) : half * H;
+        return (unsigned)(skipped * (int)a.channels + channel[c]) * 4u;
+    };
+    float A2[2][H], r[2][H], dA[2][H];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            A2[c][i] = there(i) ? a.A[(long long)channel[c] * N + state(i)] * LOG2E : 0.f;
+            r[c][i] = dA[c][i] = 0.f;
+        }
+    if (p.chunks > 1) {  // what the chunks behind this one add
+        const float* start = a.ends + (p.sequence * p.chunks + p.chunk) * (N + 1) * a.channels;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) r[c][i] = there(i) ? at(start + i * a.channels, offset(c, i)) : 0.f;
+    }
     const float bias = a.bias ? a.bias[p.loaded] : 0.f;
     const float D = a.D ? a.D[p.loaded] : 0.f;
+    const unsigned lane_bytes = p.live ? (unsigned)p.channel * SIZE : pw::OOB;
     float dD = 0.f, dbias = 0.f;
+    // which of its half's sums a lane ends with
+    const int value = Sum<1, 2 * H>::index(j), sum_state = half * H + value % H;
+    const unsigned sum_bytes = value < 0 || sum_state >= N ? pw::OOB : (unsigned)(p.block * M + value / H * N + sum_state) * 4u;
+    float next[2][H];  // states before the tile that comes next
+    auto request_states = [&](int token) {
+        const float* kept = a.kept + (p.sequence * tiles + token / T) * N * a.channels;
 #pragma unroll
-    for (int s = 0; s < N; ++s) r[s] = dA[s] = 0.f;
-    if (p.chunk + 1 < p.chunks) join(a, p, A2, r, true);
-    const int mine = Sum<0, M>::index(lane);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) next[c][i] = at(kept + i * a.channels, offset(c, i));
+    };
+    request_states(token);
     for (; token >= p.first; token -= T) {
-        float h[N], q[T][N];  // q: exp(dl A) h of the token before
-        const float* kept = a.kept + ((p.sequence * tiles + token / T) * N) * a.channels + p.loaded;
+        float before[2][H], h[T][2][H], decay[HELD ? HELD : 1][2][H];  // states before the tile and behind its tokens
 #pragma unroll
-        for (int s = 0; s < N; ++s) h[s] = kept[s * a.channels];
-        stage(tile, lds);
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < H; ++i) before[c][i] = next[c][i];
+        stage<true, true>(tile, lds);
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const bool there = token + t < p.last && p.live;
+            const bool counts = token + t < p.last && p.live;
             const float raw = (float)tile.delta[t] + bias;
-            const float dout = there ? (float)tile.dout[t] : 0.f;
-            own[t][U][lane] = there ? (float)tile.u[t] : 0.f;
-            own[t][DL][lane] = there ? time_step(a, (float)tile.delta[t], bias) : 0.f;
-            own[t][SLOPE][lane] = a.softplus ? pw::sigmoid(raw) : 1.f;
-            if (a.gate) {
+            const float dout = counts ? (float)tile.dout[t] : 0.f;
+            const float u = counts ? (float)tile.u[t] : 0.f;
+            const float dl = counts ? time_step(raw) : 0.f;
+            own[t][DL][lane] = dl;
+            own[t][X][lane] = dl * u;
+            own[t][U][lane] = u;
+            own[t][SLOPE][lane] = SOFTPLUS ? pw::sigmoid(raw) : 1.f;
+            if (GATE) {
                 const float gate = (float)tile.gate[t], s = pw::sigmoid(gate), v = gate * s;
                 own[t][DY][lane] = dout * v;
                 own[t][DGATE][lane] = dout * __builtin_fmaf(v, 1.f - s, s);
@@ -359,66 +450,84 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64), a
                 own[t][DY][lane] = dout;
             }
         }
-        if (token > p.first) request<true, true, true, true>(tile, a, p, token - T);
+        barrier();
+        const pw_rsrc to_du = rows_to(a.du, a, p, token), to_ddelta = rows_to(a.ddelta, a, p, token),
+                      to_dgate = rows_to(a.dgate, a, p, token);
+        const int count = p.last - token < T ? p.last - token : T;
+        const pw_rsrc token_sums = pw::buffer(a.token_sums + (p.sequence * a.tokens + token) * blocks * M,
+                                              (unsigned)count * (unsigned)blocks * M * 4u);
+        float y[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             __builtin_amdgcn_sched_barrier(0);
-            float B[NP], C[NP];
-            row_of(lds, t, 0, B);
-            row_of(lds, t, 1, C);
-            const float u = own[t][U][lane], dl = own[t][DL][lane], x = dl * u;
-            float y = D * u;
+            float B[H], C[H], part[2];
+            half_row(lds, t, 0, half, B);
+            half_row(lds, t, 1, half, C);
 #pragma unroll
-            for (int s = 0; s < N; ++s) {
-                q[t][s] = exp2_(dl * A2[s]) * h[s];
-                h[s] = __builtin_fmaf(x, B[s], q[t][s]);
-                y = __builtin_fmaf(C[s], h[s], y);
+            for (int c = 0; c < 2; ++c) {
+                __builtin_amdgcn_sched_barrier(0);
+                const float dl = own[t][DL][c * 32 + j], x = own[t][X][c * 32 + j];
+                part[c] = 0.f;
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    const float d = exp2_(dl * A2[c][i]);
+                    if (t >= T - HELD) decay[t - (T - HELD)][c][i] = d;
+                    h[t][c][i] = __builtin_fmaf(d, t ? h[t ? t - 1 : 0][c][i] : before[c][i], x * B[i]);
+                    part[c] = __builtin_fmaf(C[i], h[t][c][i], part[c]);
+                }
             }
-            if (a.gate) own[t][DGATE][lane] *= y;
+            y[t] = halves<0>(part[0], part[1], lane);
         }
 #pragma unroll
         for (int t = T - 1; t >= 0; --t) {
             __builtin_amdgcn_sched_barrier(0);
-            float B[NP], C[NP], sums[N];
-            row_of(lds, t, 0, B);
-            row_of(lds, t, 1, C);
-            const float u = own[t][U][lane], dy = own[t][DY][lane];
-            float dl = own[t][DL][lane];
-            asm("" : "+v"(dl));  // (its exponentials are taken again: those of the way forth would take T * N registers)
-            const float x = dl * u;
-            float gB = 0.f, gq = 0.f;
+            // (once the registers of the last token are free)
+            if (t == T - 2 && token > p.first) request<true, true, true, true>(tile, a, p, token - T);
+            if (t == STATES_AT && token > p.first) request_states(token - T);
+            float B[H], C[H], sums[2 * H], gB[2] = {}, gq[2] = {};
+            half_row(lds, t, 0, half, B);
+            half_row(lds, t, 1, half, C);
 #pragma unroll
-            for (int s = 0; s < N; ++s) {
-                const float g = __builtin_fmaf(C[s], dy, r[s]);
-                sums[s] = halves<0>(x * g, dy * __builtin_fmaf(x, B[s], q[t][s]), lane);
-                gB = __builtin_fmaf(g, B[s], gB);
-                const float w = g * q[t][s];
-                dA[s] = __builtin_fmaf(w, dl, dA[s]);
-                gq = __builtin_fmaf(w, A2[s], gq);
-                r[s] = exp2_(dl * A2[s]) * g;
-            }
-            const float total = Sum<1, N>::of(sums, lane);
-            const float du = __builtin_fmaf(gB, dl, D * dy);
-            const float ddelta = __builtin_fmaf(gB, u, gq * LN2) * own[t][SLOPE][lane];
-            if (token + t < p.last) {
-                dD = __builtin_fmaf(dy, u, dD);
-                dbias += ddelta;
-                const long long row = p.sequence * a.tokens + token + t;
-                if (mine >= 0) a.token_sums[(row * blocks + p.block) * M + mine] = total;
-                if (p.live) {
-                    ((value_t*)a.du + row * a.channels)[p.channel] = (value_t)du;
-                    ((value_t*)a.ddelta + row * a.channels)[p.channel] = (value_t)ddelta;
-                    if (a.gate) ((value_t*)a.dgate + row * a.channels)[p.channel] = (value_t)own[t][DGATE][lane];
+            for (int c = 0; c < 2; ++c) {
+                __builtin_amdgcn_sched_barrier(0);
+                const float x = own[t][X][c * 32 + j], dy = own[t][DY][c * 32 + j];
+                float dl = own[t][DL][c * 32 + j];
+                if (t < T - HELD) asm("" : "+v"(dl));  // (or the exponentials would be held)
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    const float g = __builtin_fmaf(C[i], dy, r[c][i]);
+                    sums[i] = c ? __builtin_fmaf(x, g, sums[i]) : x * g;
+                    sums[H + i] = c ? __builtin_fmaf(dy, h[t][c][i], sums[H + i]) : dy * h[t][c][i];
+                    gB[c] = __builtin_fmaf(g, B[i], gB[c]);
+                    r[c][i] = (t >= T - HELD ? decay[t >= T - HELD ? t - (T - HELD) : 0][c][i] : exp2_(dl * A2[c][i])) * g;
+                    const float w = r[c][i] * (t ? h[t ? t - 1 : 0][c][i] : before[c][i]);
+                    dA[c][i] = __builtin_fmaf(w, dl, dA[c][i]);
+                    gq[c] = __builtin_fmaf(w, A2[c][i], gq[c]);
                 }
             }
+            const float total = Sum<1, 2 * H>::of(sums, lane);
+            const float all_gB = halves<0>(gB[0], gB[1], lane), all_gq = halves<0>(gq[0], gq[1], lane);
+            const float u = own[t][U][lane], dy = own[t][DY][lane];
+            const float du = __builtin_fmaf(all_gB, own[t][DL][lane], D * dy);
+            const float ddelta = __builtin_fmaf(all_gB, u, all_gq * LN2) * own[t][SLOPE][lane];
+            dD = __builtin_fmaf(dy, u, dD);
+            dbias += ddelta;  // (of a token that is not there all are zero)
+            const unsigned row = (unsigned)t * (unsigned)a.channels * SIZE;
+            store_float(token_sums, sum_bytes + (unsigned)t * (unsigned)blocks * M * 4u, total);
+            store(to_du, lane_bytes + row, (value_t)du);
+            store(to_ddelta, lane_bytes + row, (value_t)ddelta);
+            if (GATE) store(to_dgate, lane_bytes + row, (value_t)(own[t][DGATE][lane] * __builtin_fmaf(D, u, y[t])));
         }
     }
-    if (!p.live) return;
-    float* sums = a.channel_sums + (p.sequence * p.chunks + p.chunk) * (N + 2) * a.channels + p.channel;
+    float* sums = a.channel_sums + (p.sequence * p.chunks + p.chunk) * (N + 2) * a.channels;
 #pragma unroll
-    for (int s = 0; s < N; ++s) sums[s * a.channels] = dA[s];
-    sums[N * a.channels] = dD;
-    sums[(N + 1) * a.channels] = dbias;
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+            if (there(i) && p.block * 64 + c * 32 + j < (int)a.channels) *(float*)((char*)(sums + i * a.channels) + offset(c, i)) = dA[c][i];
+    if (!p.live) return;
+    sums[N * a.channels + p.channel] = dD;
+    sums[(N + 1) * a.channels + p.channel] = dbias;
 }
 
 #elif SPIO_MODE == 4
@@ -447,6 +556,42 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
     }
     const long long chunks = (a.tokens + a.chunk - 1) / a.chunk;
     tk::column_sums({a.channel_sums, a.sums, a.sequences * chunks, a.channels, N, 2}, group - row_groups);
+}
+
+#elif SPIO_MODE == 6 || SPIO_MODE == 7
+
+// A lane is a state of a channel, and goes from chunk to chunk, v = exp(A sum dl) v + end, leaving v in the place of the
+// end.  The ends of JOINED chunks are requested at once: waiting for memory is all that it does.
+extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) SPIO_KERNEL_NAME(const Args a) {
+    constexpr bool BACK = SPIO_MODE == 7;
+    constexpr int JOINED = 8;
+    const unsigned blocks = (unsigned)((a.channels + 63) / 64);
+    const unsigned id = __builtin_amdgcn_workgroup_id_x();
+    const long long channel = id % blocks * 64 + __builtin_amdgcn_workitem_id_x();
+    const int s = (int)(id / blocks % N);
+    const long long sequence = id / blocks / N;
+    const int chunks = (int)((a.tokens + a.chunk - 1) / a.chunk);
+    if (channel >= a.channels) return;
+    const float A2 = a.A[channel * N + s] * LOG2E;
+    float v = !BACK && a.before ? a.before[(sequence * a.channels + channel) * N + s] : 0.f;
+    float* ends = a.ends + sequence * chunks * (N + 1) * a.channels + channel;
+    for (int first = 0; first < chunks; first += JOINED) {
+        float end[JOINED], sum[JOINED];
+#pragma unroll
+        for (int k = 0; k < JOINED; ++k) {
+            const int i = first + k < chunks ? first + k : chunks - 1;
+            const float* e = ends + (BACK ? chunks - 1 - i : i) * (N + 1) * a.channels;
+            end[k] = e[s * a.channels];
+            sum[k] = e[N * a.channels];
+        }
+#pragma unroll
+        for (int k = 0; k < JOINED; ++k) {
+            const int i = first + k;
+            if (i >= chunks) break;
+            ends[((BACK ? chunks - 1 - i : i) * (N + 1) + s) * a.channels] = v;
+            v = __builtin_fmaf(exp2_(sum[k] * A2), v, end[k]);
+        }
+    }
 }
 
 #else
@@ -484,8 +629,8 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
         C[i] = there ? (float)((const value_t*)a.C)[sequence * a.c_row + part * 4 + i] : 0.f;
     }
     const float u = (float)((const value_t*)a.u)[sequence * a.u_row + c];
-    const float gate = a.gate ? (float)((const value_t*)a.gate)[sequence * a.gate_row + c] : 0.f;
-    const float dl = time_step(a, (float)((const value_t*)a.delta)[sequence * a.delta_row + c], a.bias ? a.bias[c] : 0.f);
+    const float gate = GATE ? (float)((const value_t*)a.gate)[sequence * a.gate_row + c] : 0.f;
+    const float dl = time_step((float)((const value_t*)a.delta)[sequence * a.delta_row + c] + (a.bias ? a.bias[c] : 0.f));
     const float x = dl * u;
     float y = 0.f;
 #pragma unroll
@@ -499,7 +644,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
     if (at > last) return;
     if (part == 0) {
         y = __builtin_fmaf(a.D ? a.D[c] : 0.f, u, y);
-        if (a.gate) y *= gate * pw::sigmoid(gate);
+        if (GATE) y *= gate * pw::sigmoid(gate);
         ((value_t*)a.out)[item] = (value_t)y;
     }
     float* after = a.after + item * N;

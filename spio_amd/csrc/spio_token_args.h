@@ -21,7 +21,6 @@ struct SpioScanArgs {
     float* sums;          // dA [channels][states], dD [channels], dbias [channels]
     long long tokens, channels, chunk, sequences;
     long long u_row, delta_row, gate_row, b_row, c_row;
-    long long softplus;
 };
 
 struct SpioConv1dArgs {

@@ -56,7 +56,7 @@ enum Kind : int64_t {
     FPROP = 0, DGRAD = 1, WGRAD = 2, BGRAD = 3, NORM = 4, NORM_BWD = 5,
     GROUP_NORM = 6, GROUP_NORM_BWD = 7, ACTIVATION = 8, ACTIVATION_BWD = 9, PACK = 10, UNPACK = 11,
     CONV1D = 12, CONV1D_BWD = 13, CONV1D_SUMS = 14, CONV1D_STEP = 15, SCAN_ENDS = 16, SCAN = 17, SCAN_ENDS_BWD = 18, SCAN_BWD = 19,
-    SCAN_SUMS = 20, SCAN_STEP = 21, ROTARY = 22, ROTARY_BWD = 23, ROTARY_SUMS = 24
+    SCAN_SUMS = 20, SCAN_STEP = 21, SCAN_JOIN = 22, SCAN_JOIN_BWD = 23, ROTARY = 24, ROTARY_BWD = 25, ROTARY_SUMS = 26
 };
 
 // What selects a plan: the kind, the device and the numbers of the problem.
@@ -963,11 +963,13 @@ struct Conv1dFunction : torch::autograd::Function<Conv1dFunction> {
 // ---- selective scan ----
 
 constexpr int64_t SCAN_MAX_STATES = 32, SCAN_LANES = 64;
-int64_t scan_tile(int64_t states) { return states <= 8 ? 8 : states <= 16 ? 6 : 4; }
-int64_t scan_chunk(int64_t tokens, int64_t channels, int64_t sequences, int64_t states) {
-    const int64_t waves = divup(channels, SCAN_LANES) * sequences, tile = scan_tile(states);
-    const int64_t chunks = std::max(int64_t(1), std::min(1024 / waves, tokens / 32));
-    return divup(divup(tokens, chunks), tile) * tile;
+int64_t scan_tile(int64_t states) { return states <= 8 ? 8 : 4; }
+int64_t scan_chunk(int64_t tokens, int64_t channels, int64_t sequences, bool backward) {
+    const int64_t waves = divup(channels, SCAN_LANES) * sequences;
+    if (waves >= (backward ? 1024 : 700)) return tokens;
+    int64_t chunks = 4096 / waves;
+    if (tokens < 48 * chunks) chunks = std::max(int64_t(1), std::min(2048 / waves, tokens / 16));
+    return divup(divup(tokens, chunks), 8) * 8;
 }
 
 struct Scan {
@@ -980,7 +982,7 @@ struct Scan {
 struct ScanInputs {
     SpioScanArgs a = {};
     std::vector<Tensor> held;
-    ScanInputs(const Scan& sc, const variable_list& t) {
+    ScanInputs(const Scan& sc, const variable_list& t, bool backward = false) {
         auto rows = [&](int i, const void*& p, long long& row) {
             const Rows r = rows_of(t[i]);
             held.push_back(r.t);
@@ -993,12 +995,14 @@ struct ScanInputs {
         };
         rows(0, a.u, a.u_row), rows(1, a.delta, a.delta_row), rows(3, a.B, a.b_row), rows(4, a.C, a.c_row), rows(6, a.gate, a.gate_row);
         parameter(2, a.A, true), parameter(5, a.D), parameter(7, a.bias);
-        a.tokens = sc.l, a.channels = sc.c, a.sequences = sc.n, a.softplus = sc.softplus;
-        a.chunk = scan_chunk(sc.l, sc.c, sc.n, sc.s);
+        a.tokens = sc.l, a.channels = sc.c, a.sequences = sc.n;
+        a.chunk = scan_chunk(sc.l, sc.c, sc.n, backward);
     }
 };
-PlanPtr scan_plan(Kind kind, const Scan& sc, const Tensor& u) {
-    return find_plan(token_key(kind, u.get_device(), sc.s, dtype_number(u)));
+// (the first pass forward reads no gate; the sums and joins neither that nor time steps)
+PlanPtr scan_plan(Kind kind, const Scan& sc, const Tensor& u, bool gate, bool keep = false) {
+    const int64_t flags = kind == SCAN_SUMS || kind == SCAN_JOIN || kind == SCAN_JOIN_BWD ? 0 : (gate && kind != SCAN_ENDS) + 2 * sc.softplus + 4 * keep;
+    return find_plan(token_key(kind, u.get_device(), sc.s, dtype_number(u), flags));
 }
 Tensor scan_forward(Scan& sc, const variable_list& t, Tensor* kept) {
     const Tensor& u = t[0];
@@ -1013,8 +1017,11 @@ Tensor scan_forward(Scan& sc, const variable_list& t, Tensor* kept) {
     if (chunks > 1) ends = empty_1d(sc.n * chunks * (sc.s + 1) * sc.c, at::kFloat, u);
     in.a.before = floats(before), in.a.out = mut(y), in.a.after = floats(sc.after), in.a.ends = floats(ends);
     in.a.kept = kept ? floats(*kept) : nullptr;
-    if (chunks > 1) launch_structure(*scan_plan(SCAN_ENDS, sc, u), grid, stream, &in.a);
-    launch_structure(*scan_plan(SCAN, sc, u), grid, stream, &in.a);
+    if (chunks > 1) {
+        launch_structure(*scan_plan(SCAN_ENDS, sc, u, false), grid, stream, &in.a);
+        launch_structure(*scan_plan(SCAN_JOIN, sc, u, false), sc.n * sc.s * divup(sc.c, SCAN_LANES), stream, &in.a);
+    }
+    launch_structure(*scan_plan(SCAN, sc, u, t[6].defined(), kept != nullptr), grid, stream, &in.a);
     return y;
 }
 
@@ -1060,7 +1067,7 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
             return out;
         }
         RECORD_FUNCTION("spio::selective_scan_backward", tensors({dy, u, t[1], t[2], t[3], t[4], t[5], t[6], t[7]}));
-        ScanInputs in(sc, t);
+        ScanInputs in(sc, t, true);
         const int64_t chunks = divup(sc.l, in.a.chunk), blocks = divup(sc.c, SCAN_LANES), grid = sc.n * chunks * blocks;
         hipStream_t stream = c10::hip::getCurrentHIPStream(u.get_device());
         const Tensor g = dy.contiguous(), k = kept.contiguous();
@@ -1075,9 +1082,12 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
         in.a.dout = ptr(g), in.a.kept = floats(k), in.a.ends = floats(ends), in.a.du = mut(du), in.a.ddelta = mut(ddelta);
         in.a.dgate = mut(dgate), in.a.dB = mut(dB), in.a.dC = mut(dC), in.a.sums = floats(sums);
         in.a.token_sums = floats(token_sums), in.a.channel_sums = floats(channel_sums);
-        if (chunks > 1) launch_structure(*scan_plan(SCAN_ENDS_BWD, sc, u), grid, stream, &in.a);
-        launch_structure(*scan_plan(SCAN_BWD, sc, u), grid, stream, &in.a);
-        launch_structure(*scan_plan(SCAN_SUMS, sc, u), divup(sc.n * sc.l * 2 * sc.s, 256) + divup((sc.s + 2) * sc.c, SUM_COLUMNS),
+        if (chunks > 1) {
+            launch_structure(*scan_plan(SCAN_ENDS_BWD, sc, u, t[6].defined()), grid, stream, &in.a);
+            launch_structure(*scan_plan(SCAN_JOIN_BWD, sc, u, false), sc.n * sc.s * blocks, stream, &in.a);
+        }
+        launch_structure(*scan_plan(SCAN_BWD, sc, u, t[6].defined()), grid, stream, &in.a);
+        launch_structure(*scan_plan(SCAN_SUMS, sc, u, false), divup(sc.n * sc.l * 2 * sc.s, 256) + divup((sc.s + 2) * sc.c, SUM_COLUMNS),
                          stream, &in.a);
         at::AutoDispatchBelowADInplaceOrView below;
         auto sum = [&](int i, int64_t from, int64_t count) { return typed(sums.narrow(0, from, count), v[5 + i]); };
@@ -1686,7 +1696,7 @@ PyObject* selective_scan_step(PyObject*, PyObject* const* args, Py_ssize_t nargs
         RECORD_FUNCTION("spio::selective_scan_step", tensors({u, sc.before, t[1], t[2], t[3], t[4], t[5], t[6], t[7]}));
         at::AutoDispatchBelowADInplaceOrView below;
         ScanInputs in(sc, t);
-        const auto plan = scan_plan(SCAN_STEP, sc, u);
+        const auto plan = scan_plan(SCAN_STEP, sc, u, t[6].defined());
         y = empty_of({sc.n, sc.c}, u.scalar_type(), u);
         in.a.before = floats(sc.before), in.a.out = mut(y), in.a.after = floats(after);
         const int64_t lanes = sc.s <= 4 ? 1 : sc.s <= 8 ? 2 : sc.s <= 16 ? 4 : 8;

@@ -25,6 +25,8 @@ from ..kernels.selective_scan_kernel import (
     selective_scan_bwd_kernel_factory,
     selective_scan_ends_bwd_kernel_factory,
     selective_scan_ends_kernel_factory,
+    selective_scan_join_bwd_kernel_factory,
+    selective_scan_join_kernel_factory,
     selective_scan_kernel_factory,
     selective_scan_step_kernel_factory,
     selective_scan_sums_kernel_factory,
@@ -94,18 +96,22 @@ def selective_scan_forward(
         if after.numel():
             after.copy_(initial_state) if initial_state is not None else after.zero_()
         return out, after, kept
-    params = SelectiveScanParams(s, DTYPES[inputs.dtype])
-    chunk = chunk_tokens(l, c, n, s)
+    dtype, gated, softplus = DTYPES[inputs.dtype], gate is not None, bool(delta_softplus)
+    chunk = chunk_tokens(l, c, n, False)
     chunks, blocks = divup(l, chunk), divup(c, LANES)
     ends = torch.empty((n, chunks, s + 1, c), **f32) if chunks > 1 else None
     arguments = Arguments(
         STRUCT, **_rows(inputs, delta, B, C, gate), A=vector(A), D=vector(D), bias=vector(delta_bias),
         before=None if initial_state is None else initial_state.contiguous(), out=out, after=after if keep_state else None,
-        kept=kept if keep_tiles else None, ends=ends, tokens=l, channels=c, chunk=chunk, sequences=n,
-        softplus=bool(delta_softplus))  # fmt: skip
+        kept=kept if keep_tiles else None, ends=ends, tokens=l, channels=c, chunk=chunk, sequences=n)  # fmt: skip
+    grid = n * chunks * blocks
     if chunks > 1:
-        selective_scan_ends_kernel_factory.get_kernel(params, inputs.device).launch_structure(n * chunks * blocks, arguments)
-    selective_scan_kernel_factory.get_kernel(params, inputs.device).launch_structure(n * chunks * blocks, arguments)
+        ends_kernel = selective_scan_ends_kernel_factory.get_kernel(SelectiveScanParams(s, dtype, False, softplus), inputs.device)
+        ends_kernel.launch_structure(grid, arguments)
+        join = selective_scan_join_kernel_factory.get_kernel(SelectiveScanParams(s, dtype), inputs.device)
+        join.launch_structure(n * s * blocks, arguments)
+    kernel = selective_scan_kernel_factory.get_kernel(SelectiveScanParams(s, dtype, gated, softplus, bool(keep_tiles)), inputs.device)
+    kernel.launch_structure(grid, arguments)
     return out, after, kept
 
 
@@ -140,20 +146,23 @@ def selective_scan_backward(
     sums = torch.empty((c * (s + 2),), **f32)
     if du.numel() == 0:
         return du, ddelta, dB, dC, dgate, sums.zero_()
-    params = SelectiveScanParams(s, DTYPES[inputs.dtype])
-    chunk = chunk_tokens(l, c, n, s)
+    dtype, gated, softplus = DTYPES[inputs.dtype], gate is not None, bool(delta_softplus)
+    chunk = chunk_tokens(l, c, n, True)
     chunks, blocks = divup(l, chunk), divup(c, LANES)
     arguments = Arguments(
         STRUCT, **_rows(inputs, delta, B, C, gate), dout=grad_output.contiguous(), A=vector(A), D=vector(D),
         bias=vector(delta_bias), kept=kept.contiguous(), ends=torch.empty((n, chunks, s + 1, c), **f32) if chunks > 1 else None,
         du=du, ddelta=ddelta, dgate=dgate if gate is not None else None,
         token_sums=torch.empty((n, l, blocks, 2 * s), **f32), channel_sums=torch.empty((n, chunks, s + 2, c), **f32),
-        dB=dB, dC=dC, sums=sums, tokens=l, channels=c, chunk=chunk, sequences=n, softplus=bool(delta_softplus))  # fmt: skip
+        dB=dB, dC=dC, sums=sums, tokens=l, channels=c, chunk=chunk, sequences=n)  # fmt: skip
+    params = SelectiveScanParams(s, dtype, gated, softplus)
     if chunks > 1:
         selective_scan_ends_bwd_kernel_factory.get_kernel(params, inputs.device).launch_structure(n * chunks * blocks, arguments)
+        join = selective_scan_join_bwd_kernel_factory.get_kernel(SelectiveScanParams(s, dtype), inputs.device)
+        join.launch_structure(n * s * blocks, arguments)
     selective_scan_bwd_kernel_factory.get_kernel(params, inputs.device).launch_structure(n * chunks * blocks, arguments)
     grid = divup(n * l * 2 * s, 256) + divup((s + 2) * c, SUM_COLUMNS)
-    selective_scan_sums_kernel_factory.get_kernel(params, inputs.device).launch_structure(grid, arguments)
+    selective_scan_sums_kernel_factory.get_kernel(SelectiveScanParams(s, dtype), inputs.device).launch_structure(grid, arguments)
     return du, ddelta, dB, dC, dgate, sums
 
 
@@ -250,10 +259,10 @@ def selective_scan_step_op(
     out = torch.empty((n, c), dtype=inputs.dtype, device=inputs.device)
     if n == 0:
         return out
-    kernel = selective_scan_step_kernel_factory.get_kernel(SelectiveScanParams(s, DTYPES[inputs.dtype]), inputs.device)
+    params = SelectiveScanParams(s, DTYPES[inputs.dtype], gate is not None, bool(delta_softplus))
+    kernel = selective_scan_step_kernel_factory.get_kernel(params, inputs.device)
     arguments = Arguments(STRUCT, **_rows(inputs, delta, B, C, gate), A=aligned(vector(A)), D=vector(D), bias=vector(delta_bias),
-                          before=state, out=out, after=out_state, tokens=1, channels=c, chunk=1, sequences=n,
-                          softplus=bool(delta_softplus))  # fmt: skip
+                          before=state, out=out, after=out_state, tokens=1, channels=c, chunk=1, sequences=n)  # fmt: skip
     lanes = 1 if s <= 4 else 2 if s <= 8 else 4 if s <= 16 else 8
     kernel.launch_structure(divup(n * c * lanes, 256), arguments)
     return out

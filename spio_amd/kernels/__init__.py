@@ -48,6 +48,8 @@ from .selective_scan_kernel import (
     selective_scan_bwd_kernel_factory,
     selective_scan_sums_kernel_factory,
     selective_scan_step_kernel_factory,
+    selective_scan_join_kernel_factory,
+    selective_scan_join_bwd_kernel_factory,
     SelectiveScanParams,
     SelectiveScanConfig,
 )

@@ -18,27 +18,41 @@ LANES = 64  # channels of a workgroup
 
 def tile_tokens(states: int) -> int:
     """Tokens of a tile: those whose states the backward pass holds in registers at once, and the distance of the states
-    that the forward pass keeps for it."""
-    return 8 if states <= 8 else 6 if states <= 16 else 4
+    that the forward pass keeps for it.  Longer tiles keep less (4n 2048l 2048c with 16 states, forward: 98 us with 8 tokens,
+    124 with 4), but 16 states of five tokens and more have no room in half a SIMD's registers (backward: 233 us with 4
+    tokens, 254 with 5, 397 with 6, 542 with 8)."""
+    return 8 if states <= 8 else 4
 
 
-def chunk_tokens(tokens: int, channels: int, sequences: int, states: int) -> int:
-    """Tokens of a chunk, whole tiles: all of them where sequences and channels alone give every SIMD a wave."""
+def chunk_tokens(tokens: int, channels: int, sequences: int, backward: bool) -> int:
+    """Tokens of a chunk.  All of them where sequences and channels alone give most SIMDs a wave: a first pass over chunks
+    costs as much as it brings then (forward, us whole and in chunks: 1024 waves 49 and 69, 1536 waves 115 and 142; backward
+    1024 waves 138 and 134).  Else as many chunks as fill the device, whose SIMDs hold two waves of the backward pass,
+    once or, where chunks then keep 48 tokens, twice (4n 2048l 2048c backward: 2048 waves 241 us, 3072 253, 4096 217), but
+    none of fewer than 16 tokens."""
     waves = divup(channels, LANES) * sequences
-    tile = tile_tokens(states)
-    chunks = max(1, min(1024 // waves, tokens // 32))
-    return divup(divup(tokens, chunks), tile) * tile
+    if waves >= (1024 if backward else 700):
+        return tokens
+    chunks = 4096 // waves
+    if tokens < 48 * chunks:
+        chunks = max(1, min(2048 // waves, tokens // 16))
+    return divup(divup(tokens, chunks), 8) * 8
 
 
 @dataclass(frozen=True)
 class SelectiveScanParams:
-    """States of a channel, and the number of the tensors' type (group_norm_2d_kernel.DTYPES)."""
+    """States of a channel, the number of the tensors' type (group_norm_2d_kernel.DTYPES), and what the kernel does of what
+    is optional: gate, softplus of the time steps, keeping states for the backward pass."""
 
     states: int
     dtype: int = 0
+    gate: bool = False
+    softplus: bool = False
+    keep: bool = False
 
     def encode(self) -> str:
-        return f"{self.states}s_{DTYPE_NAMES[self.dtype]}"
+        flags = ("_gate" if self.gate else "") + ("_softplus" if self.softplus else "") + ("_keep" if self.keep else "")
+        return f"{self.states}s_{DTYPE_NAMES[self.dtype]}{flags}"
 
     def validate(self):
         assert 1 <= self.states <= MAX_STATES and 0 <= self.dtype <= 2
@@ -46,16 +60,18 @@ class SelectiveScanParams:
 
 @dataclass(frozen=True)
 class SelectiveScanConfig:
-    """Tokens of a tile."""
+    """Tokens of a tile, and how many of its last ones the backward pass holds the decays of: one where the registers have
+    room for it (16 states: 217 us, without 231, with two 237)."""
 
     tile: int
+    held: int = 0
 
 
 def _spec(mode, threads):
     def spec(params: SelectiveScanParams, config: SelectiveScanConfig, _device_attr=None) -> KernelSpec:
         params.validate()
-        defines = {"SPIO_MODE": mode, "SPIO_STATES": params.states, "SPIO_DTYPE": params.dtype, "SPIO_T": config.tile,
-                   "SPIO_WAVES": 2 if params.states <= 16 else 1}  # fmt: skip
+        defines = {"SPIO_MODE": mode, "SPIO_STATES": params.states, "SPIO_DTYPE": params.dtype, "SPIO_T": config.tile, "SPIO_HELD": config.held, "SPIO_WAVES": 2 if params.states <= 16 else 1, "SPIO_GATE": int(params.gate),
+                   "SPIO_SOFTPLUS": int(params.softplus), "SPIO_KEEP": int(params.keep)}  # fmt: skip
         return KernelSpec(defines, LaunchParams(grid=1, block=threads), SOURCE, takes_structure=True)
 
     return spec
@@ -67,7 +83,7 @@ def _factory(name, mode, threads):
         SelectiveScanConfig,
         None,
         kernel_name=name,
-        configs=lambda params, device_attr=None: [SelectiveScanConfig(tile_tokens(params.states))],
+        configs=lambda params, device_attr=None: [SelectiveScanConfig(tile_tokens(params.states), int(8 < params.states <= 16))],
         kernel_spec=_spec(mode, threads),
         args_checker=None,
     )
@@ -79,3 +95,5 @@ selective_scan_ends_bwd_kernel_factory = _factory("spio_selective_scan_ends_bwd"
 selective_scan_bwd_kernel_factory = _factory("spio_selective_scan_bwd", 3, 64)
 selective_scan_sums_kernel_factory = _factory("spio_selective_scan_sums", 4, 256)
 selective_scan_step_kernel_factory = _factory("spio_selective_scan_step", 5, 256)
+selective_scan_join_kernel_factory = _factory("spio_selective_scan_join", 6, 64)
+selective_scan_join_bwd_kernel_factory = _factory("spio_selective_scan_join_bwd", 7, 64)

@@ -165,15 +165,16 @@ def _token_kernel(kind, numbers):
         factories = (kernels.causal_conv1d_kernel_factory, kernels.causal_conv1d_bwd_kernel_factory,
                      kernels.causal_conv1d_sums_kernel_factory, kernels.causal_conv1d_step_kernel_factory)  # fmt: skip
         return factories[kind - 12], kernels.CausalConv1dParams(width, dtype, weight_dtype, activation)
-    if kind < 22:
+    if kind < 24:
         factories = (kernels.selective_scan_ends_kernel_factory, kernels.selective_scan_kernel_factory,
                      kernels.selective_scan_ends_bwd_kernel_factory, kernels.selective_scan_bwd_kernel_factory,
-                     kernels.selective_scan_sums_kernel_factory, kernels.selective_scan_step_kernel_factory)  # fmt: skip
-        return factories[kind - 16], kernels.SelectiveScanParams(*numbers[:2])
+                     kernels.selective_scan_sums_kernel_factory, kernels.selective_scan_step_kernel_factory,
+                     kernels.selective_scan_join_kernel_factory, kernels.selective_scan_join_bwd_kernel_factory)  # fmt: skip
+        return factories[kind - 16], kernels.SelectiveScanParams(*numbers[:2], *(bool(numbers[2] & bit) for bit in (1, 2, 4)))
     factories = (kernels.head_norm_rotary_kernel_factory, kernels.head_norm_rotary_bwd_kernel_factory,
                  kernels.head_norm_rotary_sums_kernel_factory)  # fmt: skip
     head, dtype, norm, interleaved = numbers
-    return factories[kind - 22], kernels.HeadNormRotaryParams(head, dtype, bool(norm), bool(interleaved))
+    return factories[kind - 24], kernels.HeadNormRotaryParams(head, dtype, bool(norm), bool(interleaved))
 
 
 class NativeOp(CustomOpDef):
