@@ -32,14 +32,28 @@ typedef __bf16 weight_t;
 typedef float weight_t;
 #endif
 
+// Filters and biases of eight channels: they start on 16 bytes and are W + 1 units of eight values
+__device__ inline void unit_of(const void* from, long long unit, float (&v)[8]) {
+    const pw_uint4* p = (const pw_uint4*)((const weight_t*)from + unit * 8);
+    typedef weight_t weight4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const weight4 w = ((const weight4*)p)[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * i + e] = (float)w[e];
+    }
+}
 __device__ inline void filters(const SpioConv1dArgs& a, long long channel, float (&w)[W][8], float (&bias)[8]) {
-    const weight_t* weight = (const weight_t*)a.weight + channel * W;
+    float all[W][8];
+#pragma unroll
+    for (int i = 0; i < W; ++i) unit_of(a.weight, channel / 8 * W + i, all[i]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        bias[e] = a.bias ? (float)((const weight_t*)a.bias)[channel + e] : 0.f;
+        bias[e] = 0.f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i][e] = (float)weight[e * W + i];
+        for (int i = 0; i < W; ++i) w[i][e] = all[(e * W + i) / 8][(e * W + i) % 8];
     }
+    if (a.bias) unit_of(a.bias, channel / 8, bias);
 }
 
 // The place of a lane: eight channels of a slice of a sequence
@@ -110,12 +124,12 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
                 for (int i = 0; i < W; ++i) z = __builtin_fmaf(w[i][e], x[t + i][e], z);
                 y[e] = pw::activate(z);
             }
-            tk::store(out + (token + t) * a.channels, pw::pack(y));
+            tk::store<true>(out + (token + t) * a.channels, pw::pack(y));
             // the inputs before the token behind the last
             if (a.after && token + t + 1 == a.tokens) {
 #pragma unroll
                 for (int i = 0; i < K; ++i)
-                    tk::store((value_t*)a.after + (p.sequence * K + i) * a.channels + p.channel, pw::pack(x[t + 1 + i]));
+                    tk::store<false>((value_t*)a.after + (p.sequence * K + i) * a.channels + p.channel, pw::pack(x[t + 1 + i]));
             }
         }
 #pragma unroll
@@ -193,7 +207,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
                 for (int i = 0; i < W; ++i) r = __builtin_fmaf(w[i][e], dz[K + t - i][e], r);
                 d[e] = r;
             }
-            if (at - K >= p.first) tk::store(dx + (at - K) * a.channels, pw::pack(d));
+            if (at - K >= p.first) tk::store<true>(dx + (at - K) * a.channels, pw::pack(d));
         }
 #pragma unroll
         for (int i = 0; i < K; ++i)
@@ -212,7 +226,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
 
 extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))) SPIO_KERNEL_NAME(const SpioConv1dArgs a) {
     const long long rows = a.sequences * ((a.tokens + a.slice - 1) / a.slice);
-    tk::column_sums({a.partials, a.sums, rows, a.channels, W, 1}, __builtin_amdgcn_workgroup_id_x());
+    tk::column_sums({a.partials, rows, a.channels, W, 1, a.dweight, a.dbias, nullptr}, __builtin_amdgcn_workgroup_id_x());
 }
 
 #else
@@ -238,9 +252,9 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
         for (int i = 0; i < W; ++i) z = __builtin_fmaf(w[i][e], x[i][e], z);
         y[e] = pw::activate(z);
     }
-    tk::store((value_t*)a.out + sequence * a.channels + channel, pw::pack(y));
+    tk::store<false>((value_t*)a.out + sequence * a.channels + channel, pw::pack(y));
 #pragma unroll
-    for (int i = 0; i < K; ++i) tk::store((value_t*)a.after + (sequence * K + i) * a.channels + channel, unit[i + 1]);
+    for (int i = 0; i < K; ++i) tk::store<false>((value_t*)a.after + (sequence * K + i) * a.channels + channel, unit[i + 1]);
 }
 
 #endif

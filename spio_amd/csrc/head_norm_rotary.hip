@@ -56,31 +56,31 @@ __device__ inline void cos_sin(float turn, float& c, float& s) {
     s = k & 2 ? -odd : odd;
 }
 
-// The two units of a lane, and the pairs in them
+// Stores go past the caches where the lanes of a head write whole lines at once (us with and without: 128 channels of
+// bfloat16, 4n 2048l 24q 8k 32 and 39 forward, 48 and 52 backward; 80 of float16, 2n 4097l, 32 and 29)
+constexpr bool ONCE = D / 2 * sizeof(value_t) % 128 == 0;
+
+// The two units of a lane (-1: none), and the first of the pairs in each of them that neighbours make (SPIO_INTERLEAVED:
+// four), or of the eight pairs that both make
 struct Place {
-    int unit[2];   // -1: none
-    int pair;      // of the first one: eight pairs from there on, or none (>= pairs)
+    int unit[2], pair[2];
     bool rotated;  // (SPIO_INTERLEAVED: the pairs before `pairs` are)
 };
 __device__ inline Place place(int lane, int pairs) {
     Place p;
-    if (SPIO_INTERLEAVED) {
-        p.unit[0] = 2 * lane;
-        p.pair = 8 * lane;
-        p.unit[1] = p.unit[0] + 1;
-        p.rotated = true;
-    } else {
-        const int half = pairs / 8;
-        p.rotated = lane < half;
-        p.unit[0] = p.rotated ? lane : 2 * half + 2 * (lane - half);
-        p.unit[1] = p.rotated ? lane + half : p.unit[0] + 1;
-        p.pair = 8 * lane;
-    }
+    // neighbouring lanes have neighbouring units
+    const int half = SPIO_INTERLEAVED ? 0 : pairs / 8;
+    p.rotated = SPIO_INTERLEAVED || lane < half;
+    p.unit[0] = lane < half ? lane : half + lane;
+    p.unit[1] = lane < half ? half + lane : PAIRED + lane;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (p.unit[i] >= UNITS) p.unit[i] = -1;
+    for (int i = 0; i < 2; ++i) {
+        p.pair[i] = SPIO_INTERLEAVED ? 4 * p.unit[i] : 8 * lane + 4 * i;
+        if (lane >= PAIRED || p.unit[i] >= UNITS) p.unit[i] = -1;
+    }
     return p;
 }
+__device__ inline int pair_of(const Place& p, int i) { return p.pair[i / 4] + i % 4; }
 
 // (v[0], v[1]) turned by the angles, or, `back`, by their negatives
 __device__ inline void rotate(float (&v)[2][8], const float (&c)[8], const float (&s)[8], bool rotated) {
@@ -172,16 +172,21 @@ __device__ inline void heads_of(const Rows& r, const Place& p, long long token, 
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (there && p.unit[i] >= 0)
-                    tk::store(r.out + (token * r.heads + head) * D + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
+                    tk::store<ONCE>(r.out + (token * r.heads + head) * D + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
         }
     }
 }
 
 __device__ inline void weights(const float* from, const Place& p, float (&w)[2][8]) {
+    typedef float float4_t __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[i][e] = from && p.unit[i] >= 0 ? from[p.unit[i] * 8 + e] : 0.f;
+        for (int e = 0; e < 8; e += 4) {
+            const float4_t v = from && p.unit[i] >= 0 ? *(const float4_t*)(from + p.unit[i] * 8 + e) : float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[i][e + k] = v[k];
+        }
 }
 
 }  // namespace
@@ -200,20 +205,20 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
     double frequency[8];  // turns a position
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        frequency[i] = p.rotated && p.pair + i < pairs ? a.frequencies[p.pair + i] * 0.15915494309189535 : 0.;
-    const long long groups = (long long)__builtin_amdgcn_grid_size_x() / LANES;
+        frequency[i] = p.rotated && pair_of(p, i) < pairs ? a.frequencies[pair_of(p, i)] * 0.15915494309189535 : 0.;
+    const unsigned groups = __builtin_amdgcn_grid_size_x() / LANES, items = (unsigned)(a.tokens * parts);  // (fewer than 2^31)
     // (a group's lanes stay together: they cross lanes for the norm)
-    for (long long item = ((long long)__builtin_amdgcn_workgroup_id_x() * 256 + tid) / LANES; item < a.tokens * parts; item += groups) {
-        const long long token = item / parts;
-        const int part = (int)(item % parts);
-        const long long at = token % a.position_tokens;
+    for (unsigned item = (__builtin_amdgcn_workgroup_id_x() * 256 + tid) / LANES; item < items; item += groups) {
+        const unsigned token = item / (unsigned)parts;
+        const int part = (int)(item % (unsigned)parts);
+        const unsigned at = token % (unsigned)a.position_tokens;
         const long long position = a.wide_positions ? ((const long long*)a.positions)[at] : ((const int*)a.positions)[at];
         float c[8], s[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const double turns = (double)position * frequency[i];
             cos_sin((float)(turns - __builtin_rint(turns)), c[i], s[i]);
-            if (p.rotated && p.pair + i < pairs) c[i] *= (float)a.scale, s[i] *= BACK ? -(float)a.scale : (float)a.scale;
+            if (p.rotated && pair_of(p, i) < pairs) c[i] *= (float)a.scale, s[i] *= BACK ? -(float)a.scale : (float)a.scale;
         }
         heads_of(q, p, token, part, parts, c, s, wq, (float)a.eps, dwq);
         heads_of(k, p, token, part, parts, c, s, wk, (float)a.eps, dwk);
@@ -244,7 +249,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
 
 extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))) SPIO_KERNEL_NAME(const SpioRotaryArgs a) {
     // (`parts` has the rows)
-    tk::column_sums({a.partials, a.sums, a.parts, D, 0, 2}, __builtin_amdgcn_workgroup_id_x());
+    tk::column_sums({a.partials, a.parts, D, 0, 2, nullptr, a.dq_weight, a.dk_weight}, __builtin_amdgcn_workgroup_id_x());
 }
 
 #endif

@@ -555,7 +555,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
         return;
     }
     const long long chunks = (a.tokens + a.chunk - 1) / a.chunk;
-    tk::column_sums({a.channel_sums, a.sums, a.sequences * chunks, a.channels, N, 2}, group - row_groups);
+    tk::column_sums({a.channel_sums, a.sequences * chunks, a.channels, N, 2, a.dA, a.dD, a.dbias}, group - row_groups);
 }
 
 #elif SPIO_MODE == 6 || SPIO_MODE == 7

@@ -18,7 +18,7 @@ struct SpioScanArgs {
     float* token_sums;    // [sequences][tokens][blocks of 64 channels][dB, dC]
     float* channel_sums;  // [sequences][chunks][states + 2][channels]: dA, dD, dbias
     void *dB, *dC;
-    float* sums;          // dA [channels][states], dD [channels], dbias [channels]
+    float *dA, *dD, *dbias;  // [channels][states], [channels], [channels]
     long long tokens, channels, chunk, sequences;
     long long u_row, delta_row, gate_row, b_row, c_row;
 };
@@ -28,7 +28,7 @@ struct SpioConv1dArgs {
     const void* before;                  // [sequences][width - 1][channels]: the inputs before the first token
     void *out, *after, *dx;
     float* partials;                     // [sequences][slices][width + 1][channels]: dweight, dbias
-    float* sums;                         // dweight [channels][width], dbias [channels]
+    float *dweight, *dbias;              // [channels][width], [channels]
     long long tokens, channels, sequences, slice, x_row;
 };
 
@@ -40,20 +40,12 @@ struct SpioRotaryArgs {
     const double* frequencies;               // [pairs]: radians a position
     void *q_out, *k_out;                     // (backward: the gradients of q and k)
     float* partials;                         // [workgroups][2][D]
-    float* sums;                             // [2][D]
+    float *dq_weight, *dk_weight;            // [D]
     long long tokens, q_heads, k_heads, parts, pairs;
     long long q_row, q_head, k_row, k_head;
     long long position_tokens;               // positions repeat after as many
     long long wide_positions;                // int64, else int32
     double eps, scale;
-};
-
-// The sums of `rows` rows of (turned + rest) * inner float32 values: columns [turned][inner] are stored as [inner][turned],
-// the rest behind them as they are.
-struct SpioColumnSums {
-    const float* from;
-    float* to;
-    long long rows, inner, turned, rest;
 };
 
 #endif

@@ -46,36 +46,51 @@ __device__ inline pw::Unit load(const value_t* p) {
     for (int i = 0; i < pw::QUADS; ++i) u.q[i] = ((const pw_uint4*)p)[i];
     return u;
 }
+// ONCE: past the caches, for whole lines that nobody reads soon
+template <bool ONCE>
 __device__ inline void store(value_t* p, const pw::Unit& u) {
 #pragma unroll
-    for (int i = 0; i < pw::QUADS; ++i) ((pw_uint4*)p)[i] = u.q[i];
+    for (int i = 0; i < pw::QUADS; ++i) {
+        if (ONCE)
+            __builtin_nontemporal_store(u.q[i], (pw_uint4*)p + i);
+        else
+            ((pw_uint4*)p)[i] = u.q[i];
+    }
 }
 __device__ inline void values(const pw::Unit& u, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = pw::value(u, e);
 }
 
-// Partial sums added up: workgroup `group` of 256 threads takes 16 columns, 16 lanes each of which have every 16th row; in
-// float64, since the rows may be many and their sums cancel.
-constexpr int SUM_COLUMNS = 16;
-__device__ inline void column_sums(const SpioColumnSums& a, long long group) {
-    __shared__ double parts[16][SUM_COLUMNS];
+// Sums over `rows` rows of float32 values [turned + rest][inner]: the first of them are stored as [inner][turned], the one or
+// two [inner] behind these to `first` and `second`.
+struct ColumnSums {
+    const float* from;
+    long long rows, inner, turned, rest;
+    float *to, *first, *second;
+};
+// Partial sums added up: workgroup `group` of 256 threads takes 32 columns (a line of a row), 8 lanes each of which have
+// every 8th row; in float64, since the rows may be many and their sums cancel.
+constexpr int SUM_COLUMNS = 32;
+__device__ inline void column_sums(const ColumnSums& a, long long group) {
+    constexpr int LANES = 256 / SUM_COLUMNS;
+    __shared__ double parts[LANES][SUM_COLUMNS];
     const int tid = (int)__builtin_amdgcn_workitem_id_x();
     const long long columns = (a.turned + a.rest) * a.inner;
     const long long column = group * SUM_COLUMNS + tid % SUM_COLUMNS;
     double sum = 0.;
     if (column < columns) {
 #pragma unroll 8
-        for (long long i = tid / SUM_COLUMNS; i < a.rows; i += 16) sum += a.from[i * columns + column];
+        for (long long i = tid / SUM_COLUMNS; i < a.rows; i += LANES) sum += a.from[i * columns + column];
     }
     parts[tid / SUM_COLUMNS][tid % SUM_COLUMNS] = sum;
     barrier();
     if (tid >= SUM_COLUMNS || column >= columns) return;
     sum = 0.;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += parts[i][tid];
+    for (int i = 0; i < LANES; ++i) sum += parts[i][tid];
     const long long k = column / a.inner, c = column % a.inner;
-    a.to[k < a.turned ? c * a.turned + k : column] = (float)sum;
+    *(k < a.turned ? a.to + c * a.turned + k : (k == a.turned ? a.first : a.second) + c) = (float)sum;
 }
 
 }  // namespace tk

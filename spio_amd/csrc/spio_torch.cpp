@@ -827,7 +827,7 @@ Key token_key(Kind kind, int64_t device, int64_t a, int64_t b, int64_t c = 0, in
 Tensor empty_of(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
     return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
 }
-constexpr int64_t SUM_COLUMNS = 16;  // of a workgroup that adds up partial sums
+constexpr int64_t SUM_COLUMNS = 32;  // of a workgroup that adds up partial sums
 
 // [.., values] as rows of values that are equally far apart, or a copy without gaps (functional/token_rows.py: rows_of)
 struct Rows {
@@ -900,7 +900,7 @@ PlanPtr conv1d_plan(Kind kind, const Conv1d& cv, const Tensor& x, const Tensor& 
 Tensor conv1d_forward(Conv1d& cv, const Tensor& x, const Tensor& weight, const Tensor& bias) {
     const auto plan = conv1d_plan(CONV1D, cv, x, weight);
     const Rows rows = rows_of(x, 8);
-    const Tensor w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias, before = whole(cv.before);
+    const Tensor w = whole(weight), b = whole(bias), before = whole(cv.before);
     const Tensor y = empty_of({cv.n, cv.l, cv.c}, x.scalar_type(), x);
     if (cv.keep_state) cv.after = empty_of({cv.n, cv.width - 1, cv.c}, x.scalar_type(), x);
     SpioConv1dArgs a = {};
@@ -940,23 +940,22 @@ struct Conv1dFunction : torch::autograd::Function<Conv1dFunction> {
         }
         RECORD_FUNCTION("spio::causal_conv1d_backward", tensors({dy, x, weight, bias}));
         const Rows rows = rows_of(x, 8);
-        const Tensor g = whole(dy), w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias, first = whole(before);
+        const Tensor g = whole(dy), w = whole(weight), b = whole(bias), first = whole(before);
         const auto main = conv1d_plan(CONV1D_BWD, cv, x, weight), second = conv1d_plan(CONV1D_SUMS, cv, x, weight);
         const Tensor dx = empty_of(x.sizes(), x.scalar_type(), x);
         SpioConv1dArgs a = {};
         a.slice = conv1d_slice(cv.l, cv.c, cv.n, true);
         const int64_t slices = divup(cv.l, a.slice);
         const Tensor partials = empty_1d(cv.n * slices * (cv.width + 1) * cv.c, at::kFloat, x);
-        const Tensor sums = empty_1d(cv.c * (cv.width + 1), at::kFloat, x);
+        const Tensor dweight = empty_of({cv.c, cv.width}, at::kFloat, x), dbias = empty_1d(cv.c, at::kFloat, x);
         a.x = ptr(rows.t), a.weight = ptr(w), a.bias = ptr(b), a.dy = ptr(g), a.before = ptr(first), a.dx = mut(dx);
-        a.partials = floats(partials), a.sums = floats(sums);
+        a.partials = floats(partials), a.dweight = floats(dweight), a.dbias = floats(dbias);
         a.tokens = cv.l, a.channels = cv.c, a.sequences = cv.n, a.x_row = rows.row;
         hipStream_t stream = c10::hip::getCurrentHIPStream(x.get_device());
         launch_structure(*main, divup(cv.n * slices * (cv.c / 8), 256), stream, &a);
         if (need_w || need_b) launch_structure(*second, divup((cv.width + 1) * cv.c, SUM_COLUMNS), stream, &a);
         at::AutoDispatchBelowADInplaceOrView below;
-        return {need_x ? dx : Tensor(), need_w ? typed(sums.narrow(0, 0, cv.c * cv.width).view({cv.c, cv.width}), v[6]) : Tensor(),
-                need_b ? typed(sums.narrow(0, cv.c * cv.width, cv.c), v[7]) : Tensor(), Tensor()};
+        return {need_x ? dx : Tensor(), need_w ? typed(dweight, v[6]) : Tensor(), need_b ? typed(dbias, v[7]) : Tensor(), Tensor()};
     }
 };
 
@@ -1074,14 +1073,14 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
         const Tensor du = empty_of(tensor, u.scalar_type(), u), ddelta = empty_of(tensor, u.scalar_type(), u);
         const Tensor dgate = t[6].defined() ? empty_of(tensor, u.scalar_type(), u) : Tensor();
         const Tensor dB = empty_of(row, u.scalar_type(), u), dC = empty_of(row, u.scalar_type(), u);
-        const Tensor sums = empty_1d(sc.c * (sc.s + 2), at::kFloat, u);
-        const Tensor token_sums = empty_1d(sc.n * sc.l * blocks * 2 * sc.s, at::kFloat, u);
-        const Tensor channel_sums = empty_1d(sc.n * chunks * (sc.s + 2) * sc.c, at::kFloat, u);
-        Tensor ends;
-        if (chunks > 1) ends = empty_1d(sc.n * chunks * (sc.s + 1) * sc.c, at::kFloat, u);
-        in.a.dout = ptr(g), in.a.kept = floats(k), in.a.ends = floats(ends), in.a.du = mut(du), in.a.ddelta = mut(ddelta);
-        in.a.dgate = mut(dgate), in.a.dB = mut(dB), in.a.dC = mut(dC), in.a.sums = floats(sums);
-        in.a.token_sums = floats(token_sums), in.a.channel_sums = floats(channel_sums);
+        const Tensor dA = empty_of(rate, at::kFloat, u), dD = empty_1d(sc.c, at::kFloat, u), dbias = empty_1d(sc.c, at::kFloat, u);
+        const int64_t of_tokens = sc.n * sc.l * blocks * 2 * sc.s, of_channels = sc.n * chunks * (sc.s + 2) * sc.c,
+                      of_ends = chunks > 1 ? sc.n * chunks * (sc.s + 1) * sc.c : 0;
+        const Tensor workspace = empty_1d(of_tokens + of_channels + of_ends, at::kFloat, u);
+        in.a.dout = ptr(g), in.a.kept = floats(k), in.a.du = mut(du), in.a.ddelta = mut(ddelta);
+        in.a.dgate = mut(dgate), in.a.dB = mut(dB), in.a.dC = mut(dC), in.a.dA = floats(dA), in.a.dD = floats(dD), in.a.dbias = floats(dbias);
+        in.a.token_sums = floats(workspace), in.a.channel_sums = in.a.token_sums + of_tokens;
+        in.a.ends = in.a.channel_sums + of_channels;
         if (chunks > 1) {
             launch_structure(*scan_plan(SCAN_ENDS_BWD, sc, u, t[6].defined()), grid, stream, &in.a);
             launch_structure(*scan_plan(SCAN_JOIN_BWD, sc, u, false), sc.n * sc.s * blocks, stream, &in.a);
@@ -1090,10 +1089,9 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
         launch_structure(*scan_plan(SCAN_SUMS, sc, u, false), divup(sc.n * sc.l * 2 * sc.s, 256) + divup((sc.s + 2) * sc.c, SUM_COLUMNS),
                          stream, &in.a);
         at::AutoDispatchBelowADInplaceOrView below;
-        auto sum = [&](int i, int64_t from, int64_t count) { return typed(sums.narrow(0, from, count), v[5 + i]); };
-        return {needs[0] ? du : Tensor(), needs[1] ? ddelta : Tensor(), needs[2] ? sum(2, 0, sc.c * sc.s).view(rate) : Tensor(),
-                needs[3] ? dB : Tensor(), needs[4] ? dC : Tensor(), needs[5] ? sum(5, sc.c * sc.s, sc.c) : Tensor(),
-                needs[6] ? dgate : Tensor(), needs[7] ? sum(7, sc.c * (sc.s + 1), sc.c) : Tensor(), Tensor()};
+        return {needs[0] ? du : Tensor(), needs[1] ? ddelta : Tensor(), needs[2] ? typed(dA, v[7]) : Tensor(),
+                needs[3] ? dB : Tensor(), needs[4] ? dC : Tensor(), needs[5] ? typed(dD, v[10]) : Tensor(),
+                needs[6] ? dgate : Tensor(), needs[7] ? typed(dbias, v[12]) : Tensor(), Tensor()};
     }
 };
 
@@ -1107,7 +1105,7 @@ int64_t rotary_lanes(int64_t head) {
 }
 int64_t rotary_parts(int64_t tokens, int64_t heads, int64_t head) {
     const int64_t waves = divup(tokens * rotary_lanes(head), 64);
-    return std::max(int64_t(1), std::min(divup(heads, 2), divup(2048, waves)));
+    return std::min(divup(heads, 2), std::max(divup(heads, 8), divup(4096, waves)));
 }
 int64_t rotary_grid(int64_t tokens, int64_t parts, int64_t head, bool summed) {
     const int64_t grid = divup(tokens * parts * rotary_lanes(head), ROTARY_THREADS);
@@ -1148,7 +1146,7 @@ Heads heads_of(const Tensor& t) {
 }
 variable_list rotary_forward(const Rotary& r, const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight) {
     const Heads qh = heads_of(q), kh = heads_of(k);
-    const Tensor wq = to_float_1d(q_weight), wk = to_float_1d(k_weight);
+    const Tensor wq = whole(to_float_1d(q_weight)), wk = whole(to_float_1d(k_weight));
     const Tensor qo = empty_of(r.shape(r.q_heads), q.scalar_type(), q), ko = empty_of(r.shape(r.k_heads), k.scalar_type(), k);
     SpioRotaryArgs a = r.args();
     a.q = ptr(qh.t), a.q_row = qh.row, a.q_head = qh.head, a.k = ptr(kh.t), a.k_row = kh.row, a.k_head = kh.head;
@@ -1203,20 +1201,20 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
             return {from_py(out, 0), from_py(out, 1), from_py(out, 2), from_py(out, 3), Tensor()};
         }
         RECORD_FUNCTION("spio::head_norm_rotary_backward", tensors({gq, gk, q, k, wq, wk}));
-        const Tensor gqc = whole(gq), gkc = whole(gk), wqf = to_float_1d(wq), wkf = to_float_1d(wk);
+        const Tensor gqc = whole(gq), gkc = whole(gk), wqf = whole(to_float_1d(wq)), wkf = whole(to_float_1d(wk));
         const Tensor dq = empty_of(gq.sizes(), type(6), gq), dk = empty_of(gk.sizes(), type(6), gk);
         SpioRotaryArgs a = r.args();
         const int64_t grid = rotary_grid(r.tokens(), a.parts, r.d, norm);
         Heads qh, kh;
-        Tensor partials, sums;
+        Tensor partials, dwq, dwk;
         if (norm) {
             qh = heads_of(q), kh = heads_of(k);
             a.q = ptr(qh.t), a.q_row = qh.row, a.q_head = qh.head, a.k = ptr(kh.t), a.k_row = kh.row, a.k_head = kh.head;
             partials = empty_1d(grid * 2 * r.d, at::kFloat, gq);
-            sums = empty_of({2, r.d}, at::kFloat, gq);
+            dwq = empty_1d(r.d, at::kFloat, gq), dwk = empty_1d(r.d, at::kFloat, gq);
         }
         a.dq = ptr(gqc), a.dk = ptr(gkc), a.q_weight = floats(wqf), a.k_weight = floats(wkf), a.q_out = mut(dq), a.k_out = mut(dk);
-        a.partials = floats(partials), a.sums = floats(sums);
+        a.partials = floats(partials), a.dq_weight = floats(dwq), a.dk_weight = floats(dwk);
         hipStream_t stream = c10::hip::getCurrentHIPStream(gq.get_device());
         launch_structure(*rotary_plan(ROTARY_BWD, r, gq, norm), grid, stream, &a);
         if (needs[2] || needs[3]) {
@@ -1224,8 +1222,8 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
             launch_structure(*rotary_plan(ROTARY_SUMS, r, gq, norm), divup(2 * r.d, SUM_COLUMNS), stream, &a);
         }
         at::AutoDispatchBelowADInplaceOrView below;
-        return {needs[0] ? dq : Tensor(), needs[1] ? dk : Tensor(), needs[2] ? typed(sums.select(0, 0), v[7]) : Tensor(),
-                needs[3] ? typed(sums.select(0, 1), v[8]) : Tensor(), Tensor()};
+        return {needs[0] ? dq : Tensor(), needs[1] ? dk : Tensor(), needs[2] ? typed(dwq, v[7]) : Tensor(),
+                needs[3] ? typed(dwk, v[8]) : Tensor(), Tensor()};
     }
 };
 
@@ -1610,7 +1608,7 @@ PyObject* causal_conv1d_step(PyObject*, PyObject* const* args, Py_ssize_t nargs,
         RECORD_FUNCTION("spio::causal_conv1d_step", tensors({x, cv.before, weight, bias}));
         at::AutoDispatchBelowADInplaceOrView below;
         const Rows rows = rows_of(x, 8);
-        const Tensor w = weight.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
+        const Tensor w = whole(weight), b = whole(bias);
         const auto plan = conv1d_plan(CONV1D_STEP, cv, x, weight);
         y = empty_of({cv.n, cv.c}, x.scalar_type(), x);
         SpioConv1dArgs a = {};
@@ -1720,7 +1718,8 @@ PyObject* head_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs, P
     if (!is_plain(q) || q.dim() != 4 || dtype_number(q) < 0 || !is_plain(k) || k.dim() != 4) return not_implemented();
     r.n = q.size(0), r.l = q.size(1), r.q_heads = q.size(2), r.k_heads = k.size(2), r.d = q.size(3);
     const int64_t pairs = is_plain(r.frequencies) && r.frequencies.dim() == 1 ? r.frequencies.size(0) : 0;
-    if (q.numel() == 0 || k.numel() == 0 || !fits(k, q, r.shape(r.k_heads), true) || r.d % 8 || r.d > ROTARY_MAX_HEAD ||
+    if (q.numel() == 0 || k.numel() == 0 || r.tokens() * std::max(r.q_heads, r.k_heads) >= int64_t(1) << 31 ||
+        !fits(k, q, r.shape(r.k_heads), true) || r.d % 8 || r.d > ROTARY_MAX_HEAD ||
         wq.defined() != wk.defined() || !absent_or_fits(wq, q, {r.d}, false) || !absent_or_fits(wk, q, {r.d}, false) ||
         !(r.eps > 0) || r.eps > std::numeric_limits<double>::max() || !std::isfinite(r.scale) || pairs < 1 || 2 * pairs > r.d ||
         (!r.interleaved && pairs % 8) || r.frequencies.scalar_type() != at::kDouble || r.frequencies.device() != q.device() ||

@@ -32,7 +32,7 @@ from .group_norm_2d_function import aligned, refuse_forward_derivatives
 from .token_rows import check_out_state, check_parameters, check_tokens, refuse_state_gradients, require_gpu, rows_of
 
 STRUCT = "SpioConv1dArgs"
-SUM_COLUMNS = 16
+SUM_COLUMNS = 32  # of a workgroup that adds up partial sums
 
 
 def _check(what, inputs, dims, weight, bias, activation, state):
@@ -48,11 +48,11 @@ def _check(what, inputs, dims, weight, bias, activation, state):
 
 
 def _filters(weight, bias):
-    """Weight and bias as the kernels read them: one type, no gaps."""
+    """Weight and bias as the kernels read them: one type, no gaps, on 16 bytes."""
     weight, bias = weight.detach(), None if bias is None else bias.detach()
     if weight.dtype not in DTYPES or (bias is not None and bias.dtype != weight.dtype):
         weight, bias = weight.float(), None if bias is None else bias.float()
-    return weight.contiguous(), None if bias is None else bias.contiguous()
+    return aligned(weight.contiguous()), None if bias is None else aligned(bias.contiguous())
 
 
 def _params(inputs, weight, activation):
@@ -115,7 +115,8 @@ def causal_conv1d_backward(
     partials = torch.empty((n * slices * (width + 1) * c,), dtype=torch.float32, device=x.device)
     params = _params(x, weight, activation)
     before = None if initial_state is None else aligned(initial_state.contiguous())
-    arguments = Arguments(STRUCT, x=x, weight=weight, bias=bias, dy=dy, before=before, dx=dx, partials=partials, sums=sums,
+    arguments = Arguments(STRUCT, x=x, weight=weight, bias=bias, dy=dy, before=before, dx=dx, partials=partials, dweight=sums,
+                          dbias=sums[width * c :],
                           tokens=l, channels=c, sequences=n, slice=size, x_row=row)  # fmt: skip
     main = causal_conv1d_bwd_kernel_factory.get_kernel(params, x.device)
     main.launch_structure(divup(n * slices * (c // 8), 256), arguments)

@@ -33,7 +33,7 @@ from .group_norm_2d_function import aligned, refuse_forward_derivatives
 from .token_rows import check_parameters, check_tokens, require_gpu, vector
 
 STRUCT = "SpioRotaryArgs"
-SUM_COLUMNS = 16
+SUM_COLUMNS = 32  # of a workgroup that adds up partial sums
 
 
 def _check(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, scale):
@@ -54,6 +54,7 @@ def _check(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, s
     assert positions.dtype in (torch.int32, torch.int64), "positions are int32 or int64"
     n, l = q.shape[:2]
     assert tuple(positions.shape) in ((l,), (n, l)), f"positions must be {[l]} or {[n, l]}"
+    assert n * l * max(q.shape[2], k.shape[2]) < 1 << 31, "fewer than 2^31 heads"
     assert positions.device == q.device == frequencies.device, "positions and frequencies must be on the queries' device"
 
 
@@ -78,6 +79,10 @@ def _fields(q, k, positions, frequencies, eps, scale):
                 position_tokens=positions.numel(), eps=eps, scale=scale)  # fmt: skip
 
 
+def _weight(t):
+    return None if t is None else aligned(vector(t))
+
+
 def _params(q, norm, interleaved):
     return HeadNormRotaryParams(q.shape[3], DTYPES[q.dtype], norm, bool(interleaved))
 
@@ -97,7 +102,7 @@ def head_norm_rotary_forward(
     (qx, q_row, q_head), (kx, k_row, k_head) = _heads_of(q), _heads_of(k)
     parts = parts_of(tokens, heads, d)
     arguments = Arguments(STRUCT, **_fields(q, k, positions, frequencies, eps, scale), q=qx, k=kx, q_row=q_row, q_head=q_head,
-                          k_row=k_row, k_head=k_head, q_weight=vector(q_weight), k_weight=vector(k_weight), q_out=outputs[0],
+                          k_row=k_row, k_head=k_head, q_weight=_weight(q_weight), k_weight=_weight(k_weight), q_out=outputs[0],
                           k_out=outputs[1], parts=parts)  # fmt: skip
     kernel = head_norm_rotary_kernel_factory.get_kernel(_params(q, q_weight is not None, interleaved), q.device)
     kernel.launch_structure(grid_of(tokens, parts, d, False), arguments)
@@ -135,9 +140,9 @@ def head_norm_rotary_backward(
         for name, t in (("q", q), ("k", k)):
             fields[name], fields[name + "_row"], fields[name + "_head"] = _heads_of(t)
         fields["partials"] = torch.empty((grid, 2, d), dtype=torch.float32, device=grad_q.device)
-        fields["sums"] = sums
-    fields.update(dq=aligned(grad_q.contiguous()), dk=aligned(grad_k.contiguous()), q_weight=vector(q_weight),
-                  k_weight=vector(k_weight), q_out=outputs[0], k_out=outputs[1])  # fmt: skip
+        fields["dq_weight"], fields["dk_weight"] = sums
+    fields.update(dq=aligned(grad_q.contiguous()), dk=aligned(grad_k.contiguous()), q_weight=_weight(q_weight),
+                  k_weight=_weight(k_weight), q_out=outputs[0], k_out=outputs[1])  # fmt: skip
     params = _params(grad_q, norm, interleaved)
     main = head_norm_rotary_bwd_kernel_factory.get_kernel(params, grad_q.device)
     main.launch_structure(grid, Arguments(STRUCT, **fields, parts=parts))

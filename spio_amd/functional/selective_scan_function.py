@@ -46,7 +46,7 @@ from .token_rows import (
 )
 
 STRUCT = "SpioScanArgs"
-SUM_COLUMNS = 16
+SUM_COLUMNS = 32  # of a workgroup that adds up partial sums
 
 
 def _check(what, inputs, dims, delta, A, B, C, D, gate, delta_bias, state):
@@ -154,7 +154,7 @@ def selective_scan_backward(
         bias=vector(delta_bias), kept=kept.contiguous(), ends=torch.empty((n, chunks, s + 1, c), **f32) if chunks > 1 else None,
         du=du, ddelta=ddelta, dgate=dgate if gate is not None else None,
         token_sums=torch.empty((n, l, blocks, 2 * s), **f32), channel_sums=torch.empty((n, chunks, s + 2, c), **f32),
-        dB=dB, dC=dC, sums=sums, tokens=l, channels=c, chunk=chunk, sequences=n)  # fmt: skip
+        dB=dB, dC=dC, dA=sums, dD=sums[c * s :], dbias=sums[c * (s + 1) :], tokens=l, channels=c, chunk=chunk, sequences=n)  # fmt: skip
     params = SelectiveScanParams(s, dtype, gated, softplus)
     if chunks > 1:
         selective_scan_ends_bwd_kernel_factory.get_kernel(params, inputs.device).launch_structure(n * chunks * blocks, arguments)

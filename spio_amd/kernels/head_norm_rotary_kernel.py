@@ -26,9 +26,11 @@ def lanes_of(head: int) -> int:
 
 
 def parts_of(tokens: int, heads: int, head: int) -> int:
-    """Parts that the heads of a token are split into: lanes that share a token's cosines take every parts-th head."""
+    """Parts that the heads of a token are split into: lanes that share a token's cosines take every parts-th head.  About
+    eight heads a lane, fewer where waves are few (us with 1, 2, 4, 8 and 16 parts, forward: 2n 4097l 16 heads of 80
+    channels 39, 32, 29, 31, 38; 1n 16385l 32q 8k 128d 90, 80, 77, 89, 113)."""
     waves = divup(tokens * lanes_of(head), 64)
-    return max(1, min(divup(heads, 2), divup(2048, waves)))
+    return min(divup(heads, 2), max(divup(heads, 8), divup(4096, waves)))
 
 
 def grid_of(tokens: int, parts: int, head: int, summed: bool) -> int:
