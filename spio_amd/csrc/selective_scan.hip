@@ -155,17 +155,17 @@ __device__ inline void request(Tile& tile, const Args& a, const Place& p, int to
     if (B) request_rows(tile.B, a.B, a.b_row, row0, p, token);
     if (C) request_rows(tile.C, a.C, a.c_row, row0, p, token);
 }
-// B and C of the tile in LDS, [T][2][NP]
+// B and C of the tile in LDS, [T][2][NP]; zeros from token `count` on, so that nothing that is not finite is multiplied there
 template <bool B, bool C>
-__device__ inline void stage(const Tile& tile, float* lds) {
+__device__ inline void stage(const Tile& tile, int count, float* lds) {
     const int lane = (int)__builtin_amdgcn_workitem_id_x();
     barrier();
 #pragma unroll
     for (int i = 0; i < STAGED; ++i) {
         const int e = i * 64 + lane, t = e / N, s = e % N;
         if (e >= T * N) break;
-        if (B) lds[t * 2 * NP + s] = (float)tile.B[i];
-        if (C) lds[(t * 2 + 1) * NP + s] = (float)tile.C[i];
+        if (B) lds[t * 2 * NP + s] = t < count ? (float)tile.B[i] : 0.f;
+        if (C) lds[(t * 2 + 1) * NP + s] = t < count ? (float)tile.C[i] : 0.f;
     }
     if (N % 2 && lane < 2 * T) lds[lane * NP + N] = 0.f;  // (read where the states are halved)
     barrier();
@@ -224,7 +224,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
     const long long tiles = (a.tokens + T - 1) / T;
     const unsigned lane_bytes = p.live ? (unsigned)p.channel * SIZE : pw::OOB;
     for (int token = p.first; token < p.last; token += T) {
-        stage<true, OUT>(tile, lds);
+        stage<true, OUT>(tile, p.last - token, lds);
         float u[T], dl[T], gate[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
@@ -289,7 +289,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
 #pragma unroll
     for (int s = 0; s < N; ++s) r[s] = 0.f;
     for (; token >= p.first; token -= T) {
-        stage<false, true>(tile, lds);
+        stage<false, true>(tile, p.last - token, lds);
         float dy[T], dl[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
@@ -388,10 +388,18 @@ SPIO_KERNEL_NAME(const Args a) {
     // (a state behind the last one, where they are odd: rate, B and C of zero)
     auto state = [&](int i) { return half * H + i < N ? half * H + i : N - 1; };
     auto there = [&](int i) { return half * H + i < N; };
-    // bytes from a row of channels [i] of a [N][channels] array to the lane's state i
-    auto offset = [&](int c, int i) {
-        const int skipped = N % 2 && i == H - 1 ? half * (N - H) : half * H;
-        return (unsigned)(skipped * (int)a.channels + channel[c]) * 4u;
+    // Rows of states [N][channels]: bytes from row i to the lane's state i of a channel.  What is not there, a state behind the
+    // last one or a channel, lies behind the end, where zeros are loaded.
+    unsigned offset[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int at = p.block * 64 + c * 32 + j;
+        offset[c] = at < (int)a.channels ? (unsigned)(half * H * (int)a.channels + at) * 4u : pw::OOB;
+    }
+    const int row_bytes = (int)a.channels * 4;
+    auto states = [&](const float* rows) { return pw::buffer(rows, N * (unsigned)row_bytes); };
+    auto load_state = [&](pw_rsrc rs, int c, int i) {
+        return pw::as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, (int)offset[c], i * row_bytes, 0));
     };
     float A2[2][H], r[2][H], dA[2][H];
 #pragma unroll
@@ -402,11 +410,11 @@ SPIO_KERNEL_NAME(const Args a) {
             r[c][i] = dA[c][i] = 0.f;
         }
     if (p.chunks > 1) {  // what the chunks behind this one add
-        const float* start = a.ends + (p.sequence * p.chunks + p.chunk) * (N + 1) * a.channels;
+        const pw_rsrc start = states(a.ends + (p.sequence * p.chunks + p.chunk) * (N + 1) * a.channels);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < H; ++i) r[c][i] = there(i) ? at(start + i * a.channels, offset(c, i)) : 0.f;
+            for (int i = 0; i < H; ++i) r[c][i] = load_state(start, c, i);
     }
     const float bias = a.bias ? a.bias[p.loaded] : 0.f;
     const float D = a.D ? a.D[p.loaded] : 0.f;
@@ -417,11 +425,11 @@ SPIO_KERNEL_NAME(const Args a) {
     const unsigned sum_bytes = value < 0 || sum_state >= N ? pw::OOB : (unsigned)(p.block * M + value / H * N + sum_state) * 4u;
     float next[2][H];  // states before the tile that comes next
     auto request_states = [&](int token) {
-        const float* kept = a.kept + (p.sequence * tiles + token / T) * N * a.channels;
+        const pw_rsrc kept = states(a.kept + (p.sequence * tiles + token / T) * N * a.channels);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < H; ++i) next[c][i] = at(kept + i * a.channels, offset(c, i));
+            for (int i = 0; i < H; ++i) next[c][i] = load_state(kept, c, i);
     };
     request_states(token);
     for (; token >= p.first; token -= T) {
@@ -430,11 +438,11 @@ SPIO_KERNEL_NAME(const Args a) {
         for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < H; ++i) before[c][i] = next[c][i];
-        stage<true, true>(tile, lds);
+        stage<true, true>(tile, p.last - token, lds);
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             const bool counts = token + t < p.last && p.live;
-            const float raw = (float)tile.delta[t] + bias;
+            const float raw = counts ? (float)tile.delta[t] + bias : 0.f;
             const float dout = counts ? (float)tile.dout[t] : 0.f;
             const float u = counts ? (float)tile.u[t] : 0.f;
             const float dl = counts ? time_step(raw) : 0.f;
@@ -443,7 +451,7 @@ SPIO_KERNEL_NAME(const Args a) {
             own[t][U][lane] = u;
             own[t][SLOPE][lane] = SOFTPLUS ? pw::sigmoid(raw) : 1.f;
             if (GATE) {
-                const float gate = (float)tile.gate[t], s = pw::sigmoid(gate), v = gate * s;
+                const float gate = counts ? (float)tile.gate[t] : 0.f, s = pw::sigmoid(gate), v = gate * s;
                 own[t][DY][lane] = dout * v;
                 own[t][DGATE][lane] = dout * __builtin_fmaf(v, 1.f - s, s);
             } else {
@@ -520,11 +528,12 @@ SPIO_KERNEL_NAME(const Args a) {
         }
     }
     float* sums = a.channel_sums + (p.sequence * p.chunks + p.chunk) * (N + 2) * a.channels;
+    const pw_rsrc to_dA = states(sums);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < H; ++i)
-            if (there(i) && p.block * 64 + c * 32 + j < (int)a.channels) *(float*)((char*)(sums + i * a.channels) + offset(c, i)) = dA[c][i];
+            __builtin_amdgcn_raw_buffer_store_b32(pw::as_bits(dA[c][i]), to_dA, (int)offset[c], i * row_bytes, 0);
     if (!p.live) return;
     sums[N * a.channels + p.channel] = dD;
     sums[(N + 1) * a.channels + p.channel] = dbias;

@@ -133,6 +133,7 @@ def _backward_fake(grad_output, inputs, weight, bias, activation, initial_state)
 
 def causal_conv1d_gradients(grad_output, inputs, weight, bias, activation, initial_state, needs_input, needs_weight, needs_bias):
     """Gradients of causal_conv1d in the types of the tensors they belong to, None where not needed."""
+    refuse_forward_derivatives(grad_output, inputs, weight, bias)
     dx, sums = causal_conv1d_backward(grad_output, inputs, weight, bias, activation, initial_state)
     return (
         dx if needs_input else None,

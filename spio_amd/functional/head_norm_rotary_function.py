@@ -162,6 +162,7 @@ def _backward_fake(grad_q, grad_k, q, k, q_weight, k_weight, positions, frequenc
 def head_norm_rotary_gradients(grad_q, grad_k, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, scale, needs):
     """Gradients for q, k, q_weight and k_weight in the types of these, None where not needed.  Without a norm q and k are
     not needed."""
+    refuse_forward_derivatives(grad_q, grad_k, q, k, q_weight, k_weight)
     norm = q_weight is not None
     dq, dk, sums = head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved,
                                              scale)  # fmt: skip
@@ -266,7 +267,7 @@ def rotary_frequencies(
         frequencies = base**-exponents
         turns = frequencies * (trained_tokens / (2 * math.pi))
         stay = ((turns - slow_turns) / (fast_turns - slow_turns)).clamp(0, 1)
-        frequencies = frequencies * stay + frequencies / factor * (1 - stay)
+        frequencies = frequencies * (stay + (1 - stay) / factor)
     else:
         raise ValueError(f"method must be 'linear', 'base' or 'ramp', not {method!r}")
     return frequencies.to(device)

@@ -178,6 +178,7 @@ def _backward_fake(grad_output, inputs, delta, A, B, C, D, gate, delta_bias, del
 def selective_scan_gradients(grad_output, inputs, delta, A, B, C, D, gate, delta_bias, delta_softplus, kept, needs):
     """Gradients of selective_scan for inputs, delta, A, B, C, D, gate and delta_bias in the types of these, None where
     not needed."""
+    refuse_forward_derivatives(grad_output, inputs, delta, A, B, C, D, gate, delta_bias)
     du, ddelta, dB, dC, dgate, sums = selective_scan_backward(grad_output, inputs, delta, A, B, C, D, gate, delta_bias,
                                                               delta_softplus, kept)  # fmt: skip
     c, s = A.shape

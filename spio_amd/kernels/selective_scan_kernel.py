@@ -19,8 +19,8 @@ LANES = 64  # channels of a workgroup
 def tile_tokens(states: int) -> int:
     """Tokens of a tile: those whose states the backward pass holds in registers at once, and the distance of the states
     that the forward pass keeps for it.  Longer tiles keep less (4n 2048l 2048c with 16 states, forward: 98 us with 8 tokens,
-    124 with 4), but 16 states of five tokens and more have no room in half a SIMD's registers (backward: 233 us with 4
-    tokens, 254 with 5, 397 with 6, 542 with 8)."""
+    124 with 4), but 16 states of five tokens and more have no room in half a SIMD's registers (backward: 239 us with 4
+    tokens, 275 with 5, 397 with 6, 542 with 8)."""
     return 8 if states <= 8 else 4
 
 
@@ -60,8 +60,8 @@ class SelectiveScanParams:
 
 @dataclass(frozen=True)
 class SelectiveScanConfig:
-    """Tokens of a tile, and how many of its last ones the backward pass holds the decays of: one where the registers have
-    room for it (16 states: 217 us, without 231, with two 237)."""
+    """Tokens of a tile, and how many of its last ones the backward pass holds the decays of, as many as the registers have
+    room for (4n 2048l 2048c with 16 states: none 239 us, one 238, two 231; a third is kept in memory, 480)."""
 
     tile: int
     held: int = 0
@@ -83,7 +83,7 @@ def _factory(name, mode, threads):
         SelectiveScanConfig,
         None,
         kernel_name=name,
-        configs=lambda params, device_attr=None: [SelectiveScanConfig(tile_tokens(params.states), int(8 < params.states <= 16))],
+        configs=lambda params, device_attr=None: [SelectiveScanConfig(tile_tokens(params.states), 2 * (8 < params.states <= 16))],
         kernel_spec=_spec(mode, threads),
         args_checker=None,
     )
