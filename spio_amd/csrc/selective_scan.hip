@@ -41,7 +41,6 @@ constexpr int NP = (N + 3) / 4 * 4;        // states of a row in LDS, zeros behi
 constexpr int M = 2 * N;                   // a token's B and C
 constexpr int STAGED = (T * N + 63) / 64;  // of a tile's B, a lane's, and of its C
 constexpr bool GATE = SPIO_GATE, SOFTPLUS = SPIO_SOFTPLUS, KEEP = SPIO_KEEP;
-constexpr int STATES_AT = T > 2 ? T - 3 : 0;  // token behind which there are registers for the states of the next tile
 constexpr int HELD = SPIO_HELD;            // last tokens of a tile whose decays the backward pass holds, the others are taken again
 
 typedef SpioScanArgs Args;
@@ -445,7 +444,9 @@ SPIO_KERNEL_NAME(const Args a) {
             const float raw = counts ? (float)tile.delta[t] + bias : 0.f;
             const float dout = counts ? (float)tile.dout[t] : 0.f;
             const float u = counts ? (float)tile.u[t] : 0.f;
-            const float dl = counts ? time_step(raw) : 0.f;
+            float dl = time_step(raw);
+            asm("" : "+v"(dl));  // (not a branch around it)
+            dl = counts ? dl : 0.f;
             own[t][DL][lane] = dl;
             own[t][X][lane] = dl * u;
             own[t][U][lane] = u;
@@ -464,16 +465,15 @@ SPIO_KERNEL_NAME(const Args a) {
         const int count = p.last - token < T ? p.last - token : T;
         const pw_rsrc token_sums = pw::buffer(a.token_sums + (p.sequence * a.tokens + token) * blocks * M,
                                               (unsigned)count * (unsigned)blocks * M * 4u);
+        if (token > p.first) request<true, true, true, true>(tile, a, p, token - T);
         float y[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            __builtin_amdgcn_sched_barrier(0);
             float B[H], C[H], part[2];
             half_row(lds, t, 0, half, B);
             half_row(lds, t, 1, half, C);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                __builtin_amdgcn_sched_barrier(0);
                 const float dl = own[t][DL][c * 32 + j], x = own[t][X][c * 32 + j];
                 part[c] = 0.f;
 #pragma unroll
@@ -488,16 +488,13 @@ SPIO_KERNEL_NAME(const Args a) {
         }
 #pragma unroll
         for (int t = T - 1; t >= 0; --t) {
-            __builtin_amdgcn_sched_barrier(0);
             // (once the registers of the last token are free)
-            if (t == T - 2 && token > p.first) request<true, true, true, true>(tile, a, p, token - T);
-            if (t == STATES_AT && token > p.first) request_states(token - T);
+            if (t == (T > 1 ? T - 2 : 0) && token > p.first) request_states(token - T);
             float B[H], C[H], sums[2 * H], gB[2] = {}, gq[2] = {};
             half_row(lds, t, 0, half, B);
             half_row(lds, t, 1, half, C);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                __builtin_amdgcn_sched_barrier(0);
                 const float x = own[t][X][c * 32 + j], dy = own[t][DY][c * 32 + j];
                 float dl = own[t][DL][c * 32 + j];
                 if (t < T - HELD) asm("" : "+v"(dl));  // (or the exponentials would be held)

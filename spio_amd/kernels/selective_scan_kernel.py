@@ -61,7 +61,7 @@ class SelectiveScanParams:
 @dataclass(frozen=True)
 class SelectiveScanConfig:
     """Tokens of a tile, and how many of its last ones the backward pass holds the decays of, as many as the registers have
-    room for (4n 2048l 2048c with 16 states: none 239 us, one 238, two 231; a third is kept in memory, 480)."""
+    room for (4n 2048l 2048c with 16 states: none 233 us, two 224, three 215, four, of which some are kept in memory, 238)."""
 
     tile: int
     held: int = 0
@@ -83,7 +83,7 @@ def _factory(name, mode, threads):
         SelectiveScanConfig,
         None,
         kernel_name=name,
-        configs=lambda params, device_attr=None: [SelectiveScanConfig(tile_tokens(params.states), 2 * (8 < params.states <= 16))],
+        configs=lambda params, device_attr=None: [SelectiveScanConfig(tile_tokens(params.states), (3 - params.states % 2) * (8 < params.states <= 16))],
         kernel_spec=_spec(mode, threads),
         args_checker=None,
     )
