@@ -33,6 +33,9 @@ constexpr int LANES = PAIRED <= 1 ? 1 : PAIRED <= 2 ? 2 : PAIRED <= 4 ? 4 : PAIR
 constexpr int GROUPS = 256 / LANES;      // of a workgroup
 constexpr int U = SPIO_HEADS;            // heads requested at once
 constexpr bool BACK = SPIO_MODE == 1;
+// Whether the first heads of a token are requested before its angles are computed: a backward pass with norms has no registers
+// for that
+constexpr bool AHEAD = !(BACK && SPIO_NORM);
 static_assert(D % 8 == 0 && D <= 256, "heads of up to 256 channels, whole units");
 
 // cos and sin of a fraction of a turn in [-1/2, 1/2]: the nearest quarter turn, and the Taylor series of what is left, at
@@ -102,78 +105,90 @@ struct Rows {
     int heads;
 };
 
-// The heads `part`, `part + parts`, ... of a token.
-__device__ inline void heads_of(const Rows& r, const Place& p, long long token, int part, int parts, const float (&c)[8],
-                                const float (&s)[8], const float (&w)[2][8], float eps, float (&dw)[2][8]) {
+// U heads of a token as they are in memory: `head`, head + parts, ...; those behind the last one in the place of which that
+// is read.
+struct Batch {
+    pw::Unit x[U][2], dy[U][2];
+};
+__device__ inline void request(Batch& b, const Rows& r, const Place& p, long long token, int head, int parts) {
     const value_t* x = r.x + token * r.row;
-    for (int first = part; first < r.heads; first += parts * U) {
-        pw::Unit in[U][2], grad[U][2];
+    const value_t* dy = r.dy + token * r.heads * D;
 #pragma unroll
-        for (int h = 0; h < U; ++h) {
-            const int head = first + h * parts < r.heads ? first + h * parts : first;
+    for (int h = 0; h < U; ++h) {
+        const int at = head + h * parts < r.heads ? head + h * parts : r.heads - 1;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                in[h][i] = grad[h][i] = pw::Unit{};
-                if (p.unit[i] < 0) continue;
-                if (SPIO_NORM || !BACK) in[h][i] = tk::load(x + head * r.head + p.unit[i] * 8);
-                if (BACK) grad[h][i] = tk::load(r.dy + (token * r.heads + head) * D + p.unit[i] * 8);
-            }
+        for (int i = 0; i < 2; ++i) {
+            b.x[h][i] = b.dy[h][i] = pw::Unit{};
+            if (p.unit[i] < 0) continue;
+            if (SPIO_NORM || !BACK) b.x[h][i] = tk::load(x + at * r.head + p.unit[i] * 8);
+            if (BACK) b.dy[h][i] = tk::load(dy + at * D + p.unit[i] * 8);
         }
+    }
+}
+__device__ inline void work_on(const Batch& b, const Rows& r, const Place& p, long long token, int head, int parts,
+                               const float (&c)[8], const float (&s)[8], const float (&w)[2][8], float eps, float (&dw)[2][8]) {
 #pragma unroll
-        for (int h = 0; h < U; ++h) {
-            const int head = first + h * parts;
-            const bool there = head < r.heads;
-            float v[2][8], g[2][8];
+    for (int h = 0; h < U; ++h) {
+        const bool there = head + h * parts < r.heads;
+        float v[2][8], g[2][8];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                tk::values(in[h][i], v[i]);
-                tk::values(grad[h][i], g[i]);
-            }
-            if (SPIO_NORM) {
-                float squares = 0.f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) squares = __builtin_fmaf(v[i][e], v[i][e], squares);
-                squares = tk::sum_of<LANES>(squares);
-                const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, 1.f / D, eps));
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][e] *= rstd;
-                if (BACK) {
-                    rotate(g, c, s, p.rotated);
-                    float dot = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (there) dw[i][e] = __builtin_fmaf(g[i][e], v[i][e], dw[i][e]);
-                            g[i][e] *= w[i][e];
-                            dot = __builtin_fmaf(g[i][e], v[i][e], dot);
-                        }
-                    dot = tk::sum_of<LANES>(dot) * (1.f / D);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) g[i][e] = rstd * __builtin_fmaf(-dot, v[i][e], g[i][e]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[i][e] *= w[i][e];
-                    rotate(v, c, s, p.rotated);
-                }
-            } else if (BACK) {
-                rotate(g, c, s, p.rotated);
-            } else {
-                rotate(v, c, s, p.rotated);
-            }
+        for (int i = 0; i < 2; ++i) {
+            tk::values(b.x[h][i], v[i]);
+            tk::values(b.dy[h][i], g[i]);
+        }
+        if (SPIO_NORM) {
+            float squares = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (there && p.unit[i] >= 0)
-                    tk::store<ONCE>(r.out + (token * r.heads + head) * D + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) squares = __builtin_fmaf(v[i][e], v[i][e], squares);
+            squares = tk::sum_of<LANES>(squares);
+            const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(squares, 1.f / D, eps));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] *= rstd;
+            if (BACK) {
+                rotate(g, c, s, p.rotated);
+                float dot = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (there) dw[i][e] = __builtin_fmaf(g[i][e], v[i][e], dw[i][e]);
+                        g[i][e] *= w[i][e];
+                        dot = __builtin_fmaf(g[i][e], v[i][e], dot);
+                    }
+                dot = tk::sum_of<LANES>(dot) * (1.f / D);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) g[i][e] = rstd * __builtin_fmaf(-dot, v[i][e], g[i][e]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] *= w[i][e];
+                rotate(v, c, s, p.rotated);
+            }
+        } else if (BACK) {
+            rotate(g, c, s, p.rotated);
+        } else {
+            rotate(v, c, s, p.rotated);
         }
+        value_t* out = r.out + (token * r.heads + head + h * parts) * D;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (there && p.unit[i] >= 0) tk::store<ONCE>(out + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
+    }
+}
+
+// The heads `part`, `part + parts`, ... of a token, of which the first batch has been requested where that goes AHEAD
+__device__ inline void heads_of(Batch& b, const Rows& r, const Place& p, long long token, int part, int parts,
+                                const float (&c)[8], const float (&s)[8], const float (&w)[2][8], float eps, float (&dw)[2][8]) {
+    for (int head = part; head < r.heads; head += parts * U) {
+        if (!AHEAD || head != part) request(b, r, p, token, head, parts);
+        work_on(b, r, p, token, head, parts, c, s, w, eps, dw);
     }
 }
 
@@ -211,7 +226,10 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
     for (unsigned item = (__builtin_amdgcn_workgroup_id_x() * 256 + tid) / LANES; item < items; item += groups) {
         const unsigned token = item / (unsigned)parts;
         const int part = (int)(item % (unsigned)parts);
-        const unsigned at = token % (unsigned)a.position_tokens;
+        Batch q_heads, k_heads;
+        if (AHEAD && part < q.heads) request(q_heads, q, p, token, part, parts);  // (there may be no heads at all)
+        if (AHEAD && part < k.heads) request(k_heads, k, p, token, part, parts);
+        const unsigned at = token < (unsigned)a.position_tokens ? token : token % (unsigned)a.position_tokens;
         const long long position = a.wide_positions ? ((const long long*)a.positions)[at] : ((const int*)a.positions)[at];
         float c[8], s[8];
 #pragma unroll
@@ -220,8 +238,8 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
             cos_sin((float)(turns - __builtin_rint(turns)), c[i], s[i]);
             if (p.rotated && pair_of(p, i) < pairs) c[i] *= (float)a.scale, s[i] *= BACK ? -(float)a.scale : (float)a.scale;
         }
-        heads_of(q, p, token, part, parts, c, s, wq, (float)a.eps, dwq);
-        heads_of(k, p, token, part, parts, c, s, wk, (float)a.eps, dwk);
+        heads_of(q_heads, q, p, token, part, parts, c, s, wq, (float)a.eps, dwq);
+        heads_of(k_heads, k, p, token, part, parts, c, s, wk, (float)a.eps, dwk);
     }
 #if SPIO_MODE == 1 && SPIO_NORM
     // the groups of a workgroup, one after the other
