@@ -56,7 +56,8 @@ class HeadNormRotaryParams:
 
 @dataclass(frozen=True)
 class HeadNormRotaryConfig:
-    """Heads that a lane requests at once."""
+    """Heads that a lane requests at once: two, or one in a forward pass with norms, which so has registers for more waves
+    (4n 2048l 24q 8k 128d 38 us, with two 41; without norms 2n 4097l 16q 16k 80d 39, with two 36)."""
 
     heads: int = 2
 
@@ -77,7 +78,7 @@ def _factory(name, mode):
         HeadNormRotaryConfig,
         None,
         kernel_name=name,
-        configs=lambda params, device_attr=None: [HeadNormRotaryConfig()],
+        configs=lambda params, device_attr=None: [HeadNormRotaryConfig(1 if params.norm and mode == 0 else 2)],
         kernel_spec=_spec(mode),
         args_checker=None,
     )
