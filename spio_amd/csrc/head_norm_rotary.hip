@@ -66,13 +66,14 @@ constexpr bool ONCE = D / 2 * sizeof(value_t) % 128 == 0;
 // The two units of a lane (-1: none), and the first of the pairs in each of them that neighbours make (SPIO_INTERLEAVED:
 // four), or of the eight pairs that both make
 struct Place {
-    int unit[2], pair[2];
+    int unit[2], pair[2], pairs;
     bool rotated;  // (SPIO_INTERLEAVED: the pairs before `pairs` are)
 };
 __device__ inline Place place(int lane, int pairs) {
     Place p;
     // neighbouring lanes have neighbouring units
     const int half = SPIO_INTERLEAVED ? 0 : pairs / 8;
+    p.pairs = pairs;
     p.rotated = SPIO_INTERLEAVED || lane < half;
     p.unit[0] = lane < half ? lane : half + lane;
     p.unit[1] = lane < half ? half + lane : PAIRED + lane;
@@ -85,17 +86,25 @@ __device__ inline Place place(int lane, int pairs) {
 }
 __device__ inline int pair_of(const Place& p, int i) { return p.pair[i / 4] + i % 4; }
 
-// (v[0], v[1]) turned by the angles, or, `back`, by their negatives
-__device__ inline void rotate(float (&v)[2][8], const float (&c)[8], const float (&s)[8], bool rotated) {
-    if (!rotated) return;
+// (v[0], v[1]) turned by the angles.  A pair behind the rotated ones (PART: there are such) is left alone: its sine of zero
+// times an infinity is none.
+template <bool PART>
+__device__ inline void rotate_pairs(float (&v)[2][8], const float (&c)[8], const float (&s)[8], const Place& p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float& a = SPIO_INTERLEAVED ? v[i / 4][i % 4 * 2] : v[0][i];
         float& b = SPIO_INTERLEAVED ? v[i / 4][i % 4 * 2 + 1] : v[1][i];
-        const float turned = a * c[i] - b * s[i];
-        b = __builtin_fmaf(a, s[i], b * c[i]);
-        a = turned;
+        const bool there = !PART || pair_of(p, i) < p.pairs;
+        const float turned = a * c[i] - b * s[i], other = __builtin_fmaf(a, s[i], b * c[i]);
+        a = there ? turned : a;
+        b = there ? other : b;
     }
+}
+__device__ inline void rotate(float (&v)[2][8], const float (&c)[8], const float (&s)[8], const Place& p) {
+    if (SPIO_INTERLEAVED && 2 * p.pairs < D)
+        rotate_pairs<true>(v, c, s, p);
+    else if (p.rotated)
+        rotate_pairs<false>(v, c, s, p);
 }
 
 struct Rows {
@@ -149,7 +158,7 @@ __device__ inline void work_on(const Batch& b, const Rows& r, const Place& p, lo
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[i][e] *= rstd;
             if (BACK) {
-                rotate(g, c, s, p.rotated);
+                rotate(g, c, s, p);
                 float dot = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -169,12 +178,12 @@ __device__ inline void work_on(const Batch& b, const Rows& r, const Place& p, lo
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[i][e] *= w[i][e];
-                rotate(v, c, s, p.rotated);
+                rotate(v, c, s, p);
             }
         } else if (BACK) {
-            rotate(g, c, s, p.rotated);
+            rotate(g, c, s, p);
         } else {
-            rotate(v, c, s, p.rotated);
+            rotate(v, c, s, p);
         }
         value_t* out = r.out + (token * r.heads + head + h * parts) * D;
 #pragma unroll
@@ -212,6 +221,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
     const int tid = (int)__builtin_amdgcn_workitem_id_x(), lane = tid % LANES;
     const int pairs = (int)a.pairs, parts = (int)a.parts;
     const Place p = place(lane, pairs);
+    const float eps = __builtin_fmaxf((float)a.eps, 1.17549435e-38f);  // (less counts as the smallest normal number)
     const Rows q = {(const value_t*)a.q, (const value_t*)a.dq, (value_t*)a.q_out, a.q_row, a.q_head, (int)a.q_heads};
     const Rows k = {(const value_t*)a.k, (const value_t*)a.dk, (value_t*)a.k_out, a.k_row, a.k_head, (int)a.k_heads};
     float wq[2][8], wk[2][8], dwq[2][8] = {}, dwk[2][8] = {};
@@ -238,8 +248,8 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
             cos_sin((float)(turns - __builtin_rint(turns)), c[i], s[i]);
             if (p.rotated && pair_of(p, i) < pairs) c[i] *= (float)a.scale, s[i] *= BACK ? -(float)a.scale : (float)a.scale;
         }
-        heads_of(q_heads, q, p, token, part, parts, c, s, wq, (float)a.eps, dwq);
-        heads_of(k_heads, k, p, token, part, parts, c, s, wk, (float)a.eps, dwk);
+        heads_of(q_heads, q, p, token, part, parts, c, s, wq, eps, dwq);
+        heads_of(k_heads, k, p, token, part, parts, c, s, wk, eps, dwk);
     }
 #if SPIO_MODE == 1 && SPIO_NORM
     // the groups of a workgroup, one after the other

@@ -187,10 +187,15 @@ __device__ inline void half_row(const float* lds, int t, int which, int half, fl
     for (int i = 0; i < H; ++i) v[i] = row[i];
 }
 
-// A of a channel as the exponents of 2 that its rates are
+// A rate as the exponent of 2 that it is; finite from below, so that a time step of zero (a token behind the last one) decays
+// nothing at a rate of minus infinity, either
+__device__ inline float rate(float A) {
+    const float r = A * LOG2E;
+    return r < -3.4e38f ? -3.4e38f : r;
+}
 __device__ inline void rates(const Args& a, const Place& p, float (&A2)[N]) {
 #pragma unroll
-    for (int s = 0; s < N; ++s) A2[s] = a.A[(long long)p.loaded * N + s] * LOG2E;
+    for (int s = 0; s < N; ++s) A2[s] = rate(a.A[(long long)p.loaded * N + s]);
 }
 __device__ inline float time_step(float raw) { return SOFTPLUS ? softplus(raw) : raw; }
 
@@ -405,7 +410,7 @@ SPIO_KERNEL_NAME(const Args a) {
     for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-            A2[c][i] = there(i) ? a.A[(long long)channel[c] * N + state(i)] * LOG2E : 0.f;
+            A2[c][i] = there(i) ? rate(a.A[(long long)channel[c] * N + state(i)]) : 0.f;
             r[c][i] = dA[c][i] = 0.f;
         }
     if (p.chunks > 1) {  // what the chunks behind this one add
@@ -578,7 +583,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
     const long long sequence = id / blocks / N;
     const int chunks = (int)((a.tokens + a.chunk - 1) / a.chunk);
     if (channel >= a.channels) return;
-    const float A2 = a.A[channel * N + s] * LOG2E;
+    const float A2 = rate(a.A[channel * N + s]);
     float v = !BACK && a.before ? a.before[(sequence * a.channels + channel) * N + s] : 0.f;
     float* ends = a.ends + sequence * chunks * (N + 1) * a.channels + channel;
     for (int first = 0; first < chunks; first += JOINED) {
@@ -595,7 +600,8 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
             const int i = first + k;
             if (i >= chunks) break;
             ends[((BACK ? chunks - 1 - i : i) * (N + 1) + s) * a.channels] = v;
-            v = __builtin_fmaf(exp2_(sum[k] * A2), v, end[k]);
+            // (nothing stays nothing, also where the states grow so much that the factor is infinite)
+            v = v == 0.f ? end[k] : __builtin_fmaf(exp2_(sum[k] * A2), v, end[k]);
         }
     }
 }
@@ -619,13 +625,13 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
         const float4_t v = *(const float4_t*)(before + part * 4);
         const float4_t w = *(const float4_t*)(a.A + (long long)c * N + part * 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = v[i], A2[i] = w[i] * LOG2E;
+        for (int i = 0; i < 4; ++i) h[i] = v[i], A2[i] = rate(w[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool there = part * 4 + i < N;
             h[i] = there ? before[part * 4 + i] : 0.f;
-            A2[i] = there ? a.A[(long long)c * N + part * 4 + i] * LOG2E : 0.f;
+            A2[i] = there ? rate(a.A[(long long)c * N + part * 4 + i]) : 0.f;
         }
     }
 #pragma unroll

@@ -846,7 +846,8 @@ Rows rows_of(const Tensor& t, int64_t step = 1) {
         outer = t.size(i) * t.stride(i);
         seen = true;
     }
-    const bool fits = step == 1 || (row * t.element_size() % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+    const int64_t size = row * t.element_size();
+    const bool fits = step == 1 ? size < 1 << 27 : size % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     if (even && fits && (last == 1 || t.stride(-1) == 1)) return {t, row};
     return {t.clone(at::MemoryFormat::Contiguous), last};
 }
@@ -867,9 +868,14 @@ bool on_16_bytes(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_pt
 bool writable_state(const Tensor& state, const Tensor& out, std::initializer_list<Tensor> inputs) {
     if (!is_plain(out) || out.sizes() != state.sizes() || out.scalar_type() != state.scalar_type() ||
         out.device() != state.device() || !state.is_contiguous() || !out.is_contiguous() || !on_16_bytes(state) ||
-        !on_16_bytes(out) || (state.data_ptr() != out.data_ptr() && overlap(state, out)) || wants_grad(out) || out.is_inference())
+        !on_16_bytes(out) || (state.data_ptr() != out.data_ptr() && overlap(state, out)) || wants_grad(out) ||
+        (out.is_inference() && !c10::InferenceMode::is_enabled()))
         return false;
     return std::none_of(inputs.begin(), inputs.end(), [&](const Tensor& t) { return t.defined() && overlap(t, out); });
+}
+// A state was written to (tensors of inference mode have no versions)
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return static_cast<float*>(mut(t)); }
@@ -1615,7 +1621,7 @@ PyObject* causal_conv1d_step(PyObject*, PyObject* const* args, Py_ssize_t nargs,
         a.x = ptr(rows.t), a.weight = ptr(w), a.bias = ptr(b), a.before = ptr(cv.before), a.out = mut(y), a.after = mut(after);
         a.tokens = a.slice = 1, a.channels = cv.c, a.sequences = cv.n, a.x_row = rows.row;
         launch_structure(*plan, divup(cv.n * (cv.c / 8), 64), c10::hip::getCurrentHIPStream(x.get_device()), &a);
-        after.unsafeGetTensorImpl()->bump_version();
+        written(after);
     }
     return THPVariable_Wrap(y);
     END_HANDLE_TH_ERRORS
@@ -1628,6 +1634,7 @@ bool scan_fits(const variable_list& t) {
         return false;
     std::vector<int64_t> row = u.sizes().vec();
     const int64_t c = row.back();
+    if (c >= 1 << 24) return false;
     row.back() = A.size(1);
     return fits(t[1], u, u.sizes(), true) && fits(A, u, {c, A.size(1)}, false) && fits(t[3], u, row, true) &&
            fits(t[4], u, row, true) && absent_or_fits(t[5], u, {c}, false) && absent_or_fits(t[6], u, u.sizes(), true) &&
@@ -1699,7 +1706,7 @@ PyObject* selective_scan_step(PyObject*, PyObject* const* args, Py_ssize_t nargs
         in.a.before = floats(sc.before), in.a.out = mut(y), in.a.after = floats(after);
         const int64_t lanes = sc.s <= 4 ? 1 : sc.s <= 8 ? 2 : sc.s <= 16 ? 4 : 8;
         launch_structure(*plan, divup(sc.n * sc.c * lanes, 256), c10::hip::getCurrentHIPStream(u.get_device()), &in.a);
-        after.unsafeGetTensorImpl()->bump_version();
+        written(after);
     }
     return THPVariable_Wrap(y);
     END_HANDLE_TH_ERRORS
@@ -1722,7 +1729,7 @@ PyObject* head_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs, P
         !fits(k, q, r.shape(r.k_heads), true) || r.d % 8 || r.d > ROTARY_MAX_HEAD ||
         wq.defined() != wk.defined() || !absent_or_fits(wq, q, {r.d}, false) || !absent_or_fits(wk, q, {r.d}, false) ||
         !(r.eps > 0) || r.eps > std::numeric_limits<double>::max() || !std::isfinite(r.scale) || pairs < 1 || 2 * pairs > r.d ||
-        (!r.interleaved && pairs % 8) || r.frequencies.scalar_type() != at::kDouble || r.frequencies.device() != q.device() ||
+        (!r.interleaved && pairs % 8) || r.frequencies.scalar_type() != at::kDouble || wants_grad(r.frequencies) || r.frequencies.device() != q.device() ||
         !is_plain(r.positions) || (r.positions.scalar_type() != at::kLong && r.positions.scalar_type() != at::kInt) ||
         r.positions.device() != q.device() ||
         !(r.positions.sizes() == at::IntArrayRef({r.l}) || r.positions.sizes() == at::IntArrayRef({r.n, r.l})))

@@ -29,7 +29,15 @@ from ..kernels.group_norm_2d_kernel import DTYPES
 from ..kernels.token_args import Arguments
 from ..util.math import divup
 from .group_norm_2d_function import aligned, refuse_forward_derivatives
-from .token_rows import check_out_state, check_parameters, check_tokens, refuse_state_gradients, require_gpu, rows_of
+from .token_rows import (
+    check_out_state,
+    check_parameters,
+    check_tokens,
+    refuse_inference_state,
+    refuse_state_gradients,
+    require_gpu,
+    rows_of,
+)
 
 STRUCT = "SpioConv1dArgs"
 SUM_COLUMNS = 32  # of a workgroup that adds up partial sums
@@ -237,5 +245,6 @@ def causal_conv1d_step(
     if y is not NotImplemented:
         return y
     refuse_forward_derivatives(inputs, state, weight, bias, out_state)
+    refuse_inference_state(out_state)
     with torch.no_grad():
         return causal_conv1d_step_op(inputs, state, weight, bias, activation, out_state)

@@ -6,7 +6,9 @@ without a norm of every head before it, in one pass over both tensors.
     the i-th pair (n1, n2) of a head becomes scale (n1 cos - n2 sin, n2 cos + n1 sin)
 
 Pair i is the channels (2i, 2i + 1) of a head with `interleaved`, else (i, pairs + i); channels behind the pairs stay as they
-are.  Angles are taken in float64 and there is no table of them, so that positions have no bound; everything else is float32.
+are.  Angles are taken in float64 and there is no table of them: one is off by position * frequency * 2^-53 radians, and by 2^-24
+turns, so that positions have no bound in practice.  Everything else is float32; the sum of a head's squares has to stay below
+its largest number (3.4e38).
 
 The reference has no such operators; their siblings here are the norms.
 """
@@ -199,6 +201,8 @@ def _call(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, sc
     if result is not NotImplemented:
         return result
     refuse_forward_derivatives(q, k, q_weight, k_weight)
+    if torch.is_grad_enabled() and frequencies.requires_grad:
+        raise RuntimeError("no gradients pass to frequencies: detach them")
     return head_norm_rotary_forward(q, k, q_weight, k_weight, positions, frequencies, float(eps), bool(interleaved), float(scale))
 
 
@@ -231,7 +235,7 @@ def head_norm_rotary(
 
     Args:
         q_weight, k_weight: (D,), any float type.
-        eps: positive and finite, added to the mean square.
+        eps: positive and finite, added to the mean square; below 2^-126 it counts as that.
         (the others as in `rotary`)
     """
     assert q_weight is not None and k_weight is not None, "head_norm_rotary takes weights of both norms"

@@ -39,6 +39,7 @@ from .token_rows import (
     check_out_state,
     check_parameters,
     check_tokens,
+    refuse_inference_state,
     refuse_state_gradients,
     require_gpu,
     rows_of,
@@ -52,7 +53,7 @@ SUM_COLUMNS = 32  # of a workgroup that adds up partial sums
 def _check(what, inputs, dims, delta, A, B, C, D, gate, delta_bias, state):
     assert inputs.dim() == dims, f"{what} takes {'[sequences, tokens, channels]' if dims == 3 else '[sequences, channels]'}"
     c = inputs.shape[-1]
-    assert c > 0, f"{what} takes at least one channel"
+    assert 0 < c < 1 << 24, f"{what} takes from one to 2^24 - 1 channels"
     assert inputs.shape[-2] < 1 << 30, f"{what} takes fewer than 2^30 tokens of a sequence"
     assert A.dim() == 2 and 1 <= A.shape[1] <= MAX_STATES, f"A is [channels, 1..{MAX_STATES}]"
     s = A.shape[1]
@@ -296,5 +297,6 @@ def selective_scan_step(
     if y is not NotImplemented:
         return y
     refuse_forward_derivatives(inputs, state, delta, A, B, C, D, gate, delta_bias, out_state)
+    refuse_inference_state(out_state)
     with torch.no_grad():
         return selective_scan_step_op(inputs, state, delta, A, B, C, D, gate, delta_bias, bool(delta_softplus), out_state)

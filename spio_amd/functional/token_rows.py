@@ -6,6 +6,8 @@ import torch
 
 from ..kernels.group_norm_2d_kernel import DTYPES
 
+MAX_ROW = 1 << 27  # bytes from row to row of a tensor that is read in tiles
+
 
 def check_tokens(what: str, **tensors: Optional[torch.Tensor]):
     """Types and devices of the tensors of an operator: one of the three types, the first one's, on its device."""
@@ -30,15 +32,17 @@ def require_gpu(what: str, t: torch.Tensor):
 
 def rows_of(t: Optional[torch.Tensor], step: int = 1) -> Tuple[Optional[torch.Tensor], int]:
     """[sequences, tokens, values] (or [sequences, values]) as rows of values that are equally far apart: the tensor itself,
-    or a copy without gaps where it is not that, or where rows do not start on 16 bytes though `step` (8) values are
-    loaded at once.  Also their distance in values."""
+    or a copy without gaps where it is not that, where rows do not start on 16 bytes though `step` (8) values are loaded at
+    once, or where a tile of eight rows that are read by their distance to the first would pass 31 bits.  Also their distance
+    in values."""
     if t is None:
         return None, 0
     *lead, last = t.shape
     sizes = [(size, stride) for size, stride in zip(lead, t.stride()) if size != 1]
     row = sizes[-1][1] if sizes else last
     even = all(outer[1] == inner[0] * inner[1] for outer, inner in zip(sizes, sizes[1:]))
-    fits = step == 1 or (row * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0)
+    size = row * t.element_size()
+    fits = size < MAX_ROW if step == 1 else size % 16 == 0 and t.data_ptr() % 16 == 0
     if even and fits and (last == 1 or t.stride(-1) == 1):
         return t, row
     t = t.clone(memory_format=torch.contiguous_format)
@@ -54,6 +58,12 @@ def refuse_state_gradients(*tensors):
     """A state passes from call to call without a history; a gradient of it would silently be missing."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("no gradients pass through a state: detach it")
+
+
+def refuse_inference_state(t: torch.Tensor):
+    """As torch's own operators do, which keep no versions of such tensors."""
+    if t.is_inference() and not torch.is_inference_mode_enabled():
+        raise RuntimeError("a state that was made in inference mode is updated there only")
 
 
 def _extent(t: torch.Tensor) -> Tuple[int, int]:

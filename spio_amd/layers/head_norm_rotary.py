@@ -19,12 +19,13 @@ class HeadNormRotary(nn.Module):
         for name in ("q_weight", "k_weight"):
             weight = nn.Parameter(torch.ones(channels, device=device, dtype=dtype)) if norm else None
             self.register_parameter(name, weight)
-        frequencies = rotary_frequencies(channels if rotated is None else rotated, device=device, **scaling)
-        self.register_buffer("frequencies", frequencies, persistent=False)
+        self.scaling = dict(channels=channels if rotated is None else rotated, **scaling)
+        self.register_buffer("frequencies", rotary_frequencies(**self.scaling, device=device), persistent=False)
 
     def _apply(self, fn, recurse=True):
-        """Frequencies go with the module to a device, but stay float64 where it is cast."""
-        frequencies = self.frequencies
+        """Frequencies go with the module to a device, but stay float64 where it is cast; those of a module without memory
+        (the meta device) are made again."""
+        frequencies = rotary_frequencies(**self.scaling) if self.frequencies.is_meta else self.frequencies
         super()._apply(fn, recurse)
         self.frequencies = frequencies.to(self.frequencies.device)
         return self

@@ -35,7 +35,7 @@ class SelectiveScan(nn.Module):
 
     def empty_state(self, sequences) -> torch.Tensor:
         """The state before the first token."""
-        return self.D.new_zeros((sequences, self.channels, self.states)).detach()
+        return self.D.new_zeros((sequences, self.channels, self.states), dtype=torch.float32).detach()
 
     def forward(self, x, delta, B, C, gate=None, initial_state=None, return_state=False):
         return selective_scan(x, delta, -self.log_rates.float().exp(), B, C, self.D, gate, self.delta_bias, True, initial_state,

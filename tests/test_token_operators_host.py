@@ -156,6 +156,18 @@ def test_rows_of():
     assert rows_of(wide[..., :16], 8)[0].data_ptr() == wide.data_ptr()
     for t in (wide[..., 2:18], torch.zeros(3, 7, 18)[..., :16]):  # rows that do not start on 16 bytes
         assert rows_of(t, 8)[0].data_ptr() != t.data_ptr()
+    far = torch.empty((1 << 26) + 16, dtype=torch.float16)  # eight rows of which pass 31 bits
+    for row, copied in (((1 << 26) - 8, False), (1 << 26, True)):
+        t = far.as_strided((1, 2, 16), (0, row, 1))
+        assert (rows_of(t)[0].data_ptr() != t.data_ptr()) == copied and rows_of(t, 8)[1] == row
+
+
+def test_frequencies_have_no_gradients():
+    leaf = FREQUENCIES.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="frequencies"):
+        rotary(Q, Q, POSITIONS, leaf)
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU only"):
+        rotary(Q, Q, POSITIONS, leaf)
 
 
 def test_heads_of():
