@@ -29,10 +29,12 @@ namespace {
 using tk::value_t;
 constexpr int D = SPIO_HEAD, UNITS = D / 8;
 constexpr int PAIRED = (UNITS + 1) / 2;  // lanes of a head that have channels
-constexpr int LANES = PAIRED <= 1 ? 1 : PAIRED <= 2 ? 2 : PAIRED <= 4 ? 4 : PAIRED <= 8 ? 8 : 16;
+// (a norm's sums cross a power of two of lanes)
+constexpr int LANES = !SPIO_NORM ? PAIRED : PAIRED <= 1 ? 1 : PAIRED <= 2 ? 2 : PAIRED <= 4 ? 4 : PAIRED <= 8 ? 8 : 16;
 constexpr int GROUPS = 256 / LANES;      // of a workgroup
 constexpr int U = SPIO_HEADS;            // heads requested at once
 constexpr bool BACK = SPIO_MODE == 1;
+constexpr bool FULL = UNITS == 2 * LANES;  // no lane is without channels
 // Whether the first heads of a token are requested before its angles are computed: a backward pass with norms has no registers
 // for that
 constexpr bool AHEAD = !(BACK && SPIO_NORM);
@@ -59,10 +61,6 @@ __device__ inline void cos_sin(float turn, float& c, float& s) {
     s = k & 2 ? -odd : odd;
 }
 
-// Stores go past the caches where the lanes of a head write whole lines at once (us with and without: 128 channels of
-// bfloat16, 4n 2048l 24q 8k 32 and 39 forward, 48 and 52 backward; 80 of float16, 2n 4097l, 32 and 29)
-constexpr bool ONCE = D / 2 * sizeof(value_t) % 128 == 0;
-
 // The two units of a lane (-1: none), and the first of the pairs in each of them that neighbours make (SPIO_INTERLEAVED:
 // four), or of the eight pairs that both make
 struct Place {
@@ -71,12 +69,11 @@ struct Place {
 };
 __device__ inline Place place(int lane, int pairs) {
     Place p;
-    // neighbouring lanes have neighbouring units
-    const int half = SPIO_INTERLEAVED ? 0 : pairs / 8;
+    const int half = pairs / 8;
     p.pairs = pairs;
     p.rotated = SPIO_INTERLEAVED || lane < half;
-    p.unit[0] = lane < half ? lane : half + lane;
-    p.unit[1] = lane < half ? half + lane : PAIRED + lane;
+    p.unit[0] = SPIO_INTERLEAVED ? 2 * lane : lane < half ? lane : half + lane;
+    p.unit[1] = SPIO_INTERLEAVED ? 2 * lane + 1 : lane < half ? half + lane : PAIRED + lane;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         p.pair[i] = SPIO_INTERLEAVED ? 4 * p.unit[i] : 8 * lane + 4 * i;
@@ -124,13 +121,13 @@ __device__ inline void request(Batch& b, const Rows& r, const Place& p, long lon
     const value_t* dy = r.dy + token * r.heads * D;
 #pragma unroll
     for (int h = 0; h < U; ++h) {
-        const int at = head + h * parts < r.heads ? head + h * parts : r.heads - 1;
+        const int last = r.heads ? r.heads - 1 : 0, at = head + h * parts < last ? head + h * parts : last;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+            const int unit = FULL || p.unit[i] >= 0 ? p.unit[i] : 0;
             b.x[h][i] = b.dy[h][i] = pw::Unit{};
-            if (p.unit[i] < 0) continue;
-            if (SPIO_NORM || !BACK) b.x[h][i] = tk::load(x + at * r.head + p.unit[i] * 8);
-            if (BACK) b.dy[h][i] = tk::load(dy + at * D + p.unit[i] * 8);
+            if (SPIO_NORM || !BACK) b.x[h][i] = tk::load(x + at * r.head + unit * 8);
+            if (BACK) b.dy[h][i] = tk::load(dy + at * D + unit * 8);
         }
     }
 }
@@ -144,6 +141,10 @@ __device__ inline void work_on(const Batch& b, const Rows& r, const Place& p, lo
         for (int i = 0; i < 2; ++i) {
             tk::values(b.x[h][i], v[i]);
             tk::values(b.dy[h][i], g[i]);
+            if (SPIO_NORM && !FULL && p.unit[i] < 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] = g[i][e] = 0.f;
+            }
         }
         if (SPIO_NORM) {
             float squares = 0.f;
@@ -188,16 +189,25 @@ __device__ inline void work_on(const Batch& b, const Rows& r, const Place& p, lo
         value_t* out = r.out + (token * r.heads + head + h * parts) * D;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (there && p.unit[i] >= 0) tk::store<ONCE>(out + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
+            if (there && (FULL || p.unit[i] >= 0)) tk::store<true>(out + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
     }
 }
 
-// The heads `part`, `part + parts`, ... of a token, of which the first batch has been requested where that goes AHEAD
+// What was requested before is not moved behind what follows
+__device__ inline void pinned() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// The heads `part`, `part + parts`, ... of a token, of which the first batch has been requested.  The next one is requested before
+// the present one is worked on (behind the last one that is read again): its wait would be for the stores before it, too.
 __device__ inline void heads_of(Batch& b, const Rows& r, const Place& p, long long token, int part, int parts,
                                 const float (&c)[8], const float (&s)[8], const float (&w)[2][8], float eps, float (&dw)[2][8]) {
     for (int head = part; head < r.heads; head += parts * U) {
-        if (!AHEAD || head != part) request(b, r, p, token, head, parts);
+        Batch next;
+        request(next, r, p, token, head + parts * U, parts);
+        pinned();
         work_on(b, r, p, token, head, parts, c, s, w, eps, dw);
+        b = next;
     }
 }
 
@@ -207,9 +217,10 @@ __device__ inline void weights(const float* from, const Place& p, float (&w)[2][
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
-            const float4_t v = from && p.unit[i] >= 0 ? *(const float4_t*)(from + p.unit[i] * 8 + e) : float4_t{0.f, 0.f, 0.f, 0.f};
+            const bool there = FULL || p.unit[i] >= 0;
+            const float4_t v = from ? *(const float4_t*)(from + (there ? p.unit[i] : 0) * 8 + e) : float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[i][e + k] = v[k];
+            for (int k = 0; k < 4; ++k) w[i][e + k] = there ? v[k] : 0.f;
         }
 }
 
@@ -218,37 +229,46 @@ __device__ inline void weights(const float* from, const Place& p, float (&w)[2][
 #if SPIO_MODE < 2
 
 extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))) SPIO_KERNEL_NAME(const SpioRotaryArgs a) {
-    const int tid = (int)__builtin_amdgcn_workitem_id_x(), lane = tid % LANES;
-    const int pairs = (int)a.pairs, parts = (int)a.parts;
+    const int tid = (int)__builtin_amdgcn_workitem_id_x(), lane = tid % LANES, group = tid / LANES;
+    if (group >= GROUPS) return;  // (not with norms)
+    const int pairs = (int)a.pairs, parts = (int)a.parts, wide = (int)a.wide_positions;
     const Place p = place(lane, pairs);
     const float eps = __builtin_fmaxf((float)a.eps, 1.17549435e-38f);  // (less counts as the smallest normal number)
-    const Rows q = {(const value_t*)a.q, (const value_t*)a.dq, (value_t*)a.q_out, a.q_row, a.q_head, (int)a.q_heads};
-    const Rows k = {(const value_t*)a.k, (const value_t*)a.dk, (value_t*)a.k_out, a.k_row, a.k_head, (int)a.k_heads};
+    Rows q = {(const value_t*)a.q, (const value_t*)a.dq, (value_t*)a.q_out, a.q_row, a.q_head, (int)a.q_heads};
+    Rows k = {(const value_t*)a.k, (const value_t*)a.dk, (value_t*)a.k_out, a.k_row, a.k_head, (int)a.k_heads};
+    if (!q.heads) q.x = k.x, q.dy = k.dy, q.row = k.row;
+    if (!k.heads) k.x = q.x, k.dy = q.dy, k.row = q.row;
     float wq[2][8], wk[2][8], dwq[2][8] = {}, dwk[2][8] = {};
     weights(SPIO_NORM ? a.q_weight : nullptr, p, wq);
     weights(SPIO_NORM ? a.k_weight : nullptr, p, wk);
-    double frequency[8];  // turns a position
+    // (those of lanes and pairs that are not rotated are not used; nothing here waits for what is loaded, or the heads would
+    // be requested later)
+    double frequency[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        frequency[i] = p.rotated && pair_of(p, i) < pairs ? a.frequencies[pair_of(p, i)] * 0.15915494309189535 : 0.;
-    const unsigned groups = __builtin_amdgcn_grid_size_x() / LANES, items = (unsigned)(a.tokens * parts);  // (fewer than 2^31)
+    for (int i = 0; i < 8; ++i) frequency[i] = a.frequencies[pair_of(p, i) < pairs ? pair_of(p, i) : 0];
+    const unsigned groups = __builtin_amdgcn_grid_size_x() / 256 * GROUPS, items = (unsigned)(a.tokens * parts);  // (fewer than 2^31)
     // (a group's lanes stay together: they cross lanes for the norm)
-    for (unsigned item = (__builtin_amdgcn_workgroup_id_x() * 256 + tid) / LANES; item < items; item += groups) {
+    for (unsigned item = __builtin_amdgcn_workgroup_id_x() * GROUPS + group; item < items; item += groups) {
         const unsigned token = item / (unsigned)parts;
         const int part = (int)(item % (unsigned)parts);
-        Batch q_heads, k_heads;
-        if (AHEAD && part < q.heads) request(q_heads, q, p, token, part, parts);  // (there may be no heads at all)
-        if (AHEAD && part < k.heads) request(k_heads, k, p, token, part, parts);
         const unsigned at = token < (unsigned)a.position_tokens ? token : token % (unsigned)a.position_tokens;
-        const long long position = a.wide_positions ? ((const long long*)a.positions)[at] : ((const int*)a.positions)[at];
+        // (requested before the heads: loads come back in their order.  Of an int64 the halves apart, of an int32 the one)
+        const int* slot = (const int*)a.positions + (unsigned long long)at * (unsigned)(1 + wide); const int low = slot[0], high = slot[wide];
+        Batch q_heads, k_heads;
+        request(q_heads, q, p, token, part, parts);
+        if (AHEAD) request(k_heads, k, p, token, part, parts);
+        pinned();
+        const double position = wide ? __builtin_fma((double)high, 4294967296., (double)(unsigned)low) : (double)low;
+        const double turned = position * 0.15915494309189535;  // by a frequency of one
         float c[8], s[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const double turns = (double)position * frequency[i];
+            const double turns = turned * frequency[i];
             cos_sin((float)(turns - __builtin_rint(turns)), c[i], s[i]);
-            if (p.rotated && pair_of(p, i) < pairs) c[i] *= (float)a.scale, s[i] *= BACK ? -(float)a.scale : (float)a.scale;
+            c[i] *= (float)a.scale, s[i] *= BACK ? -(float)a.scale : (float)a.scale;
         }
         heads_of(q_heads, q, p, token, part, parts, c, s, wq, eps, dwq);
+        if (!AHEAD) request(k_heads, k, p, token, part, parts);
         heads_of(k_heads, k, p, token, part, parts, c, s, wk, eps, dwk);
     }
 #if SPIO_MODE == 1 && SPIO_NORM
@@ -261,7 +281,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (p.unit[i] >= 0) sums[tid / LANES][p.unit[i] * 8 + e] = which ? dwk[i][e] : dwq[i][e];
+                if (p.unit[i] >= 0) sums[group][p.unit[i] * 8 + e] = which ? dwk[i][e] : dwq[i][e];
         tk::barrier();
         for (int d = tid; d < D; d += 256) {
             float sum = 0.f;

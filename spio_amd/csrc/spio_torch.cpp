@@ -1104,17 +1104,18 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
 // ---- rotary positions and norms of heads ----
 
 constexpr int64_t ROTARY_MAX_HEAD = 256, ROTARY_THREADS = 256, ROTARY_SUMMED = 512;
-int64_t rotary_lanes(int64_t head) {
-    int64_t lanes = 1;
+int64_t rotary_lanes(int64_t head, bool norm) {
+    int64_t lanes = norm ? 1 : divup(head, 16);
     while (lanes * 16 < head) lanes *= 2;
     return lanes;
 }
-int64_t rotary_parts(int64_t tokens, int64_t heads, int64_t head) {
-    const int64_t waves = divup(tokens * rotary_lanes(head), 64);
-    return std::min(divup(heads, 2), std::max(divup(heads, 8), divup(4096, waves)));
+int64_t rotary_parts(int64_t heads) {
+    int64_t parts = 1;
+    while (parts * 8 <= heads) parts *= 2;
+    return parts;
 }
-int64_t rotary_grid(int64_t tokens, int64_t parts, int64_t head, bool summed) {
-    const int64_t grid = divup(tokens * parts * rotary_lanes(head), ROTARY_THREADS);
+int64_t rotary_grid(int64_t tokens, int64_t parts, int64_t head, bool norm, bool summed) {
+    const int64_t grid = divup(tokens * parts, ROTARY_THREADS / rotary_lanes(head, norm));
     return summed ? std::min(grid, ROTARY_SUMMED) : grid;
 }
 
@@ -1124,12 +1125,11 @@ struct Rotary {
     double eps, scale;
     Tensor positions, frequencies;  // have no gradients
     int64_t tokens() const { return n * l; }
-    int64_t parts() const { return rotary_parts(tokens(), std::max(q_heads, k_heads), d); }
     std::vector<int64_t> shape(int64_t heads) const { return {n, l, heads, d}; }
     SpioRotaryArgs args() const {
         SpioRotaryArgs a = {};
         a.positions = ptr(positions), a.frequencies = static_cast<const double*>(ptr(frequencies));
-        a.tokens = tokens(), a.q_heads = q_heads, a.k_heads = k_heads, a.parts = parts(), a.pairs = frequencies.numel();
+        a.tokens = tokens(), a.q_heads = q_heads, a.k_heads = k_heads, a.parts = rotary_parts(std::max(q_heads, k_heads)), a.pairs = frequencies.numel();
         a.position_tokens = positions.numel(), a.wide_positions = positions.scalar_type() == at::kLong;
         a.eps = eps, a.scale = scale;
         return a;
@@ -1157,7 +1157,7 @@ variable_list rotary_forward(const Rotary& r, const Tensor& q, const Tensor& k, 
     SpioRotaryArgs a = r.args();
     a.q = ptr(qh.t), a.q_row = qh.row, a.q_head = qh.head, a.k = ptr(kh.t), a.k_row = kh.row, a.k_head = kh.head;
     a.q_weight = floats(wq), a.k_weight = floats(wk), a.q_out = mut(qo), a.k_out = mut(ko);
-    launch_structure(*rotary_plan(ROTARY, r, q, wq.defined()), rotary_grid(r.tokens(), a.parts, r.d, false),
+    launch_structure(*rotary_plan(ROTARY, r, q, wq.defined()), rotary_grid(r.tokens(), a.parts, r.d, wq.defined(), false),
                      c10::hip::getCurrentHIPStream(q.get_device()), &a);
     return {qo, ko};
 }
@@ -1210,7 +1210,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
         const Tensor gqc = whole(gq), gkc = whole(gk), wqf = whole(to_float_1d(wq)), wkf = whole(to_float_1d(wk));
         const Tensor dq = empty_of(gq.sizes(), type(6), gq), dk = empty_of(gk.sizes(), type(6), gk);
         SpioRotaryArgs a = r.args();
-        const int64_t grid = rotary_grid(r.tokens(), a.parts, r.d, norm);
+        const int64_t grid = rotary_grid(r.tokens(), a.parts, r.d, norm, norm);
         Heads qh, kh;
         Tensor partials, dwq, dwk;
         if (norm) {

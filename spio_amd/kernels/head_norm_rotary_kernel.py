@@ -17,24 +17,21 @@ THREADS = 256
 SUMMED_WORKGROUPS = 512  # of a backward pass with norms, each of which leaves a row of sums
 
 
-def lanes_of(head: int) -> int:
-    """Lanes of a head: two units of eight channels each, a power of two."""
-    lanes = 1
-    while lanes * 16 < head:
-        lanes *= 2
-    return lanes
+def lanes_of(head: int, norm: bool) -> int:
+    """Lanes of a head: one for two units of eight channels, with norms, whose sums cross them, a power of two."""
+    return divup(head, 16) if not norm else 1 << (divup(head, 16) - 1).bit_length()
 
 
-def parts_of(tokens: int, heads: int, head: int) -> int:
-    """Parts that the heads of a token are split into: lanes that share a token's cosines take every parts-th head.  About
-    eight heads a lane, fewer where waves are few (us with 1, 2, 4, 8 and 16 parts, forward: 2n 4097l 16 heads of 80
-    channels 39, 32, 29, 31, 38; 1n 16385l 32q 8k 128d 90, 80, 77, 89, 113)."""
-    waves = divup(tokens * lanes_of(head), 64)
-    return min(divup(heads, 2), max(divup(heads, 8), divup(4096, waves)))
+def parts_of(heads: int) -> int:
+    """Parts that the heads of a token are split into: lanes that share a token's cosines take every parts-th head.  A power
+    of two, for four to seven heads a lane (us with 1, 2, 4 and 8 parts, forward: 2n 4097l 16 heads of 80 channels 35, 32,
+    28, 27; 4n 2048l 24q 8k 128d with norms 37, 36, 37, 37, backward 50, 49, 48, 50; 1n 16385l 32q 8k 82, 75, 73, 73; 400
+    tokens, 24q 8k 14.0, 10.6, 9.6, 11.7)."""
+    return 1 << max(0, (heads // 4).bit_length() - 1)
 
 
-def grid_of(tokens: int, parts: int, head: int, summed: bool) -> int:
-    grid = divup(tokens * parts * lanes_of(head), THREADS)
+def grid_of(tokens: int, parts: int, head: int, norm: bool, summed: bool) -> int:
+    grid = divup(tokens * parts, THREADS // lanes_of(head, norm))
     return min(grid, SUMMED_WORKGROUPS) if summed else grid
 
 
@@ -56,8 +53,8 @@ class HeadNormRotaryParams:
 
 @dataclass(frozen=True)
 class HeadNormRotaryConfig:
-    """Heads that a lane requests at once: two, or one in a forward pass with norms, which so has registers for more waves
-    (4n 2048l 24q 8k 128d 38 us, with two 41; without norms 2n 4097l 16q 16k 80d 39, with two 36)."""
+    """Heads that a lane requests at once (4n 2048l 24q 8k 128d with norms, forward and backward, us: one 39 and 49, two 37 and
+    48, four 38 and 57)."""
 
     heads: int = 2
 
@@ -78,7 +75,7 @@ def _factory(name, mode):
         HeadNormRotaryConfig,
         None,
         kernel_name=name,
-        configs=lambda params, device_attr=None: [HeadNormRotaryConfig(1 if params.norm and mode == 0 else 2)],
+        configs=lambda params, device_attr=None: [HeadNormRotaryConfig()],
         kernel_spec=_spec(mode),
         args_checker=None,
     )

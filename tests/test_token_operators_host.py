@@ -212,11 +212,11 @@ def test_work_is_cut_alike_on_both_paths():
                     assert other.scan_chunk(tokens, channels, sequences, backward) == chunk_tokens(tokens, channels, sequences, backward)
                     assert other.conv1d_slice(tokens, channels, sequences, backward) == slice_tokens(tokens, channels, sequences, backward)
         for heads in (1, 2, 9, 64):
-            for head in (8, 32, 80, 128, 256):
-                parts = parts_of(tokens, heads, head)
-                assert other.rotary_parts(tokens, heads, head) == parts and 1 <= parts <= heads
+            for head, norm in ((h, norm) for h in (8, 32, 80, 128, 256) for norm in (False, True)):
+                parts = parts_of(heads)
+                assert other.rotary_parts(heads) == parts and 1 <= parts <= heads
                 for summed in (False, True):
-                    assert other.rotary_grid(tokens, parts, head, summed) == grid_of(tokens, parts, head, summed)
+                    assert other.rotary_grid(tokens, parts, head, norm, summed) == grid_of(tokens, parts, head, norm, summed)
     for states in range(1, 33):
         assert other.scan_tile(states) == tile_tokens(states)
 
@@ -231,7 +231,8 @@ def test_chunks_and_slices_cover_the_tokens():
                 assert chunk >= tokens or chunk % 8 == 0  # whole tiles
                 assert -(-tokens // chunk) * waves <= max(4096, waves)
     assert all(8 % tile_tokens(states) == 0 for states in range(1, 33))
-    assert [lanes_of(d) for d in (8, 16, 24, 32, 64, 80, 128, 136, 256)] == [1, 1, 2, 2, 4, 8, 8, 16, 16]
+    assert [lanes_of(d, True) for d in (8, 16, 24, 32, 64, 80, 128, 136, 256)] == [1, 1, 2, 2, 4, 8, 8, 16, 16]
+    assert [lanes_of(d, False) for d in (8, 16, 24, 32, 64, 80, 128, 136, 256)] == [1, 1, 2, 2, 4, 5, 8, 9, 16]
 
 
 def test_frequencies():
