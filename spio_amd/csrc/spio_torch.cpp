@@ -1109,7 +1109,9 @@ int64_t rotary_lanes(int64_t head, bool norm) {
     while (lanes * 16 < head) lanes *= 2;
     return lanes;
 }
-int64_t rotary_parts(int64_t heads) {
+int64_t rotary_parts(int64_t tokens, int64_t heads, int64_t head, bool norm) {
+    const int64_t most = divup(heads, 2);
+    if (divup(tokens * rotary_lanes(head, norm), 64) * most < 256) return most;
     int64_t parts = 1;
     while (parts * 8 <= heads) parts *= 2;
     return parts;
@@ -1126,10 +1128,10 @@ struct Rotary {
     Tensor positions, frequencies;  // have no gradients
     int64_t tokens() const { return n * l; }
     std::vector<int64_t> shape(int64_t heads) const { return {n, l, heads, d}; }
-    SpioRotaryArgs args() const {
+    SpioRotaryArgs args(bool norm) const {
         SpioRotaryArgs a = {};
         a.positions = ptr(positions), a.frequencies = static_cast<const double*>(ptr(frequencies));
-        a.tokens = tokens(), a.q_heads = q_heads, a.k_heads = k_heads, a.parts = rotary_parts(std::max(q_heads, k_heads)), a.pairs = frequencies.numel();
+        a.tokens = tokens(), a.q_heads = q_heads, a.k_heads = k_heads, a.parts = rotary_parts(tokens(), std::max(q_heads, k_heads), d, norm), a.pairs = frequencies.numel();
         a.position_tokens = positions.numel(), a.wide_positions = positions.scalar_type() == at::kLong;
         a.eps = eps, a.scale = scale;
         return a;
@@ -1154,7 +1156,7 @@ variable_list rotary_forward(const Rotary& r, const Tensor& q, const Tensor& k, 
     const Heads qh = heads_of(q), kh = heads_of(k);
     const Tensor wq = whole(to_float_1d(q_weight)), wk = whole(to_float_1d(k_weight));
     const Tensor qo = empty_of(r.shape(r.q_heads), q.scalar_type(), q), ko = empty_of(r.shape(r.k_heads), k.scalar_type(), k);
-    SpioRotaryArgs a = r.args();
+    SpioRotaryArgs a = r.args(wq.defined());
     a.q = ptr(qh.t), a.q_row = qh.row, a.q_head = qh.head, a.k = ptr(kh.t), a.k_row = kh.row, a.k_head = kh.head;
     a.q_weight = floats(wq), a.k_weight = floats(wk), a.q_out = mut(qo), a.k_out = mut(ko);
     launch_structure(*rotary_plan(ROTARY, r, q, wq.defined()), rotary_grid(r.tokens(), a.parts, r.d, wq.defined(), false),
@@ -1209,7 +1211,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
         RECORD_FUNCTION("spio::head_norm_rotary_backward", tensors({gq, gk, q, k, wq, wk}));
         const Tensor gqc = whole(gq), gkc = whole(gk), wqf = whole(to_float_1d(wq)), wkf = whole(to_float_1d(wk));
         const Tensor dq = empty_of(gq.sizes(), type(6), gq), dk = empty_of(gk.sizes(), type(6), gk);
-        SpioRotaryArgs a = r.args();
+        SpioRotaryArgs a = r.args(norm);
         const int64_t grid = rotary_grid(r.tokens(), a.parts, r.d, norm, norm);
         Heads qh, kh;
         Tensor partials, dwq, dwk;

@@ -103,7 +103,7 @@ def head_norm_rotary_forward(
         return tuple(outputs)
     (qx, q_row, q_head), (kx, k_row, k_head) = _heads_of(q), _heads_of(k)
     norm = q_weight is not None
-    parts = parts_of(heads)
+    parts = parts_of(tokens, heads, d, norm)
     arguments = Arguments(STRUCT, **_fields(q, k, positions, frequencies, eps, scale), q=qx, k=kx, q_row=q_row, q_head=q_head,
                           k_row=k_row, k_head=k_head, q_weight=_weight(q_weight), k_weight=_weight(k_weight), q_out=outputs[0],
                           k_out=outputs[1], parts=parts)  # fmt: skip
@@ -135,7 +135,7 @@ def head_norm_rotary_backward(
     if tokens * heads == 0:
         return (*outputs, sums.zero_())
     fields = _fields(grad_q, grad_k, positions, frequencies, eps, scale)
-    parts = parts_of(heads)
+    parts = parts_of(tokens, heads, d, norm)
     grid = grid_of(tokens, parts, d, norm, norm)
     if norm:
         assert q.shape == grad_q.shape and k.shape == grad_k.shape and q.dtype == k.dtype == grad_q.dtype, "inputs of another norm"

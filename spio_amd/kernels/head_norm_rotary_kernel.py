@@ -22,11 +22,16 @@ def lanes_of(head: int, norm: bool) -> int:
     return divup(head, 16) if not norm else 1 << (divup(head, 16) - 1).bit_length()
 
 
-def parts_of(heads: int) -> int:
+def parts_of(tokens: int, heads: int, head: int, norm: bool) -> int:
     """Parts that the heads of a token are split into: lanes that share a token's cosines take every parts-th head.  A power
     of two, for four to seven heads a lane (us with 1, 2, 4 and 8 parts, forward: 2n 4097l 16 heads of 80 channels 35, 32,
     28, 27; 4n 2048l 24q 8k 128d with norms 37, 36, 37, 37, backward 50, 49, 48, 50; 1n 16385l 32q 8k 82, 75, 73, 73; 400
-    tokens, 24q 8k 14.0, 10.6, 9.6, 11.7)."""
+    tokens, 24q 8k 14.0, 10.6, 9.6, 11.7).  Two heads a lane where all lanes then are fewer waves than compute units, as
+    with one token a sequence (8n 12q 12k 64d with 2, 4, 6 parts 5.6, 5.0, 4.2; 8n 32q 8k 128d with norms, 8 and 16, 6.1 and
+    5.2)."""
+    most = divup(heads, 2)
+    if divup(tokens * lanes_of(head, norm), 64) * most < 256:
+        return most
     return 1 << max(0, (heads // 4).bit_length() - 1)
 
 

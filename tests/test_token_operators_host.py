@@ -213,8 +213,8 @@ def test_work_is_cut_alike_on_both_paths():
                     assert other.conv1d_slice(tokens, channels, sequences, backward) == slice_tokens(tokens, channels, sequences, backward)
         for heads in (1, 2, 9, 64):
             for head, norm in ((h, norm) for h in (8, 32, 80, 128, 256) for norm in (False, True)):
-                parts = parts_of(heads)
-                assert other.rotary_parts(heads) == parts and 1 <= parts <= heads
+                parts = parts_of(tokens, heads, head, norm)
+                assert other.rotary_parts(tokens, heads, head, norm) == parts and 1 <= parts <= heads
                 for summed in (False, True):
                     assert other.rotary_grid(tokens, parts, head, norm, summed) == grid_of(tokens, parts, head, norm, summed)
     for states in range(1, 33):
