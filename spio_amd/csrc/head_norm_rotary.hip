@@ -17,7 +17,10 @@
 // are a head, and a group of them has the same head numbers modulo `parts` of a token.  So cosines and sines are computed
 // once for all of these, and the sums of a norm cross lanes of a row only.  Angles are taken in turns in float64 (a
 // position of six digits leaves float32 no digits behind the turns), of which the fraction is exact in float32.
-// HBM-bound: 2 + 2 bytes a value forward, 2 + 2 + 2 backward for 16-bit types.
+// HBM-bound: 2 + 2 bytes a value forward, 2 + 2 + 2 backward with norms for 16-bit types.  4n 2048l, 24 and 8 heads of 128
+// channels with norms in bfloat16: forward 36 us (3.7 TB/s), backward 44 (4.6 TB/s), sums 4; 16385 tokens of 32 and 8 heads 71
+// (4.7 TB/s); 2n 4097l, 16 and 16 heads of 80 channels without, 28 and 26.  Without angles these are the same, without stores
+// 26 of 36 and 21 of 34, with one head a lane at once slower: it waits for memory, and most for what it reads.
 #include "spio_tokens.h"
 
 #ifndef SPIO_MODE
@@ -35,8 +38,8 @@ constexpr int GROUPS = 256 / LANES;      // of a workgroup
 constexpr int U = SPIO_HEADS;            // heads requested at once
 constexpr bool BACK = SPIO_MODE == 1;
 constexpr bool FULL = UNITS == 2 * LANES;  // no lane is without channels
-// Whether the first heads of a token are requested before its angles are computed: a backward pass with norms has no registers
-// for that
+// Whether the first heads of both tensors are requested before a token's angles are computed, or of k behind those of q: a
+// backward pass with norms has no registers for that (4n 2048l 24q 8k 128d 50 us, else 48)
 constexpr bool AHEAD = !(BACK && SPIO_NORM);
 static_assert(D % 8 == 0 && D <= 256, "heads of up to 256 channels, whole units");
 
@@ -112,7 +115,7 @@ struct Rows {
 };
 
 // U heads of a token as they are in memory: `head`, head + parts, ...; those behind the last one in the place of which that
-// is read.
+// is read, and the first unit in the place of none.  No branch is in the way, so that a wait is for what is needed alone.
 struct Batch {
     pw::Unit x[U][2], dy[U][2];
 };
@@ -189,6 +192,7 @@ __device__ inline void work_on(const Batch& b, const Rows& r, const Place& p, lo
         value_t* out = r.out + (token * r.heads + head + h * parts) * D;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
+            // (past the caches: 2n 4097l 16q 16k 80d 28 us, else 33)
             if (there && (FULL || p.unit[i] >= 0)) tk::store<true>(out + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
     }
 }
@@ -253,7 +257,8 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
         const int part = (int)(item % (unsigned)parts);
         const unsigned at = token < (unsigned)a.position_tokens ? token : token % (unsigned)a.position_tokens;
         // (requested before the heads: loads come back in their order.  Of an int64 the halves apart, of an int32 the one)
-        const int* slot = (const int*)a.positions + (unsigned long long)at * (unsigned)(1 + wide); const int low = slot[0], high = slot[wide];
+        const int* slot = (const int*)a.positions + (unsigned long long)at * (unsigned)(1 + wide);
+        const int low = slot[0], high = slot[wide];
         Batch q_heads, k_heads;
         request(q_heads, q, p, token, part, parts);
         if (AHEAD) request(k_heads, k, p, token, part, parts);

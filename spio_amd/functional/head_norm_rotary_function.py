@@ -6,7 +6,7 @@ without a norm of every head before it, in one pass over both tensors.
     the i-th pair (n1, n2) of a head becomes scale (n1 cos - n2 sin, n2 cos + n1 sin)
 
 Pair i is the channels (2i, 2i + 1) of a head with `interleaved`, else (i, pairs + i); channels behind the pairs stay as they
-are.  Angles are taken in float64 and there is no table of them: one is off by position * frequency * 2^-53 radians, and by 2^-24
+are.  Angles are taken in float64 and there is no table of them: one is off by position * frequency * 2^-52 radians, and by 2^-24
 turns, so that positions have no bound in practice.  Everything else is float32; the sum of a head's squares has to stay below
 its largest number (3.4e38).
 

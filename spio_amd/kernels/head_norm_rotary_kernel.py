@@ -14,7 +14,9 @@ from .launch_params import LaunchParams
 SOURCE = "head_norm_rotary.hip"
 MAX_HEAD = 256
 THREADS = 256
-SUMMED_WORKGROUPS = 512  # of a backward pass with norms, each of which leaves a row of sums
+# Workgroups of a backward pass with norms, each of which leaves a row of sums: two a compute unit (4n 2048l 24q 8k 128d 48 us,
+# with 1024 as long and twice the rows)
+SUMMED_WORKGROUPS = 512
 
 
 def lanes_of(head: int, norm: bool) -> int:
