@@ -18,9 +18,9 @@
 // once for all of these, and the sums of a norm cross lanes of a row only.  Angles are taken in turns in float64 (a
 // position of six digits leaves float32 no digits behind the turns), of which the fraction is exact in float32.
 // HBM-bound: 2 + 2 bytes a value forward, 2 + 2 + 2 backward with norms for 16-bit types.  4n 2048l, 24 and 8 heads of 128
-// channels with norms in bfloat16: forward 36 us (3.7 TB/s), backward 44 (4.6 TB/s), sums 4; 16385 tokens of 32 and 8 heads 71
-// (4.7 TB/s); 2n 4097l, 16 and 16 heads of 80 channels without, 28 and 26.  Without angles these are the same, without stores
-// 26 of 36 and 21 of 34, with one head a lane at once slower: it waits for memory, and most for what it reads.
+// channels with norms in bfloat16: forward 32 us (4.2 TB/s), backward 44 (4.6 TB/s), sums 4; 16385 tokens of 32 and 8 heads 71
+// (4.7 TB/s); 2n 4097l, 16 and 16 heads of 80 channels without, 30 each (2.9 TB/s).  Without angles these are the same, without stores
+// a forward pass of 36 takes 26 and one of 34 21: it waits for memory, and most for what it reads.
 #include "spio_tokens.h"
 
 #ifndef SPIO_MODE

@@ -28,9 +28,9 @@
 // What bounds it are vector instructions, for each state and token forward a product, an exponential (which takes a SIMD as
 // long as two others), a product and two multiply-adds, backward those and eight more, and one or two exponentials.  4n
 // 2048l 2048c with 16 states, gate and softplus in bfloat16, 64 chunks of each sequence's 32 tokens (us, and the share of the
-// time in which vector instructions issue): ends 71 (95 %), join 10, outputs with kept states 94 (82 %, 302 MB written), ends
-// back 68 (93 %), join 10, gradients 222 (83 %), sums 10; the tensors of all of these would move in 51.  Without chunks,
-// 128n 196l 768c: outputs 152, gradients 320; a prompt of 1n 4099l 1536c 33 + 11 + 40.
+// time in which vector instructions issue): ends 70 (95 %), join 10, outputs with kept states 93 (83 %, 302 MB written), ends
+// back 67 (93 %), join 11, gradients 218 (83 %), sums 11; the tensors of all of these would move in 51.  Without chunks,
+// 128n 196l 768c: outputs 146 (53 %), gradients 299 (74 %); a prompt of 1n 4099l 1536c 32 + 11 + 40.
 #include "spio_tokens.h"
 
 #ifndef SPIO_MODE
