@@ -28,7 +28,7 @@ def chunk_tokens(tokens: int, channels: int, sequences: int, backward: bool) -> 
     """Tokens of a chunk.  All of them where sequences and channels alone give most SIMDs a wave: a first pass over chunks
     costs as much as it brings then (forward, us whole and in chunks: 1024 waves 49 and 69, 1536 waves 115 and 142; backward
     1024 waves 138 and 134).  Else as many chunks as fill the device, whose SIMDs hold two waves of the backward pass,
-    once or, where chunks then keep 48 tokens, twice (4n 2048l 2048c backward: 2048 waves 241 us, 3072 253, 4096 217), but
+    once or, where chunks then keep 48 tokens, twice (4n 2048l 2048c backward: 2048 waves 241 us, 4096 217), but
     none of fewer than 16 tokens."""
     waves = divup(channels, LANES) * sequences
     if waves >= (1024 if backward else 700):
@@ -70,7 +70,8 @@ class SelectiveScanConfig:
 def _spec(mode, threads):
     def spec(params: SelectiveScanParams, config: SelectiveScanConfig, _device_attr=None) -> KernelSpec:
         params.validate()
-        defines = {"SPIO_MODE": mode, "SPIO_STATES": params.states, "SPIO_DTYPE": params.dtype, "SPIO_T": config.tile, "SPIO_HELD": config.held, "SPIO_WAVES": 2 if params.states <= 16 else 1, "SPIO_GATE": int(params.gate),
+        defines = {"SPIO_MODE": mode, "SPIO_STATES": params.states, "SPIO_DTYPE": params.dtype, "SPIO_T": config.tile,
+                   "SPIO_HELD": config.held, "SPIO_WAVES": 2 if params.states <= 16 else 1, "SPIO_GATE": int(params.gate),
                    "SPIO_SOFTPLUS": int(params.softplus), "SPIO_KEEP": int(params.keep)}  # fmt: skip
         return KernelSpec(defines, LaunchParams(grid=1, block=threads), SOURCE, takes_structure=True)
 
