@@ -14,6 +14,7 @@ from .launch_params import LaunchParams
 SOURCE = "selective_scan.hip"
 MAX_STATES = 32
 LANES = 64  # channels of a workgroup
+ENDS, OUT, ENDS_BACK = 0, 1, 2  # modes of the kernel
 
 
 def tile_tokens(states: int) -> int:
@@ -67,6 +68,13 @@ class SelectiveScanConfig:
     held: int = 0
 
 
+def _config(mode, params):
+    """The tile between kept states where these are written or read, else eight tokens (1n 4099l 1536c 73.0 us, with four 75.1)."""
+    if mode in (ENDS, ENDS_BACK) or (mode == OUT and not params.keep):
+        return SelectiveScanConfig(8)
+    return SelectiveScanConfig(tile_tokens(params.states), (3 - params.states % 2) * (8 < params.states <= 16))
+
+
 def _spec(mode, threads):
     def spec(params: SelectiveScanParams, config: SelectiveScanConfig, _device_attr=None) -> KernelSpec:
         params.validate()
@@ -84,7 +92,7 @@ def _factory(name, mode, threads):
         SelectiveScanConfig,
         None,
         kernel_name=name,
-        configs=lambda params, device_attr=None: [SelectiveScanConfig(tile_tokens(params.states), (3 - params.states % 2) * (8 < params.states <= 16))],
+        configs=lambda params, device_attr=None: [_config(mode, params)],
         kernel_spec=_spec(mode, threads),
         args_checker=None,
     )
