@@ -174,7 +174,8 @@ def causal_conv1d(
     inputs: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
     initial_state: Optional[torch.Tensor] = None, return_state: bool = False,
 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:  # fmt: skip
-    """act(convolution along the tokens), each channel by itself.
+    """act(convolution along the tokens), each channel by itself.  The state is that of the last tokens as they are: of
+    sequences padded behind it holds the padding.
 
     Args:
         inputs: (N, L, C) float16, bfloat16 or float32, C a multiple of 8; rows may be part of wider ones.

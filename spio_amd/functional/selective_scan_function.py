@@ -221,9 +221,13 @@ def selective_scan(
 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:  # fmt: skip
     """The selective scan of (N, L, C) inputs with S states a channel.
 
+    A token whose time step is zero (delta of minus infinity with softplus) leaves the states as they are: so sequences of
+    different lengths are padded, in front or behind.  With gradients the states before every fourth token (eighth with up to
+    eight states) are kept, in float32.
+
     Args:
         inputs, delta, gate: (N, L, C) float16, bfloat16 or float32, all of one type; rows may be part of wider ones.
-            `gate` is optional.
+            `gate` is optional.  C below 2^24.
         A: (C, S), S up to 32; negative where the states are to decay.  D, delta_bias: optional (C,).  Any float type.
         B, C: (N, L, S) in the inputs' type, the same for all channels.
         delta_softplus: softplus of delta (with its bias) instead of that itself.
