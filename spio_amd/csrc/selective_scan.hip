@@ -40,7 +40,7 @@
 namespace {
 
 constexpr int N = SPIO_STATES;
-constexpr int T = SPIO_T;                       // tokens of a tile, and between kept states
+constexpr int T = SPIO_T;                  // tokens of a tile, and between kept states where there are such
 constexpr int NP = (N + 3) / 4 * 4;        // states of a row in LDS, zeros behind the last one
 constexpr int M = 2 * N;                   // a token's B and C
 constexpr int STAGED = (T * N + 63) / 64;  // of a tile's B, a lane's, and of its C

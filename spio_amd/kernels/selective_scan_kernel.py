@@ -19,9 +19,8 @@ ENDS, OUT, ENDS_BACK = 0, 1, 2  # modes of the kernel
 
 def tile_tokens(states: int) -> int:
     """Tokens of a tile: those whose states the backward pass holds in registers at once, and the distance of the states
-    that the forward pass keeps for it.  Longer tiles keep less (4n 2048l 2048c with 16 states, forward: 98 us with 8 tokens,
-    124 with 4), but 16 states of five tokens and more have no room in half a SIMD's registers (backward: 239 us with 4
-    tokens, 275 with 5, 397 with 6, 542 with 8)."""
+    that the forward pass keeps for it.  Longer tiles keep less, but 16 states of five tokens and more have no room in half a
+    SIMD's registers (4n 2048l 2048c backward: 239 us with 4 tokens, 275 with 5, 397 with 6, 542 with 8)."""
     return 8 if states <= 8 else 4
 
 
