@@ -111,7 +111,7 @@ __device__ inline value_t load(pw_rsrc rs, unsigned lane_bytes, unsigned bytes) 
     return __builtin_bit_cast(value_t, __builtin_amdgcn_raw_buffer_load_b16(rs, (int)lane_bytes, (int)bytes, 0));
 #endif
 }
-// (The offset within the range is the lane's alone: it is what is compared with the end.)
+// (What may be behind the end is so by the lane's offset: the scalar one is not relied upon there.)
 __device__ inline void store(pw_rsrc rs, unsigned lane_bytes, value_t v) {
 #if SPIO_DTYPE == 2
     __builtin_amdgcn_raw_buffer_store_b32(pw::as_bits(v), rs, (int)lane_bytes, 0, 0);
@@ -396,8 +396,10 @@ SPIO_KERNEL_NAME(const Args a) {
     // (a state behind the last one, where they are odd: rate, B and C of zero)
     auto state = [&](int i) { return half * H + i < N ? half * H + i : N - 1; };
     auto there = [&](int i) { return half * H + i < N; };
-    // Rows of states [N][channels]: bytes from row i to the lane's state i of a channel.  What is not there, a state behind the
-    // last one or a channel, lies behind the end, where zeros are loaded.
+    // Rows of states [N][channels]: bytes from row i to the lane's state i of a channel.  What is not there, a channel or a state
+    // behind the last one (of the upper half, where they are odd), is behind the end by the lane's offset alone: zeros are loaded
+    // there, stores dropped.  (The device counts the scalar offset of row i against the end as well, but the builtin does not promise
+    // that.)
     unsigned offset[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -406,8 +408,9 @@ SPIO_KERNEL_NAME(const Args a) {
     }
     const int row_bytes = (int)a.channels * 4;
     auto states = [&](const float* rows) { return pw::buffer(rows, N * (unsigned)row_bytes); };
+    auto offset_of = [&](int c, int i) { return (int)(N % 2 && i == H - 1 && half ? pw::OOB : offset[c]); };
     auto load_state = [&](pw_rsrc rs, int c, int i) {
-        return pw::as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, (int)offset[c], i * row_bytes, 0));
+        return pw::as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, offset_of(c, i), i * row_bytes, 0));
     };
     float A2[2][H], r[2][H], dA[2][H];
 #pragma unroll
@@ -539,7 +542,7 @@ SPIO_KERNEL_NAME(const Args a) {
     for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < H; ++i)
-            __builtin_amdgcn_raw_buffer_store_b32(pw::as_bits(dA[c][i]), to_dA, (int)offset[c], i * row_bytes, 0);
+            __builtin_amdgcn_raw_buffer_store_b32(pw::as_bits(dA[c][i]), to_dA, offset_of(c, i), i * row_bytes, 0);
     if (!p.live) return;
     sums[N * a.channels + p.channel] = dD;
     sums[(N + 1) * a.channels + p.channel] = dbias;
