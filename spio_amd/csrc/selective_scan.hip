@@ -608,8 +608,11 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
             const int i = first + k;
             if (i >= chunks) break;
             ends[((BACK ? chunks - 1 - i : i) * (N + 1) + s) * a.channels] = v;
-            // (nothing stays nothing, also where the states grow so much that the factor is infinite)
-            v = v == 0.f ? end[k] : __builtin_fmaf(exp2_(sum[k] * A2), v, end[k]);
+            // The factor's whole powers of two go into v first: by itself it may be infinite, or zero, where its product with
+            // a small, or a large, v is not.  (They are bounded, as v's are; nothing stays nothing at an infinite factor.)
+            const float power = sum[k] * A2;
+            const int whole = (int)__builtin_amdgcn_fmed3f(power, -400.f, 400.f);
+            v = v == 0.f ? end[k] : __builtin_fmaf(exp2_(power - (float)whole), __builtin_ldexpf(v, whole), end[k]);
         }
     }
 }

@@ -5,7 +5,9 @@ import pytest
 import torch
 
 from spio_amd.functional.selective_scan_function import selective_scan_backward, selective_scan_forward
-from tests.test_selective_scan_gpu import FLOAT, _tensors
+from spio_amd.kernels.selective_scan_kernel import chunk_tokens
+from tests import token_reference as ref
+from tests.test_selective_scan_gpu import FLOAT, NAMES, _tensors, _train
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +26,26 @@ def test_what_lies_behind_the_kept_states_is_not_read(s):
     got = selective_scan_backward(dy, *t.values(), True, part)
     assert all(a.isfinite().all() and torch.equal(a, b) for a, b in zip(got, expected))
     assert memory[kept.numel() :].isnan().all()
+
+
+def test_chunks_whose_factor_no_number_holds():
+    """Three chunks of 16 tokens, the states of which grow or decay by e^100 in the middle one: from 1e-30 and from 1e30 to numbers
+    that are there, though the factor is not; gradients the same way back."""
+    n, l, c, s = 1, 48, 2, 1
+    assert [chunk_tokens(l, c, n, backward) for backward in (False, True)] == [16, 16]
+    delta = torch.full((n, l, c), 1.0 / 64, device="cuda")
+    delta[:, 16:32] = 6.25
+    t = {"u": torch.zeros(n, l, c, device="cuda"), "delta": delta, "A": torch.tensor([[1.0], [-1.0]], device="cuda"),
+         "B": torch.ones(n, l, s, device="cuda"), "C": torch.full((n, l, s), 0.75, device="cuda"), "D": None, "gate": None, "bias": None}  # fmt: skip
+    before = torch.tensor([[[1e-30], [1e30]]], device="cuda")
+    dy = torch.tensor([1e-30, 1e30], device="cuda").expand(n, l, c).contiguous()
+    dy[:, :32] = 0.0
+    expected = ref.scan(*t.values(), False, before, dy)
+    got = _train(t, False, before, dy)
+    # exponents of 100.5 in all: a product, a rate and a sum of time steps of them are off by half a unit each
+    terms = 3 * l + s + 80 + 2 * 101
+    ref.check("y", got["y"], *expected[0], terms)
+    for i, name in enumerate(NAMES):
+        if t[name] is not None:
+            ref.check("d" + name, got["d" + name], *expected[2 + i], 2 * terms + l)
+    assert got["y"][0, 40, 0] > 1e13 and 0 < got["y"][0, 40, 1] < 1e-12 and got["du"][0, 3, 0] > 1e11 and 0 < got["du"][0, 3, 1] < 1e-12
