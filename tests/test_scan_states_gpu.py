@@ -4,10 +4,11 @@ partner in the other half of a wave, those of other tiles, and idle lanes of a s
 import pytest
 import torch
 
+from spio_amd.functional import selective_scan, selective_scan_step
 from spio_amd.functional.selective_scan_function import selective_scan_backward, selective_scan_forward
 from spio_amd.kernels.selective_scan_kernel import chunk_tokens
 from tests import token_reference as ref
-from tests.test_selective_scan_gpu import FLOAT, NAMES, _tensors, _train
+from tests.test_selective_scan_gpu import BF16, FLOAT, HALF, NAMES, _tensors, _train
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +50,45 @@ def test_chunks_whose_factor_no_number_holds():
         if t[name] is not None:
             ref.check("d" + name, got["d" + name], *expected[2 + i], 2 * terms + l)
     assert got["y"][0, 40, 0] > 1e13 and 0 < got["y"][0, 40, 1] < 1e-12 and got["du"][0, 3, 0] > 1e11 and 0 < got["du"][0, 3, 1] < 1e-12
+
+
+# Numbers of states with code of their own: tiles of eight tokens (up to 8 states) and of four; last decays held (9 to 16, odd
+# ones one fewer) or none; one wave a SIMD (17 and more); odd ones; partly filled sums over lanes.  Lengths that end inside a
+# tile, channels of parts of a wave; several chunks, and (more than 1023 sequences) one.
+STATES = [
+    (2, 37, 33, 8, FLOAT, True), (1, 85, 70, 9, FLOAT, True), (2, 41, 33, 12, BF16, False), (1, 67, 70, 15, FLOAT, True),
+    (2, 35, 33, 17, FLOAT, True), (1, 53, 70, 31, HALF, False), (1, 50, 33, 3, FLOAT, True), (2, 39, 70, 21, FLOAT, False),
+    (1025, 5, 33, 9, FLOAT, True), (1025, 7, 3, 15, FLOAT, False), (1025, 5, 33, 17, FLOAT, True), (1025, 11, 5, 8, FLOAT, False),
+    (1025, 6, 5, 31, FLOAT, True), (1025, 9, 5, 12, HALF, False),
+]  # fmt: skip
+
+
+@pytest.mark.parametrize("n,l,c,s,dtype,softplus", STATES)
+def test_outputs_and_gradients(n, l, c, s, dtype, softplus):
+    t, before, dy = _tensors(n, l, c, s, dtype, softplus, True, True, softplus, True)
+    assert (chunk_tokens(l, c, n, True) < l) == (n < 1024)
+    expected = ref.scan(*t.values(), softplus, before, dy)
+    got = _train(t, softplus, before, dy)
+    # as for other numbers of states: three roundings a token in a state, sums over states; over channels in 32 bits; over a
+    # chunk's tokens in 32 and the chunks' in 64
+    terms = 3 * l + s + 80
+    ref.check("y", got["y"], *expected[0], terms)
+    for i, name in enumerate(NAMES):
+        if t[name] is not None:
+            more = c if name in "BC" else l if name in ("A", "D", "bias") else 0
+            ref.check("d" + name, got["d" + name], *expected[2 + i], 2 * terms + more)
+    with torch.no_grad():
+        plain, after = selective_scan(*t.values(), softplus, before, return_state=True)
+    ref.check("y without gradients", plain, *expected[0], terms)
+    ref.check("state", after, *expected[1], terms)
+
+
+@pytest.mark.parametrize("s,dtype", [(12, BF16), (17, FLOAT), (20, FLOAT), (3, HALF), (28, FLOAT)])
+def test_step(s, dtype):
+    """Lanes without states beside whole ones (12, 20, 28 states: three, five and seven of four and eight) and parts of one."""
+    t, before, _ = _tensors(5, 1, 37, s, dtype, state=True)
+    expected = ref.scan(*t.values(), True, before, None)
+    u, *rest = [v if v is None or v.dim() < 3 else v[:, 0] for v in t.values()]
+    y = selective_scan_step(u, before, *rest, True)
+    ref.check("y", y, expected[0][0][:, 0], expected[0][1][:, 0], s + 80)
+    ref.check("state", before, *expected[1], 80)
