@@ -1730,7 +1730,7 @@ PyObject* head_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs, P
     if (q.numel() == 0 || k.numel() == 0 || r.tokens() * std::max(r.q_heads, r.k_heads) >= int64_t(1) << 31 ||
         !fits(k, q, r.shape(r.k_heads), true) || r.d % 8 || r.d > ROTARY_MAX_HEAD ||
         wq.defined() != wk.defined() || !absent_or_fits(wq, q, {r.d}, false) || !absent_or_fits(wk, q, {r.d}, false) ||
-        !(r.eps > 0) || r.eps > std::numeric_limits<double>::max() || !std::isfinite(r.scale) || pairs < 1 || 2 * pairs > r.d ||
+        !(r.eps > 0) || r.eps > std::numeric_limits<double>::max() || !(std::fabs(r.scale) <= std::numeric_limits<float>::max()) || pairs < 1 || 2 * pairs > r.d ||
         (!r.interleaved && pairs % 8) || r.frequencies.scalar_type() != at::kDouble || wants_grad(r.frequencies) || r.frequencies.device() != q.device() ||
         !is_plain(r.positions) || (r.positions.scalar_type() != at::kLong && r.positions.scalar_type() != at::kInt) ||
         r.positions.device() != q.device() ||

@@ -48,7 +48,7 @@ def _check(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, s
     check_parameters(what, q, q_weight=(q_weight, (d,)), k_weight=(k_weight, (d,)))
     assert (q_weight is None) == (k_weight is None), "weights of both norms or of none"
     assert q_weight is None or 0 < eps < float("inf"), "eps must be positive and finite"
-    assert math.isfinite(scale), "scale must be finite"
+    assert abs(scale) <= torch.finfo(torch.float32).max, "scale must be a finite float32 number"
     assert frequencies.dim() == 1 and frequencies.dtype == torch.float64, "frequencies are float64 [pairs]"
     pairs = frequencies.shape[0]
     assert 0 < pairs and 2 * pairs <= d, "a head has two channels for every frequency"
@@ -220,7 +220,7 @@ def rotary(
         frequencies: (pairs,) float64, radians a position (`rotary_frequencies`); 2 * pairs channels of a head are turned.
             Without `interleaved` a multiple of 8.
         interleaved: pairs are neighbouring channels instead of one of each half.
-        scale: factor of the turned channels.
+        scale: factor of the turned channels, a finite float32 number.
 
     Returns:
         Queries and keys of the same shapes and type, without gaps.
