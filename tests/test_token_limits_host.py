@@ -4,6 +4,8 @@ import pytest
 import torch
 
 from spio_amd.functional import head_norm_rotary, rotary, rotary_frequencies
+from spio_amd.kernels.causal_conv1d_kernel import slice_tokens
+from spio_amd.util.math import divup
 
 Q, W, POSITIONS, FREQUENCIES = torch.zeros(2, 5, 4, 32), torch.ones(32), torch.arange(5), rotary_frequencies(32)
 
@@ -21,3 +23,12 @@ def test_scales_that_are_no_float32_numbers_are_refused(scale):
 def test_smallest_and_largest_scales_are_taken(scale):
     with pytest.raises(ValueError, match="GPU only"):
         rotary(Q, Q, POSITIONS, FREQUENCIES, scale=scale)
+
+
+def test_rows_of_filter_sums():
+    """Fewer than 4096 and the sequences together, and one at least of each."""
+    for tokens in (1, 2, 3, 16, 17, 513, 2048, 4099, 100000, 5000000):
+        for sequences in (1, 2, 127, 128, 4095, 4096, 8192, 65536):
+            for channels in (8, 200, 2048):
+                rows = sequences * divup(tokens, slice_tokens(tokens, channels, sequences, True))
+                assert sequences <= rows < 4096 + sequences, (tokens, sequences, channels, rows)
