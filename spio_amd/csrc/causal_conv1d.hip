@@ -12,7 +12,7 @@
 // inputs, and backward the last dz, in registers, so that every tensor is read once but for the W - 1 tokens beside a
 // slice.  Neighbouring lanes have neighbouring channels, then the next slice.  HBM-bound: 2 + 2 bytes a value forward,
 // 2 + 2 + 2 backward for 16-bit types.  8n 2048l 2048c, four taps and silu in bfloat16: forward 28 us (5.0 TB/s), backward 44
-// (5.4 TB/s; vector instructions issue in 80 % of it), sums 5; a prompt of 2051 tokens of 1536 channels 6.5, a token 2.1, which
+// (5.4 TB/s; vector instructions issue in 79 % of it), sums 5; a prompt of 2051 tokens of 1536 channels 6.7, a token 2.2, which
 // is what a launch takes.
 #include "spio_tokens.h"
 

@@ -18,9 +18,11 @@
 // once for all of these, and the sums of a norm cross lanes of a row only.  Angles are taken in turns in float64 (a
 // position of six digits leaves float32 no digits behind the turns), of which the fraction is exact in float32.
 // HBM-bound: 2 + 2 bytes a value forward, 2 + 2 + 2 backward with norms for 16-bit types.  4n 2048l, 24 and 8 heads of 128
-// channels with norms in bfloat16: forward 32 us (4.2 TB/s), backward 44 (4.6 TB/s), sums 4; 16385 tokens of 32 and 8 heads 71
-// (4.7 TB/s); 2n 4097l, 16 and 16 heads of 80 channels without, 30 each (2.9 TB/s).  Without angles these are the same, without stores
-// a forward pass of 36 takes 26 and one of 34 21: it waits for memory, and most for what it reads.
+// channels with norms in bfloat16: forward 32 us (4.2 TB/s), backward 44 (4.6 TB/s; vector instructions issue in half of it), sums 4;
+// 16385 tokens of 32 and 8 heads 73 (4.6 TB/s); 2n 4097l, 16 and 16 heads of 80 channels without, 29 and 30 (3.0 TB/s), twice what a
+// copy takes: there is one item for each group of lanes, so that all of them read, turn and write at about the same time.  Traced, of
+// two sets of tensors in turn; back to back over five sets 37, 48, 73 and 28.  It waits for memory, most for what it reads:
+// without angles the passes took as long, without stores one of 36 us took 26.
 #include "spio_tokens.h"
 
 #ifndef SPIO_MODE
@@ -39,7 +41,7 @@ constexpr int U = SPIO_HEADS;            // heads requested at once
 constexpr bool BACK = SPIO_MODE == 1;
 constexpr bool FULL = UNITS == 2 * LANES;  // no lane is without channels
 // Whether the first heads of both tensors are requested before a token's angles are computed, or of k behind those of q: a
-// backward pass with norms has no registers for that (4n 2048l 24q 8k 128d 50 us, else 48)
+// backward pass with norms has no registers for that (4n 2048l 24q 8k 128d 51 us, else 48)
 constexpr bool AHEAD = !(BACK && SPIO_NORM);
 static_assert(D % 8 == 0 && D <= 256, "heads of up to 256 channels, whole units");
 
@@ -192,7 +194,7 @@ __device__ inline void work_on(const Batch& b, const Rows& r, const Place& p, lo
         value_t* out = r.out + (token * r.heads + head + h * parts) * D;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            // (past the caches: 2n 4097l 16q 16k 80d 28 us, else 33)
+            // (past the caches: 2n 4097l 16q 16k 80d 28 us, else 34)
             if (there && (FULL || p.unit[i] >= 0)) tk::store<true>(out + p.unit[i] * 8, pw::pack(BACK ? g[i] : v[i]));
     }
 }

@@ -27,10 +27,11 @@
 //
 // What bounds it are vector instructions, for each state and token forward a product, an exponential (which takes a SIMD as
 // long as two others), a product and two multiply-adds, backward those and eight more, and one or two exponentials.  4n
-// 2048l 2048c with 16 states, gate and softplus in bfloat16, 64 chunks of each sequence's 32 tokens (us, and the share of the
-// time in which vector instructions issue): ends 70 (95 %), join 10, outputs with kept states 93 (83 %, 302 MB written), ends
-// back 67 (93 %), join 11, gradients 218 (83 %), sums 11; the tensors of all of these would move in 51.  Without chunks,
-// 128n 196l 768c: outputs 146 (53 %), gradients 299 (74 %); a prompt of 1n 4099l 1536c 32 + 11 + 40.
+// 2048l 2048c with 16 states, gate and softplus in bfloat16, each sequence in 32 chunks of 64 tokens (us traced, and the share of the
+// time in which vector instructions issue): ends 70 (98 %), join 11, outputs with kept states 94 (83 %, and 427 MB at 4.6
+// TB/s, of which 268 are kept states: memory as much as instructions), ends back 68 (96 %), join 11, gradients 231 (84 %), sums
+// 11; the tensors of all of these would move in 46.  Without chunks, 128n 196l 768c: outputs 151 (53 %), gradients 315 (74 %),
+// 1536 waves on 1024 SIMDs; a prompt of 1n 4099l 1536c in 74 chunks 30 (74 %) + 12 + 38 (72 %).
 #include "spio_tokens.h"
 
 #ifndef SPIO_MODE
@@ -579,8 +580,8 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))
 #elif SPIO_MODE == 6 || SPIO_MODE == 7
 
 // A lane is a state of a channel, and goes from chunk to chunk, v = exp(A sum dl) v + end, leaving v in the place of the
-// end.  The ends of JOINED chunks are requested at once: waiting for memory is all that it does (4n 2048l 2048c training, all
-// launches, with 4, 8, 16 and 32 at once: 484, 454, 482 and 509 us).
+// end.  The ends of JOINED chunks are requested at once: waiting for memory is all that it does (4n 2048l 2048c, 32 chunks, with 4, 8,
+// 16 and 32 at once 8.9, 8.7, 10.7 and 26 us; 1n 4099l 1536c, 74 chunks, 11.0, 10.9, 14.5 and 28).
 extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) SPIO_KERNEL_NAME(const Args a) {
     constexpr bool BACK = SPIO_MODE == 7;
     constexpr int JOINED = 8;
@@ -619,7 +620,7 @@ extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(64, 64))) 
 
 #else
 
-// (64n 1536c 16 states 5.0 us: 2.2 a launch takes, 13.6 MB in the rest)
+// (64n 1536c 16 states 5.1 us: 2.2 a launch takes, 13.6 MB in the rest)
 // One token: a lane has four states of a channel, so that a wave's loads of states are whole lines; the lanes of a channel
 // (a power of two) add their parts of y.
 extern "C" __global__ void __attribute__((amdgpu_flat_work_group_size(256, 256))) SPIO_KERNEL_NAME(const Args a) {

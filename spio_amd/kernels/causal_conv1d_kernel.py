@@ -19,8 +19,8 @@ UNROLL = 4
 
 def slice_tokens(tokens: int, channels: int, sequences: int, backward: bool) -> int:
     """Tokens that a lane walks along: as many as leave 2^17 lanes, from 4 to 32, or 16 to 256 backward, where a lane also leaves
-    a row of sums and reads the tokens beside its slice again (us: 8n 2048l 2048c forward with 4, 8, 16, 32, 64 tokens 39, 30, 28,
-    25, 24, backward with 16, 32, 64, 128 60, 53, 51, 78; 1n 2051l 1536c forward with 4, 16, 32 8.1, 8.6, 12.1); and so many
+    a row of sums and reads the tokens beside its slice again (us: 8n 2048l 2048c forward with 4, 8, 16, 32, 64 tokens 40, 30, 28,
+    25, 24, backward with 16, 32, 64, 128 60, 53, 50, 81; 1n 2051l 1536c forward with 4, 8, 16, 32 8.2, 7.8, 8.7, 12.1); and so many
     that there are fewer rows of sums than 4096 and the sequences together, of which each leaves one at least: a lane stays
     within its sequence."""
     lanes = channels // 8 * sequences

@@ -26,9 +26,9 @@ def lanes_of(head: int, norm: bool) -> int:
 
 def parts_of(tokens: int, heads: int, head: int, norm: bool) -> int:
     """Parts that the heads of a token are split into: lanes that share a token's cosines take every parts-th head.  A power
-    of two, for four to seven heads a lane (us with 1, 2, 4 and 8 parts, forward: 2n 4097l 16 heads of 80 channels 35, 32,
-    28, 27; 4n 2048l 24q 8k 128d with norms 37, 36, 37, 37, backward 50, 49, 48, 50; 1n 16385l 32q 8k 82, 75, 73, 73; 400
-    tokens, 24q 8k 14.0, 10.6, 9.6, 11.7).  Two heads a lane where all lanes then are fewer waves than compute units, as
+    of two, for four to seven heads a lane (us with 1, 2, 4 and 8 parts, forward: 2n 4097l 16 heads of 80 channels 34, 32,
+    28, 28; 4n 2048l 24q 8k 128d with norms 37, 36, 37, 38, backward 49, 49, 48, 51; 1n 16385l 32q 8k 81, 74, 73, 73; 400
+    tokens, 24q 8k 13.9, 10.4, 9.6, 11.7).  Two heads a lane where all lanes then are fewer waves than compute units, as
     with one token a sequence (8n 12q 12k 64d with 2, 4, 6 parts 5.6, 5.0, 4.2; 8n 32q 8k 128d with norms, 8 and 16, 6.1 and
     5.2)."""
     most = divup(heads, 2)
@@ -61,7 +61,7 @@ class HeadNormRotaryParams:
 @dataclass(frozen=True)
 class HeadNormRotaryConfig:
     """Heads that a lane requests at once (4n 2048l 24q 8k 128d with norms, forward and backward, us: one 39 and 49, two 37 and
-    48, four 38 and 57)."""
+    48, four 38 and 60)."""
 
     heads: int = 2
 
