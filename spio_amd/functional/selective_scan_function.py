@@ -222,8 +222,8 @@ def selective_scan(
     """The selective scan of (N, L, C) inputs with S states a channel.
 
     A token whose time step is zero (delta of minus infinity with softplus) leaves the states as they are: so sequences of
-    different lengths are padded, in front or behind.  Its inputs and B (and C, with gradients) have to be finite: zero times
-    what is not is NaN.  With gradients the states before every fourth token (eighth with up to eight states) are kept, in
+    different lengths are padded, in front or behind.  Its inputs and B, with gradients also C, gate and grad_output, have to be
+    finite: zero times what is not is NaN.  With gradients the states before every fourth token (eighth with up to eight states) are kept, in
     float32.
 
     Args:
