@@ -223,8 +223,8 @@ def selective_scan(
 
     A token whose time step is zero (delta of minus infinity with softplus) leaves the states as they are: so sequences of
     different lengths are padded, in front or behind.  Its inputs and B, with gradients also C, gate and grad_output, have to be
-    finite: zero times what is not is NaN.  With gradients the states before every fourth token (eighth with up to eight states) are kept, in
-    float32.
+    finite: zero times what is not is NaN.  With gradients the states before every fourth token (eighth with up to eight states)
+    are kept, in float32.
 
     Args:
         inputs, delta, gate: (N, L, C) float16, bfloat16 or float32, all of one type; rows may be part of wider ones.
